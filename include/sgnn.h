@@ -534,6 +534,76 @@ int sgnn_edge_rows_to_tiles(const float* e, int64_t ld, int32_t width, const int
 int sgnn_edge_tiles_to_rows(const float* e0t, int32_t width, const int32_t* perm, const int32_t* rowptr, int64_t n,
                             int64_t num_edges, float scale, float* out, int64_t ld, int32_t accumulate, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Typed operators (linear.hip, norm.hip, muon.hip): the Linear, LayerNorm and
+ * optimiser steps of an MLP block in fp32, bf16 or fp16, at any sizes and
+ * alignment.  Every sum, statistic and state is held in fp32; a 16-bit output
+ * is rounded once, to nearest even.  Deterministic: no float atomics, and the
+ * summation order depends on the sizes alone.  NaN and infinity propagate.
+ * `dtype` is an sgnn_dtype; pointers to its elements are aligned to one
+ * element, leading dimensions (ld) are in elements; "dense" means ld = width.
+ * ------------------------------------------------------------------------- */
+typedef enum sgnn_dtype { SGNN_F32 = 0, SGNN_BF16 = 1, SGNN_F16 = 2 } sgnn_dtype;
+typedef enum sgnn_act {
+  SGNN_ACT_NONE = 0,
+  SGNN_ACT_RELU = 1,      /* slope 0 at z = 0 */
+  SGNN_ACT_GELU = 2,      /* z (1 + erf(z / sqrt 2)) / 2 */
+  SGNN_ACT_GELU_TANH = 3, /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+  SGNN_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+} sgnn_act;
+
+/* y[M][N] = act(z) (+ residual), z = x[M][K] w[N][K]^T (+ bias[N]): one nn.Linear of build_mlp
+ * (graph_network.py:7-45) with its activation and the block's residual (:176) in the epilogue.
+ * bias, residual and z may be NULL; z (dense [M][N]) receives the pre-activation values the backward pass
+ * reads.  K = 0 gives z = bias.  y and z may overlap no input; residual may be y itself.
+ * workspace: sgnn_linear_workspace_bytes(dtype, M, N, K) bytes, 256-B aligned. */
+size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K);
+int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
+                int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* z, void* y,
+                int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+/* Its backward pass from dy [M][N]: dz = dy act'(z), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = sum_m dz
+ * (all dense; NULL skips one; the residual's gradient is dy).  z (dense) as saved by sgnn_linear; for
+ * SGNN_ACT_RELU the output y of a call without residual serves as well; not read for SGNN_ACT_NONE.
+ * 16-bit types: dz is rounded once to the type before the two products, as their matrix instructions read it;
+ * db sums the unrounded values.  M = 0 gives dw = db = 0.
+ * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, act) bytes, 256-B aligned. */
+size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act);
+int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const void* z,
+                    int32_t act, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw,
+                    void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y[n][width] = (x - mean) rstd gamma + beta (+ residual) per row, rstd = 1 / sqrt(var + eps) with the biased
+ * variance (nn.LayerNorm, graph_network.py:86-96), x and residual rows at ldx / ldr, y dense.  gamma, beta and
+ * residual may be NULL; gamma and beta are of type wdtype (dtype, or SGNN_F32).  mean / rstd [n] fp32 receive
+ * the row statistics when not NULL.  y may be x (when x is dense) or the residual. */
+int sgnn_norm(int32_t dtype, int32_t wdtype, const void* x, int64_t ldx, int64_t n, int32_t width, const void* gamma,
+              const void* beta, const void* residual, int64_t ldr, float eps, void* y, float* mean, float* rstd,
+              void* stream);
+/* Its backward pass: dx (dense) = rstd (g - mean(g) - xhat mean(g xhat)), g = dy gamma, and in the same pass
+ * over the rows dgamma[c] = sum_r dy xhat, dbeta[c] = sum_r dy (type wdtype).  dx, dgamma, dbeta may be NULL.
+ * n = 0 gives dgamma = dbeta = 0.  workspace: sgnn_norm_bwd_workspace_bytes(n, width) bytes, 256-B aligned. */
+size_t sgnn_norm_bwd_workspace_bytes(int64_t n, int32_t width);
+int sgnn_norm_bwd(int32_t dtype, int32_t wdtype, const void* dy, int64_t ldd, const void* x, int64_t ldx,
+                  const float* mean, const float* rstd, const void* gamma, int64_t n, int32_t width, void* dx,
+                  void* dgamma, void* dbeta, void* workspace, size_t workspace_bytes, void* stream);
+
+/* One matrix of sgnn_newton_schulz: `in` [rows][cols] at ld_in, `out` at ld_out (may be `in`). */
+typedef struct sgnn_matrix {
+  const void* in; void* out;
+  int64_t ld_in, ld_out;
+  int32_t rows, cols;
+} sgnn_matrix;
+/* out = the orthogonalised in, per matrix: X = in / (|in|_F + eps), then `steps` times
+ * X <- a X + (b G + c G^2) X with G = X X^T (X transposed first where rows > cols): every singular value s of
+ * in / |in|_F goes through s <- a s + b s^3 + c s^5, which for (3.4445, -4.7750, 2.0315) brings it near 1 in
+ * five steps (the update of the Muon optimiser).  `mats` is a HOST array of `count` matrices of any shapes
+ * (read during the call only); matrices of one shape that stand next to each other share their launches.
+ * Zero matrices give zeros.  Products are formed to fp32 accuracy whatever the type.
+ * workspace: sgnn_newton_schulz_workspace_bytes(mats, count) bytes (reads the shapes alone), 256-B aligned. */
+size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, int32_t count);
+int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_t count, int32_t steps, float a, float b,
+                       float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

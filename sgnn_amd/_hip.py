@@ -72,7 +72,14 @@ class SgnnReduceDesc(ctypes.Structure):
                 ("scale", c_float)]
 
 
+class SgnnMatrix(ctypes.Structure):
+    """struct sgnn_matrix (include/sgnn.h)."""
+    _fields_ = [("in_", c_void_p), ("out", c_void_p), ("ld_in", c_int64), ("ld_out", c_int64), ("rows", c_int32),
+                ("cols", c_int32)]
+
+
 P_SAVES = ctypes.POINTER(SgnnSaves)
+P_MATRIX = ctypes.POINTER(SgnnMatrix)
 SLAB_EDGE, SLAB_NODE, SLAB_UV, SLAB_DECODER, SLAB_ENC_NODE, SLAB_ENC_EDGE = range(6)
 
 # name -> (restype, argtypes); every symbol include/sgnn.h declares
@@ -191,7 +198,28 @@ SIGNATURES = {
                                              c_void_p, c_int64, c_int32, c_void_p]),
     "sgnn_edge_rows_to_tiles": (ctypes.c_int, [c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_int64, c_int64,
                                                c_void_p, c_void_p]),
+    "sgnn_linear_workspace_bytes": (ctypes.c_size_t, [c_int32, c_int64, c_int64, c_int64]),
+    "sgnn_linear": (ctypes.c_int, [c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                   c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, ctypes.c_size_t,
+                                   c_void_p]),
+    "sgnn_linear_bwd_workspace_bytes": (ctypes.c_size_t, [c_int32, c_int64, c_int64, c_int64, c_int32]),
+    "sgnn_linear_bwd": (ctypes.c_int, [c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32,
+                                       c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+                                       ctypes.c_size_t, c_void_p]),
+    "sgnn_norm": (ctypes.c_int, [c_int32, c_int32, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
+                                 c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "sgnn_norm_bwd_workspace_bytes": (ctypes.c_size_t, [c_int64, c_int32]),
+    "sgnn_norm_bwd": (ctypes.c_int, [c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                     c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_void_p,
+                                     ctypes.c_size_t, c_void_p]),
+    "sgnn_newton_schulz_workspace_bytes": (ctypes.c_size_t, [P_MATRIX, c_int32]),
+    "sgnn_newton_schulz": (ctypes.c_int, [c_int32, P_MATRIX, c_int32, c_int32, c_float, c_float, c_float, c_float,
+                                          c_void_p, ctypes.c_size_t, c_void_p]),
 }
+
+# sgnn_dtype / sgnn_act (include/sgnn.h)
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 _LIB: Optional[ctypes.CDLL] = None
 

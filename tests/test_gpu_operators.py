@@ -1,0 +1,570 @@
+"""functional.linear, functional.layer_norm and muon.newton_schulz against plain
+implementations in 64 bits.
+
+Tolerances are counted from the arithmetic, with u = 2^-24 (half a step of fp32)
+and h = finfo(type).eps / 2 (half a step of the output's type):
+  * a sum of K products in fp32 is off by at most (K + 2) u times the sum of the
+    products' magnitudes; an affine or activation step adds a few u of its operands;
+  * a 16-bit output adds h of its value; values kept in 16 bits between the two
+    passes (z, dz) add h of themselves, carried on by the slopes.
+Inputs that are small whole numbers make every sum exact: those tests ask for equal
+values, so a wrong index, edge or stride cannot hide in a tolerance."""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+IDS = ["f32", "bf16", "f16"]
+ACTS = ["none", "relu", "gelu", "gelu_tanh", "silu"]
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def rounded(t, ref):
+    """The most by which rounding to t moves ref: half a step of its value, and below the type's smallest normal number
+    half of the subnormals' one step, smallest_normal * eps / 2 (fp16: 2^-14 * 2^-10 / 2 = 2^-25)."""
+    return half_step(t) * ref.abs() + torch.finfo(t).smallest_normal * half_step(t)
+
+
+def act64(z, act):
+    f = torch.nn.functional
+    return {"none": lambda v: v, "relu": f.relu, "gelu": f.gelu, "gelu_tanh": lambda v: f.gelu(v, approximate="tanh"),
+            "silu": f.silu}[act](z)
+
+
+def within(got, ref, tol, what):
+    got = got.detach().double().cpu()
+    assert got.shape == ref.shape, what
+    over = (got - ref).abs() - tol
+    assert not torch.isnan(over).any() and float(over.max() if over.numel() else 0.0) <= 0.0, (
+        f"{what}: worst |difference| {float((got - ref).abs().max()):.3e} at tolerance "
+        f"{float(torch.as_tensor(tol).max()):.3e}")
+
+
+def whole(shape, seed, low=-2, high=3, dtype=torch.float32):
+    return torch.from_numpy(np.random.default_rng(seed).integers(low, high, shape).astype(np.float32)).to(dtype)
+
+
+def normal(shape, seed, scale=1.0):
+    return torch.from_numpy((scale * np.random.default_rng(seed).standard_normal(shape)).astype(np.float32))
+
+
+def strided(t, lead, offset):
+    """t as a view with `lead` unused columns beside it, starting `offset` elements into its storage (on the GPU)."""
+    rows, cols = t.shape
+    flat = torch.full((rows * (cols + lead) + offset + 8,), float("nan"), dtype=t.dtype, device="cuda")
+    view = flat[offset:offset + rows * (cols + lead)].view(rows, cols + lead)[:, :cols]
+    view.copy_(t)
+    return view
+
+
+# ----------------------------------------------------------------------------- linear
+SIZES = [(1, 1, 1), (1, 64, 64), (3, 17, 5), (80, 64, 64), (16, 32, 256), (33, 130, 96), (65, 100, 515), (127, 129, 63),
+         (128, 128, 128), (257, 72, 200), (300, 264, 40), (2, 1000, 1032), (17, 8, 2048), (515, 3, 7), (1030, 96, 384),
+         (256, 256, 64), (255, 512, 72)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", SIZES)
+def test_linear_whole_numbers_are_exact(dtype, M, N, K):
+    """Forward and all gradients on whole numbers: every fp32 sum is exact, so the only rounding is the output's."""
+    from sgnn_amd import functional
+    x, w, b = whole((M, K), 1, dtype=dtype), whole((N, K), 2, dtype=dtype), whole((N,), 3, dtype=dtype)
+    r, dy = whole((M, N), 4, dtype=dtype), whole((M, N), 5, dtype=dtype)
+    for act, res in (("none", None), ("relu", None), ("relu", r), ("none", r)):
+        z = x.double() @ w.double().T + b.double()
+        y = (act64(z, act) + (0.0 if res is None else res.double())).to(dtype)
+        dz = dy.double() * (z > 0) if act == "relu" else dy.double()
+        leaves = [t.cuda().requires_grad_(True) for t in (x, w, b) + ((r,) if res is not None else ())]
+        got = functional.linear(*leaves[:3], activation=act, residual=leaves[3] if res is not None else None)
+        grads = torch.autograd.grad(got, leaves, dy.cuda())
+        what = f"{act} residual={res is not None}"
+        assert torch.equal(got.detach().cpu(), y), what
+        for name, g, ref in zip(("dx", "dw", "db", "dres"), grads,
+                                (dz @ w.double(), dz.T @ x.double(), dz.sum(0), dy.double())):
+            assert torch.equal(g.cpu(), ref.to(dtype)), f"{what} {name}"
+        with torch.no_grad():
+            again = functional.linear(*leaves[:3], activation=act, residual=leaves[3] if res is not None else None)
+        assert torch.equal(again, got.detach()), what
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("lead,offset", [(0, 1), (1, 0), (3, 5), (8, 0), (8, 8)])
+def test_linear_strides_and_alignment(dtype, lead, offset):
+    """Operands with unused columns, at storage offsets that no vector is aligned to: what lies between the rows is
+    never read into a result (it is NaN here)."""
+    from sgnn_amd import functional
+    M, N, K = 70, 75, 88
+    x, w, r, dy = (whole(s, i, dtype=dtype) for i, s in enumerate([(M, K), (N, K), (M, N), (M, N)]))
+    xs, wsd, rs, dys = (strided(t, lead, offset) for t in (x, w, r, dy))
+    leaves = [t.requires_grad_(True) for t in (xs, wsd, rs)]
+    got = functional.linear(leaves[0], leaves[1], None, "relu", leaves[2])
+    dx, dw, dres = torch.autograd.grad(got, leaves, dys)
+    z = x.double() @ w.double().T
+    dz = dy.double() * (z > 0)
+    assert torch.equal(got.detach().cpu(), (z.relu() + r.double()).to(dtype))
+    assert torch.equal(dx.cpu(), (dz @ w.double()).to(dtype)) and torch.equal(dw.cpu(), (dz.T @ x.double()).to(dtype))
+    assert torch.equal(dres.cpu(), dy)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("M,N,K", [(37, 50, 70), (130, 140, 260), (1, 96, 600)])
+def test_linear_against_64_bits(dtype, act, M, N, K):
+    from sgnn_amd import functional
+    h = half_step(dtype)
+    h16 = h if dtype != torch.float32 else 0.0   # of values kept in the type between the passes
+    x, w, b, r, dy = (t.to(dtype) for t in (normal((M, K), 1), normal((N, K), 2, K ** -0.5), normal((N,), 3),
+                                            normal((M, N), 4), normal((M, N), 5)))
+    z = x.double() @ w.double().T + b.double()
+    if act == "relu":   # keep every z far enough from the slope's jump
+        x = x.clone()
+        b = (b.double() + 40.0 * (torch.arange(N) % 2 * 2 - 1)).to(dtype)
+        z = x.double() @ w.double().T + b.double()
+        assert float(z.abs().min()) > 1.0
+    d = [t.double().requires_grad_(True) for t in (x, w, b, r)]
+    ref = act64(d[0] @ d[1].T + d[2], act) + d[3]
+    ref_grads = torch.autograd.grad(ref, d, dy.double())
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b, r)]
+    got = functional.linear(*leaves[:3], activation=act, residual=leaves[3])
+    grads = torch.autograd.grad(got, leaves, dy.cuda())
+    # z, then the activation (slope at most 1.13; its functions good to (|z| + 8) 2 u of |z|), then the residual
+    mags = x.double().abs() @ w.double().abs().T + b.double().abs()
+    ez = (K + 4) * U * mags
+    ey = 1.13 * ez + (z.abs() + 8) * 2 * U * z.abs() + 2 * U * (z.abs() + r.double().abs())
+    within(got, ref.detach(), ey * (1 + h) + rounded(dtype, ref.detach()), f"y {act}")
+    # dz: slopes change by at most 0.8 per unit of z (nothing for none and relu, away from 0)
+    bend = 0.0 if act in ("none", "relu") else 0.8
+    slope = torch.autograd.grad(act64(zz := z.clone().requires_grad_(True), act).sum(), zz)[0]
+    dz = dy.double() * slope
+    edz = dy.double().abs() * (bend * (ez + h16 * z.abs()) + (z.abs() + 8) * 8 * U) + (h16 > 0) * rounded(dtype, dz) * (act != "none")
+    ad, aw, ax = dz.abs(), w.double().abs(), x.double().abs()
+    tols = ((N + 4) * U * (ad @ aw) + edz @ aw, (M + 4) * U * (ad.T @ ax) + edz.T @ ax,
+            (M + 4) * U * ad.sum(0) + edz.sum(0), 0.0)
+    for name, g, rg, tol in zip(("dx", "dw", "db", "dres"), grads, ref_grads, tols):
+        within(g, rg, tol * (1 + h) + rounded(dtype, rg) * (name != "dres"), f"{name} {act}")
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_long_reduction(dtype):
+    """The weight's gradient of many rows, and its bias', are whole-number exact (each partial sum < 2^24)."""
+    from sgnn_amd import functional
+    M, N, K = 20011, 40, 24
+    x, w, dy = whole((M, K), 1, dtype=dtype), whole((N, K), 2, dtype=dtype), whole((M, N), 3, dtype=dtype)
+    b = torch.zeros(N, dtype=dtype)
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(functional.linear(*leaves), leaves, dy.cuda())
+    assert torch.equal(dw.cpu(), (dy.double().T @ x.double()).to(dtype))
+    assert torch.equal(db.cpu(), dy.double().sum(0).to(dtype))
+    assert torch.equal(dx.cpu(), (dy.double() @ w.double()).to(dtype))
+
+
+def test_linear_gradient_against_differences():
+    """fp32 gradients against central differences of the operator's own sum, in a direction of each input."""
+    from sgnn_amd import functional
+    t = [normal(s, i, 0.5).cuda() for i, s in enumerate([(9, 20), (13, 20), (13,), (9, 13)])]
+    dirs = [normal(tuple(v.shape), 50 + i).cuda() for i, v in enumerate(t)]
+    for act in ("gelu", "gelu_tanh", "silu"):
+        leaves = [v.clone().requires_grad_(True) for v in t]
+        grads = torch.autograd.grad(functional.linear(*leaves[:3], act, leaves[3]).double().sum(), leaves)
+        for i in range(4):
+            def value(step):
+                args = [v + step * dirs[i] if j == i else v for j, v in enumerate(t)]
+                return float(functional.linear(*args[:3], act, args[3]).double().sum())
+            e = 2.0 ** -6
+            diff = (value(e) - value(-e)) / (2 * e)
+            # 9 * 13 outputs of magnitude < 16, each off by < 64 u of it; a third derivative of magnitude < 2 along
+            # the direction, whose size per output is < 12: e^2 / 6 * 2 * 12^3 per output at the very worst
+            tol = 117 * 16 * 64 * U / e + 117 * e * e / 6 * 2 * 12 ** 3 * 0.01
+            assert abs(diff - float((grads[i].double() * dirs[i].double()).sum())) <= tol, (act, i)
+
+
+def test_linear_edges_of_sizes():
+    from sgnn_amd import functional
+    for dtype in TYPES:
+        w, b = whole((6, 4), 1, dtype=dtype).cuda().requires_grad_(True), whole((6,), 2, dtype=dtype).cuda().requires_grad_(True)
+        x = torch.empty(0, 4, dtype=dtype, device="cuda", requires_grad=True)
+        y = functional.linear(x, w, b, "gelu")
+        assert y.shape == (0, 6)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty(0, 6, dtype=dtype, device="cuda"))
+        assert dx.shape == (0, 4) and not dw.any() and not db.any()
+        assert functional.linear(x.detach(), w[:0]).shape == (0, 0)
+        # no input features: the bias alone
+        x0, w0 = torch.empty(5, 0, dtype=dtype, device="cuda"), torch.empty(6, 0, dtype=dtype, device="cuda")
+        assert torch.equal(functional.linear(x0, w0, b.detach(), "relu"), b.detach().relu().expand(5, 6))
+        # leading dimensions, one vector, an expanded row, a transposed matrix
+        x3 = whole((2, 3, 4), 5, dtype=dtype).cuda()
+        ref = (x3.double() @ w.detach().double().T).to(dtype)
+        assert torch.equal(functional.linear(x3, w.detach()), ref)
+        assert torch.equal(functional.linear(x3[0, 0], w.detach()), ref[0, 0])
+        row = x3[0, :1].expand(7, 4)
+        assert torch.equal(functional.linear(row, w.detach()), ref[0, :1].expand(7, 6))
+        xt = x3[0].t().contiguous().t()
+        assert torch.equal(functional.linear(xt, w.detach()), ref[0])
+
+
+def test_linear_non_finite_values_propagate():
+    """A NaN or infinity reaches exactly the outputs that read it, as fp32 arithmetic has it; ReLU keeps a NaN."""
+    from sgnn_amd import functional
+    for dtype in TYPES:
+        x, w = whole((40, 48), 1, 1, 4, dtype=dtype), whole((72, 48), 2, 1, 4, dtype=dtype)
+        x[3, 5], x[7, 9], x[8, 47], w[11, 2] = float("nan"), float("inf"), float("-inf"), float("inf")
+        ref = x.double() @ w.double().T
+        for act in ("none", "relu"):
+            got = functional.linear(x.cuda(), w.cuda(), activation=act).cpu().double()
+            want = ref if act == "none" else torch.where(ref < 0, torch.zeros_like(ref), ref)
+            assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(1.5, 1e9, -1e9),
+                                                                          want.to(dtype).double().nan_to_num(1.5, 1e9, -1e9))
+
+
+def test_linear_refuses():
+    from sgnn_amd import functional
+    x, w = torch.zeros(3, 4, device="cuda"), torch.zeros(5, 4, device="cuda")
+    bad = [lambda: functional.linear(x.double(), w.double()), lambda: functional.linear(x, w.bfloat16()),
+           lambda: functional.linear(x, w.t()), lambda: functional.linear(x, w, torch.zeros(4, device="cuda")),
+           lambda: functional.linear(x, w, torch.zeros(5)), lambda: functional.linear(x, w, activation="tanh"),
+           lambda: functional.linear(x, w, residual=torch.zeros(3, 4, device="cuda")),
+           lambda: functional.linear(x, w, residual=torch.zeros(5, device="cuda")),
+           lambda: functional.linear(x, w[0])]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
+# ----------------------------------------------------------------------------- layer norm
+LN_SIZES = [(1, 1), (1, 64), (2, 3), (80, 64), (5, 128), (513, 96), (33, 100), (7, 771), (300, 256), (64, 1000),
+            (9, 4096), (3, 5003), (2, 8192), (4, 9000), (1000, 16), (129, 24), (2, 20000)]
+
+
+def _ln64(x, w, b, r, eps):
+    y = torch.nn.functional.layer_norm(x, (x.shape[-1],), w, b, eps)
+    return y if r is None else y + r
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("n,width", LN_SIZES)
+@pytest.mark.parametrize("w32", [False, True])
+def test_layer_norm_against_64_bits(dtype, n, width, w32):
+    from sgnn_amd import functional
+    wtype = torch.float32 if w32 else dtype
+    h, eps = half_step(dtype), 1e-5
+    x = (normal((n, width), 1, 2.0) + 1.5).to(dtype)
+    w, b = (1.0 + normal((width,), 2, 0.2)).to(wtype), normal((width,), 3, 0.3).to(wtype)
+    r, dy = normal((n, width), 4).to(dtype), normal((n, width), 5).to(dtype)
+    for res in (None, r):
+        given = [x, w, b] + ([r] if res is not None else [])
+        d = [t.double().requires_grad_(True) for t in given]
+        ref = _ln64(*d[:3], d[3] if res is not None else None, eps)
+        ref_grads = torch.autograd.grad(ref, d, dy.double())
+        leaves = [t.cuda().requires_grad_(True) for t in given]
+        got = functional.layer_norm(*leaves[:3], residual=leaves[3] if res is not None else None, eps=eps)
+        grads = torch.autograd.grad(got, leaves, dy.cuda())
+        x64, w64, up = x.double(), w.double(), dy.double()
+        mean = x64.mean(1, keepdim=True)
+        rstd = 1.0 / (x64.var(1, unbiased=False, keepdim=True) + eps).sqrt()
+        hat = (x64 - mean) * rstd
+        # a row sum: at most width / 8 + 16 additions deep
+        c = (width / 8 + 16) * U
+        emean = c * x64.abs().mean(1, keepdim=True)
+        ehat = rstd * (emean + 2 * U * (x64.abs() + mean.abs())) + hat.abs() * (c + 8 * U) + hat.abs() * rstd ** 2 * emean ** 2
+        ey = w64.abs() * ehat + 4 * U * ((hat * w64).abs() + b.double().abs() + (res.double().abs() if res is not None else 0))
+        within(got, ref.detach(), ey * (1 + h) + rounded(dtype, ref.detach()), "y")
+        g = up * w64
+        gm, ghm = g.mean(1, keepdim=True), (g * hat).mean(1, keepdim=True)
+        agm, aghm = g.abs().mean(1, keepdim=True), (g * hat).abs().mean(1, keepdim=True)
+        egm = c * agm
+        eghm = c * aghm + (g.abs() * ehat).mean(1, keepdim=True)
+        inner = g - gm - hat * ghm
+        edx = rstd * (egm + hat.abs() * eghm + ehat * ghm.abs() + 6 * U * (g.abs() + gm.abs() + (hat * ghm).abs())) \
+            + (c + 16 * U) * rstd * inner.abs() + rstd ** 3 * emean ** 2 * inner.abs()
+        edw = (n + 4) * U * (up * hat).abs().sum(0) + (up.abs() * ehat).sum(0)
+        edb = (n + 4) * U * up.abs().sum(0)
+        for name, gr, rg, tol in zip(("dx", "dw", "db", "dres"), grads, ref_grads, (edx, edw, edb, 0.0)):
+            kind = wtype if name in ("dw", "db") else dtype
+            assert gr.dtype == kind
+            within(gr, rg, tol * (1 + half_step(kind)) + rounded(kind, rg) * (name != "dres"), name)
+        with torch.no_grad():
+            again = functional.layer_norm(*leaves[:3], residual=leaves[3] if res is not None else None, eps=eps)
+        assert torch.equal(again, got.detach())
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("lead,offset", [(0, 1), (1, 0), (3, 5), (8, 8)])
+@pytest.mark.parametrize("width", [72, 88, 203, 1024])
+def test_layer_norm_strides_and_alignment(dtype, lead, offset, width):
+    """The same bits from strided, unaligned rows as from dense ones."""
+    from sgnn_amd import functional
+    x, r, dy = (normal((50, width), i).to(dtype) for i in range(3))
+    w, b = normal((width,), 4).to(dtype).cuda().requires_grad_(True), normal((width,), 5).to(dtype).cuda().requires_grad_(True)
+    outs = []
+    for make in (lambda t: t.cuda(), lambda t: strided(t, lead, offset)):
+        xs, rs, dys = make(x).requires_grad_(True), make(r).requires_grad_(True), make(dy)
+        y = functional.layer_norm(xs, w, b, residual=rs)
+        outs.append([y.detach(), *torch.autograd.grad(y, (xs, w, b, rs), dys)])
+    h = half_step(dtype)
+    for a, c in zip(*outs):
+        # the lanes' share of a row may differ with the alignment: at most a last step of the output's type apart
+        within(a, c.double().cpu(), (2 * h + 64 * U) * (c.double().cpu().abs() + (0 if h > U else c.double().cpu().abs().max())), "strided")
+
+
+def test_layer_norm_without_weights_and_edges():
+    from sgnn_amd import functional
+    x = normal((6, 40), 1).cuda()
+    ref = _ln64(x.double(), None, None, None, 1e-5).cpu()
+    within(functional.layer_norm(x), ref, 64 * U * (1 + ref.abs()), "no weights")
+    w = normal((40,), 2).cuda()
+    within(functional.layer_norm(x, w), ref * w.double().cpu(), 64 * U * (1 + ref.abs()) * w.double().cpu().abs(), "no bias")
+    within(functional.layer_norm(x, None, w), ref + w.double().cpu(), 64 * U * (1 + ref.abs() + w.double().cpu().abs()), "no weight")
+    xg, wg = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    dx, db = torch.autograd.grad(functional.layer_norm(xg, None, wg).sum(), (xg, wg))
+    within(db, torch.full((40,), 6.0, dtype=torch.float64), 0.0, "db without a weight")
+    within(dx, torch.zeros(6, 40, dtype=torch.float64), 256 * U, "dx of a sum without a weight")
+    # no rows; a constant row (variance 0); leading dimensions
+    e = torch.empty(0, 40, device="cuda", requires_grad=True)
+    dw, db = torch.autograd.grad(functional.layer_norm(e, wg, wg2 := w.clone().requires_grad_(True)), (wg, wg2),
+                                 torch.empty(0, 40, device="cuda"))
+    assert not dw.any() and not db.any()
+    const = torch.full((3, 40), 7.25, device="cuda")
+    assert torch.equal(functional.layer_norm(const, w, w), w.expand(3, 40))
+    x3 = normal((2, 3, 40), 3).cuda()
+    assert torch.equal(functional.layer_norm(x3, w), functional.layer_norm(x3.view(6, 40), w).view(2, 3, 40))
+    # a mean that is large against the spread: the differences are taken before they are squared
+    far = (normal((4, 512), 9) + 4096.0).cuda()
+    ref = _ln64(far.double(), None, None, None, 1e-5).cpu()
+    within(functional.layer_norm(far), ref, (512 / 8 + 16) * U * 4100.0 * 1.2, "far from 0")
+
+
+def test_layer_norm_non_finite_rows_stay_alone():
+    from sgnn_amd import functional
+    for dtype in TYPES:
+        x = normal((70, 130), 1).to(dtype).cuda()
+        clean = functional.layer_norm(x)
+        x[3, 7], x[9, 129] = float("nan"), float("inf")
+        got = functional.layer_norm(x)
+        keep = torch.ones(70, dtype=torch.bool, device="cuda")
+        keep[3] = keep[9] = False
+        assert torch.equal(got[keep], clean[keep]) and got[3].isnan().all() and got[9].isnan().all()
+
+
+def test_layer_norm_refuses():
+    from sgnn_amd import functional
+    x, w = torch.zeros(3, 4, device="cuda"), torch.zeros(4, device="cuda")
+    bad = [lambda: functional.layer_norm(x.double()), lambda: functional.layer_norm(x, w[:3]),
+           lambda: functional.layer_norm(x, w.bfloat16()), lambda: functional.layer_norm(x.half(), w, w.half()),
+           lambda: functional.layer_norm(x, w, residual=x[:2]), lambda: functional.layer_norm(x, w, eps=-1.0),
+           lambda: functional.layer_norm(x, w.cpu()), lambda: functional.layer_norm(torch.zeros(3, 0, device="cuda"))]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
+# ----------------------------------------------------------------------------- newton-schulz
+def ns64(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    a, b, c = coefficients
+    x = g.double()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    norm = x.norm(dim=(-2, -1), keepdim=True) + eps
+    x = torch.where(norm > 0, x / norm, torch.zeros_like(x))
+    for _ in range(steps):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * gram @ gram) @ x
+    return x.mT if tall else x
+
+
+def ns_tol(ref, dtype, m, n):
+    """Norm-wise: 15 products, each off by 4 sqrt(m + n) u of its size (rounding errors of random sign), and later
+    steps' slopes multiply what came before by at most 2.2 twice (near 1, |p'(s)| / (p(s) / s) < 2.2)."""
+    return 15 * 4 * (m + n) ** 0.5 * U * 2.2 ** 2 + 2 * half_step(dtype) * (dtype != torch.float32)
+
+
+NS_SIZES = [(1, 1), (1, 7), (5, 1), (3, 4), (16, 16), (17, 31), (64, 64), (100, 60), (128, 128), (128, 384), (129, 200),
+            (60, 515), (300, 260), (200, 1031)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("m,n", NS_SIZES)
+def test_newton_schulz_against_64_bits(dtype, m, n):
+    from sgnn_amd import muon
+    g = (0.02 * normal((m, n), 1)).to(dtype)
+    for t in (g, g.t()):
+        ref = ns64(t)
+        got = muon.newton_schulz(t.cuda())
+        assert got.dtype == dtype and got.shape == t.shape
+        err = float((got.double().cpu() - ref).norm() / ref.norm())
+        assert err <= ns_tol(ref, dtype, m, n), err
+    if min(m, n) >= 16:   # singular values near 1: what the steps are for
+        s = torch.linalg.svdvals(muon.newton_schulz(g.cuda()).double().cpu())
+        assert float(s.max()) < 1.3
+
+
+@pytest.mark.parametrize("steps,coefficients", [(0, (3.4445, -4.7750, 2.0315)), (1, (1.5, -0.5, 0.0)), (12, (1.875, -1.25, 0.375))])
+def test_newton_schulz_steps_and_coefficients(steps, coefficients):
+    from sgnn_amd import muon
+    g = normal((48, 80), 3).cuda()
+    ref = ns64(g.cpu(), steps, coefficients)
+    got = muon.newton_schulz(g, steps=steps, coefficients=coefficients).double().cpu()
+    assert float((got - ref).norm() / ref.norm()) <= max(3 * steps, 1) * 4 * 128 ** 0.5 * U * 4
+    if steps == 12:   # the cubic-order convergent polynomial: orthonormal rows
+        assert float((got @ got.T - torch.eye(48, dtype=torch.float64)).abs().max()) < 1e-3
+
+
+def test_newton_schulz_batches_and_lists():
+    """A batch, a list of several shapes, strided and transposed inputs give each matrix' own bits."""
+    from sgnn_amd import muon
+    batch = normal((5, 40, 72), 1).cuda()
+    alone = torch.stack([muon.newton_schulz(m) for m in batch])
+    assert torch.equal(muon.newton_schulz(batch), alone)
+    others = [normal((40, 72), 2).cuda(), normal((130, 150), 3).cuda(), normal((3, 20, 9), 4).cuda(), batch,
+              torch.empty(0, 5, device="cuda"), normal((130, 150), 5).cuda(), normal((1, 1), 6).cuda()]
+    for t, got in zip(others, muon.newton_schulz(others)):
+        assert got.shape == t.shape and torch.equal(got, muon.newton_schulz(t))
+    wide = normal((40, 100), 7).cuda()
+    assert torch.equal(muon.newton_schulz(wide[:, 3:75]), muon.newton_schulz(wide[:, 3:75].contiguous()))
+    assert torch.equal(muon.newton_schulz(wide.t()), muon.newton_schulz(wide.t().contiguous()))
+    assert torch.equal(muon.newton_schulz(batch[::2]), alone[::2])
+    assert torch.equal(muon.newton_schulz(batch.transpose(0, 1)[:, 1]), muon.newton_schulz(batch[1]))
+    assert muon.newton_schulz([]) == []
+
+
+def test_newton_schulz_special_values():
+    from sgnn_amd import muon
+    for dtype in TYPES:
+        zero = torch.zeros(30, 40, dtype=dtype, device="cuda")
+        assert torch.equal(muon.newton_schulz(zero), zero) and torch.equal(muon.newton_schulz(zero, eps=0.0), zero)
+        g = normal((30, 40), 1).to(dtype).cuda()
+        g[4], g[:, 7] = 0, 0           # dead rows and columns stay exactly 0
+        got = muon.newton_schulz(g)
+        assert not got[4].any() and not got[:, 7].any()
+        big = (g.float() * (2.0 ** 100 if dtype != torch.float16 else 2.0 ** 10)).to(dtype)   # squares overflow fp32
+        if dtype != torch.float16:
+            ref = ns64(big.cpu())
+            assert float((muon.newton_schulz(big).double().cpu() - ref).norm() / ref.norm()) <= ns_tol(ref, dtype, 30, 40)
+        g[0, 0] = float("nan")
+        assert muon.newton_schulz(g).isnan().any()
+    # tiny gradients: eps decides
+    small = normal((20, 30), 2).cuda() * 1e-9
+    ref = ns64(small.cpu())
+    assert float((muon.newton_schulz(small).double().cpu() - ref).norm() / ref.norm()) <= ns_tol(ref, torch.float32, 20, 30)
+
+
+def test_newton_schulz_refuses():
+    from sgnn_amd import muon
+    x = torch.zeros(3, 4, device="cuda")
+    bad = [lambda: muon.newton_schulz(x.double()), lambda: muon.newton_schulz(x[0]), lambda: muon.newton_schulz([x, x.half()]),
+           lambda: muon.newton_schulz(x, steps=-1), lambda: muon.newton_schulz(x, eps=-1.0),
+           lambda: muon.newton_schulz(x[None, None]), lambda: muon.newton_schulz([x, x.cpu()])]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
+
+
+# ----------------------------------------------------------------------------- together
+def _block(functional, x, p):
+    h = functional.linear(x, p[0], p[1], "gelu")
+    return functional.layer_norm(functional.linear(h, p[2], p[3], residual=x), p[4], p[5], residual=x)
+
+
+def _block_params(width, hidden, dtype):
+    return [normal((hidden, width), 1, width ** -0.5), normal((hidden,), 2, 0.1), normal((width, hidden), 3, hidden ** -0.5),
+            normal((width,), 4, 0.1), 1.0 + normal((width,), 5, 0.1), normal((width,), 6, 0.1)]
+
+
+@pytest.mark.parametrize("dtype,tol", [(torch.float32, 1e-5), (torch.bfloat16, 4e-2)], ids=["f32", "bf16"])
+def test_training_step_of_a_block(dtype, tol):
+    """linear + gelu, linear + residual, layer_norm + residual, their gradients and the orthogonalised update of both
+    weights, as one step: against 64 bits.  fp32: a chain of ~10 sums of <= 200 terms, (200 + 4) u * 10 < 1e-4 in the
+    worst case, 1e-5 in the norm; bf16: ten roundings of 2^-9 in the norm, doubled."""
+    from sgnn_amd import functional, muon
+    x, dy = normal((77, 64), 11).to(dtype), normal((77, 64), 12).to(dtype)
+    params = [t.to(dtype) for t in _block_params(64, 200, dtype)]
+    p64 = [t.double().requires_grad_(True) for t in params]
+    hid = act64(x.double() @ p64[0].T + p64[1], "gelu")
+    y64 = _ln64(hid @ p64[2].T + p64[3] + x.double(), p64[4], p64[5], x.double(), 1e-5)
+    g64 = torch.autograd.grad(y64, p64, dy.double())
+    p = [t.cuda().requires_grad_(True) for t in params]
+    y = _block(functional, x.cuda(), p)
+    grads = torch.autograd.grad(y, p, dy.cuda())
+    for name, got, ref in [("y", y.detach(), y64.detach())] + list(zip(["w1", "b1", "w2", "b2", "gamma", "beta"], grads, g64)):
+        assert float((got.double().cpu() - ref).norm() / ref.norm()) <= tol, name
+    updates = muon.newton_schulz([grads[0], grads[2]])
+    for u, g in zip(updates, (grads[0], grads[2])):
+        ref = ns64(g.cpu())
+        assert float((u.double().cpu() - ref).norm() / ref.norm()) <= ns_tol(ref, dtype, 64, 200)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_captured_step_replays(dtype):
+    """Forward, backward and the orthogonalised updates in one graph: every replay gives the eager results of the
+    inputs of the moment, with eager work in between."""
+    from sgnn_amd import functional, muon
+    params = [t.to(dtype).cuda().requires_grad_(True) for t in _block_params(64, 200, dtype)]
+    x = torch.zeros(77, 64, dtype=dtype, device="cuda")
+    dy = torch.zeros(77, 64, dtype=dtype, device="cuda")
+
+    def step():
+        y = _block(functional, x, params)
+        grads = torch.autograd.grad(y, params, dy)
+        return [y.detach(), *grads, *muon.newton_schulz([grads[0], grads[2]])]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for seed in range(4):
+        x.copy_(normal((77, 64), 20 + seed).to(dtype))
+        dy.copy_(normal((77, 64), 30 + seed).to(dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        replayed = [o.clone() for o in outs]
+        for a, b in zip(replayed, step()):
+            assert torch.equal(a, b), seed
+
+
+def test_two_streams_at_once():
+    """The same operators on two streams, interleaved: neither sees the other's workspace."""
+    from sgnn_amd import functional, muon
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    data = [[normal((2000, 96), 3 * i + j).cuda() for j in range(2)] + [normal((80, 96), 40 + i, 0.1).cuda()] for i in range(2)]
+
+    def step(x, dy, w):
+        w = w.detach().requires_grad_(True)
+        y = functional.layer_norm(functional.linear(x, w, None, "silu"), None, None)
+        g, = torch.autograd.grad(y, w, dy[:, :80].contiguous())
+        return y.detach(), g, muon.newton_schulz(g)
+
+    want = [step(*d) for d in data]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(step(*data[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for outs in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(outs, want[i]))
+
+
+def test_runs_repeat_bit_for_bit():
+    from sgnn_amd import functional, muon
+    x, dy = normal((3001, 100), 1).cuda(), normal((3001, 90), 2).cuda()
+    w = normal((90, 100), 3, 0.1).cuda().requires_grad_(True)
+    b, g, be = (normal((90,), i).cuda().requires_grad_(True) for i in (4, 5, 6))
+    runs = []
+    for _ in range(3):
+        y = functional.layer_norm(functional.linear(x, w, b, "gelu"), g, be)
+        grads = torch.autograd.grad(y, (w, b, g, be), dy)
+        runs.append([y.detach(), *grads, muon.newton_schulz(grads[0])])
+    for other in runs[1:]:
+        assert all(torch.equal(a, c) for a, c in zip(runs[0], other))

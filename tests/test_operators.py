@@ -1,0 +1,98 @@
+"""The typed operators' refusals that need no GPU: the C entry points check every
+argument before they touch the device, and the Python ones refuse CPU tensors."""
+import ctypes
+
+import pytest
+import torch
+
+from sgnn_amd import _hip, functional, muon
+
+INVALID = _hip.SGNN_ERR_INVALID
+P = 256   # a non-null pointer that no refused call reads
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _hip.load_library()
+
+
+def _linear(lib, dtype=0, M=4, N=4, K=4, x=P, ldx=4, w=P, ldw=4, act=0, res=None, ldr=4, y=P, ldy=4, nws=1 << 30):
+    return lib.sgnn_linear(dtype, M, N, K, x, ldx, w, ldw, None, act, res, ldr, None, y, ldy, P, nws, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=3), dict(dtype=-1), dict(act=5), dict(act=-1), dict(M=-1), dict(N=-1), dict(K=-1), dict(x=None),
+    dict(w=None), dict(y=None), dict(ldx=3), dict(ldw=3), dict(ldy=3), dict(res=P, ldr=3)])
+def test_linear_refuses(lib, bad):
+    assert _linear(lib, **bad) == INVALID
+    assert "linear" in lib.sgnn_last_error().decode()
+
+
+def test_empty_calls_need_no_device(lib):
+    assert _linear(lib, M=0) == _hip.SGNN_OK and _linear(lib, N=0) == _hip.SGNN_OK
+    assert lib.sgnn_norm(0, 0, None, 4, 0, 4, None, None, None, 4, 1e-5, None, None, None, None) == _hip.SGNN_OK
+    assert lib.sgnn_newton_schulz(0, None, 0, 5, 1.0, 0.0, 0.0, 0.0, None, 0, None) == _hip.SGNN_OK
+    empty = (_hip.SgnnMatrix * 1)(_hip.SgnnMatrix(None, None, 0, 0, 0, 7))
+    assert lib.sgnn_newton_schulz_workspace_bytes(empty, 1) == 0
+    assert lib.sgnn_newton_schulz(0, empty, 1, 5, 1.0, 0.0, 0.0, 0.0, None, 0, None) == _hip.SGNN_OK
+
+
+def _linear_bwd(lib, dtype=0, M=4, N=4, K=4, dy=P, ldd=4, z=P, act=3, x=P, ldx=4, w=P, ldw=4, dx=P, dw=P, db=P,
+                nws=1 << 30):
+    return lib.sgnn_linear_bwd(dtype, M, N, K, dy, ldd, z, act, x, ldx, w, ldw, dx, dw, db, P, nws, None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=7), dict(act=9), dict(M=-1), dict(dy=None), dict(ldd=3), dict(z=None), dict(x=None), dict(ldx=3),
+    dict(w=None), dict(ldw=3), dict(nws=0)])
+def test_linear_bwd_refuses(lib, bad):
+    assert _linear_bwd(lib, **bad) == INVALID
+    assert "linear_bwd" in lib.sgnn_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dtype=5), dict(dtype=1, wdtype=2), dict(n=-1), dict(width=0), dict(x=None), dict(y=None), dict(ldx=3),
+    dict(res=P, ldr=3), dict(eps=-1.0), dict(eps=float("nan"))])
+def test_norm_refuses(lib, bad):
+    a = dict(dtype=0, wdtype=0, n=4, width=4, x=P, ldx=4, y=P, res=None, ldr=4, eps=1e-5)
+    a.update(bad)
+    if "wdtype" not in bad:
+        a["wdtype"] = a["dtype"]
+    assert lib.sgnn_norm(a["dtype"], a["wdtype"], a["x"], a["ldx"], a["n"], a["width"], None, None, a["res"],
+                         a["ldr"], a["eps"], a["y"], None, None, None) == INVALID
+    assert "norm" in lib.sgnn_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=5), dict(n=-1), dict(width=0), dict(dy=None), dict(x=None), dict(mean=None),
+                                 dict(rstd=None), dict(ldd=3), dict(ldx=3), dict(nws=0)])
+def test_norm_bwd_refuses(lib, bad):
+    a = dict(dtype=0, n=4, width=4, dy=P, ldd=4, x=P, ldx=4, mean=P, rstd=P, nws=1 << 20)
+    a.update(bad)
+    assert lib.sgnn_norm_bwd(a["dtype"], a["dtype"], a["dy"], a["ldd"], a["x"], a["ldx"], a["mean"], a["rstd"], None,
+                             a["n"], a["width"], P, P, P, P, a["nws"], None) == INVALID
+    assert "norm_bwd" in lib.sgnn_last_error().decode()
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=4), dict(count=-1), dict(steps=-1), dict(eps=-1.0), dict(null=True),
+                                 dict(rows=-1), dict(ld=3), dict(in_=None), dict(nws=0)])
+def test_newton_schulz_refuses(lib, bad):
+    a = dict(dtype=0, count=1, steps=5, eps=0.0, null=False, rows=4, ld=4, in_=P, nws=1 << 20)
+    a.update(bad)
+    mats = (_hip.SgnnMatrix * 1)(_hip.SgnnMatrix(a["in_"], P, a["ld"], 4, a["rows"], 4))
+    assert lib.sgnn_newton_schulz(a["dtype"], None if a["null"] else mats, a["count"], a["steps"], 1.0, 0.0, 0.0,
+                                  a["eps"], P, a["nws"], None) == INVALID
+    assert "newton_schulz" in lib.sgnn_last_error().decode()
+
+
+def test_matrix_struct_matches_header():
+    assert ctypes.sizeof(_hip.SgnnMatrix) == 40
+
+
+def test_python_entry_points_refuse_cpu_tensors():
+    x, w = torch.zeros(3, 4), torch.zeros(5, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        functional.linear(x, w)
+    with pytest.raises(ValueError, match="GPU"):
+        functional.layer_norm(x)
+    with pytest.raises(ValueError, match="GPU"):
+        muon.newton_schulz(x)
