@@ -1,5 +1,14 @@
-// One matrix product for every operand type and storage order (gemm.h): 64 x 64 output tiles, operands staged
-// as fp32 through LDS, v_mfma_f32_32x32x2_f32.
+// One matrix product for every operand type and storage order (gemm.h).
+//
+//   k_gemm16   bf16 / fp16 operands on v_mfma_f32_16x16x32: double-buffered LDS tiles of 64 k, filled by the
+//              direct-to-LDS loads where the operands' rows are 16-byte aligned, through registers elsewhere
+//   k_gemm32   fp32 operands as three bf16 parts each (8 + 8 + 8 bits, split exactly while they are staged), six
+//              bf16 products per fp32 one
+//   k_gemm_row few rows of x: each wave streams its share of w's rows into registers, LDS only for the join
+//
+// Both tiled kernels hold D[n][m] (w's rows on the accumulators' rows, x's on the lanes): a lane then has four
+// consecutive n of one m, which go through LDS once more so that the epilogue's loads and stores are whole
+// 16-byte pieces of rows at any alignment.
 #include "gemm.h"
 
 #include "ops_types.h"
@@ -7,86 +16,698 @@
 namespace {
 using namespace sgnn;
 
-constexpr int kTile = 64;    // output tile (M and N) per workgroup
-constexpr int kKc = 16;      // K per LDS stage
-constexpr int kLdT = kTile + 4;
-constexpr int kThreads = 256;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+// 16 bytes at any element's alignment (one global_load/store_dwordx4: unaligned access is on for this target)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
-// 64 rows (m or n) x 16 k of an operand into LDS as S[k][row], zero outside the matrix.
-template <typename T>
-SGNN_DEV void stage(float* S, const T* p, int64_t ld, bool cols, int64_t rows, int64_t K, int64_t r0, int64_t k0) {
-  const int t = threadIdx.x;
+#define SGNN_LDS __attribute__((address_space(3)))
+#define SGNN_GLB __attribute__((address_space(1)))
+
+struct GemmArgs {
+  const void *A, *B, *bias, *res;
+  void *z, *C;
+  float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
+  int64_t lda, ldb, ldr, ldc, M, N, K, batch_a, batch_b, batch_r, batch_c;
+  int32_t act, nsplit, tiles_m, tiles_n;
+  float alpha, beta;
+};
+
+// ----------------------------------------------------------------------------- epilogue
+template <int ACT>
+SGNN_DEV void act_n(float* v, int n) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int r = cols ? (t & 15) * 4 + c : t >> 2, k = cols ? t >> 4 : (t & 3) * 4 + c;
-    const int64_t gr = r0 + r, gk = k0 + k;
-    S[k * kLdT + r] = gr < rows && gk < K ? to_float(p[cols ? gk * ld + gr : gr * ld + gk]) : 0.0f;
+  for (int i = 0; i < 8; ++i)
+    if (i < n) v[i] = act_value<ACT>(v[i]);
+}
+
+SGNN_DEV void act_any(int32_t act, float* v, int n) {  // act is the same for every lane
+  switch (act) {
+    case SGNN_ACT_RELU: act_n<SGNN_ACT_RELU>(v, n); break;
+    case SGNN_ACT_GELU: act_n<SGNN_ACT_GELU>(v, n); break;
+    case SGNN_ACT_GELU_TANH: act_n<SGNN_ACT_GELU_TANH>(v, n); break;
+    case SGNN_ACT_SILU: act_n<SGNN_ACT_SILU>(v, n); break;
+    default: break;
   }
 }
 
-template <typename T, int ACT>
-__global__ __launch_bounds__(kThreads) void k_gemm_typed(Gemm g) {
-  __shared__ float As[kKc * kLdT];
-  __shared__ float Bs[kKc * kLdT];
-  const int l = lane_id(), w = wave_id();
-  const int wm = w >> 1, wn = w & 1;
-  const int64_t m0 = (int64_t)blockIdx.x * kTile, n0 = (int64_t)blockIdx.y * kTile, b = blockIdx.z;
-  const T* A = static_cast<const T*>(g.A) + b * g.batch_a;
-  const T* B = static_cast<const T*>(g.B) + b * g.batch_b;
-  f32x16 acc;
+// 16 bytes of T at any alignment <-> floats
+template <typename T>
+SGNN_DEV void load_vec(const T* p, float* v) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  const TV t = __builtin_bit_cast(TV, (u32x4)*reinterpret_cast<const u32x4_any*>(p));
 #pragma unroll
-  for (int r = 0; r < 16; ++r) acc[r] = 0.0f;
-  for (int64_t k0 = 0; k0 < g.K; k0 += kKc) {
-    stage(As, A, g.lda, g.a_cols, g.M, g.K, m0, k0);
-    stage(Bs, B, g.ldb, g.b_cols, g.N, g.K, n0, k0);
+  for (int i = 0; i < V; ++i) v[i] = to_float(t[i]);
+}
+template <typename T>
+SGNN_DEV void store_vec(T* p, const float* v) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  TV t;
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = from_float<T>(v[i]);
+  *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, t);
+}
+
+// V consecutive outputs (m, n ..) of one lane; cnt of them exist.
+template <typename T>
+SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float* v, int cnt) {
+  constexpr int V = 16 / sizeof(T);
+  const bool whole = cnt >= V;
+  float t[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] *= g.alpha;
+  if (g.bias) {
+    const T* p = static_cast<const T*>(g.bias) + n;
+    if (whole) {
+      load_vec(p, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += t[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < cnt) v[i] += to_float(p[i]);
+    }
+  }
+  if (g.z) {
+    T* p = static_cast<T*>(g.z) + m * g.N + n;
+    if (whole) {
+      store_vec(p, v);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < cnt) p[i] = from_float<T>(v[i]);
+    }
+  }
+  act_any(g.act, v, V);
+  if (g.res) {
+    const T* p = static_cast<const T*>(g.res) + b * g.batch_r + m * g.ldr + n;
+    if (whole) {
+      load_vec(p, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += g.beta * t[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < cnt) v[i] += g.beta * to_float(p[i]);
+    }
+  }
+  T* p = static_cast<T*>(g.C) + b * g.batch_c + m * g.ldc + n;
+  if (whole) {
+    store_vec(p, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < cnt) p[i] = from_float<T>(v[i]);
+  }
+}
+
+// A wave's accumulators (TM x TN sub-tiles of 16 x 16, lane l: m = l & 15, n = 4 (l >> 4) + r) to memory, 16 rows
+// of m at a time through `buf` (16 x 16 TN floats of its own).  16-byte pieces are XORed with m, so that the 16
+// rows of one write, which are a multiple of all banks apart, fall on different ones.
+template <typename T, int TM, int TN>
+SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][TN], int64_t b, int split, int64_t m0,
+                         int64_t n0) {
+  const int l = lane_id();
+  constexpr int kPieces = 4 * TN;  // 16-byte pieces per row of 16 TN floats
+  constexpr int kMask = kPieces - 1 < 15 ? kPieces - 1 : 15;
+  const int lm = l & 15;
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const int piece = (4 * j + (l >> 4)) ^ (lm & kMask);
+      *reinterpret_cast<f32x4*>(buf + lm * 16 * TN + piece * 4) = acc[i][j];
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (g.part) {
+#pragma unroll 1
+      for (int t = l; t < 16 * kPieces; t += 64) {
+        const int r = t / kPieces, p = t % kPieces;
+        const f32x4 v = *reinterpret_cast<const f32x4*>(buf + r * 16 * TN + (p ^ (r & kMask)) * 4);
+        const int64_t m = m0 + 16 * i + r, n = n0 + 4 * p;
+        if (m >= g.M || n >= g.N) continue;
+        float* o = g.part + ((int64_t)split * g.M + m) * g.N + n;
+        if (n + 4 <= g.N) {
+          *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, v);
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            if (n + q < g.N) o[q] = v[q];
+        }
+      }
+    } else {
+      constexpr int V = 16 / sizeof(T), kPer = V / 4;
+#pragma unroll 1
+      for (int t = l; t < 16 * kPieces / kPer; t += 64) {
+        const int r = t / (kPieces / kPer), p = (t % (kPieces / kPer)) * kPer;
+        float v[V];
+#pragma unroll
+        for (int q = 0; q < kPer; ++q) {
+          const f32x4 f = *reinterpret_cast<const f32x4*>(buf + r * 16 * TN + ((p + q) ^ (r & kMask)) * 4);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
+        }
+        const int64_t m = m0 + 16 * i + r, n = n0 + 4 * p;
+        if (m < g.M && n < g.N) finish<T>(g, b, m, n, v, (int)min((int64_t)V, g.N - n));
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
+// Workgroup -> tile.  Consecutive workgroups go to the 8 XCDs in turn, each with an L2 of its own: XCD x takes the
+// x-th contiguous share of the tiles, in groups of 8 row tiles by all column tiles, so that the tiles resident on
+// one L2 share their operands' rows.
+SGNN_DEV void tile_of(const GemmArgs& g, int& tm, int& tn) {
+  const int total = g.tiles_m * g.tiles_n, id = blockIdx.x;
+  const int xcd = id & 7, q = total >> 3, r = total & 7;
+  const int t = xcd * q + min(xcd, r) + (id >> 3);
+  constexpr int kGroup = 8;
+  const int per = kGroup * g.tiles_n, grp = t / per, rest = t - grp * per;
+  const int rows = min(kGroup, g.tiles_m - grp * kGroup);
+  const int col = rest / rows;
+  tn = __builtin_amdgcn_readfirstlane(col);
+  tm = __builtin_amdgcn_readfirstlane(grp * kGroup + rest - col * rows);
+}
+
+// This workgroup's blocks of k.
+SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& last) {
+  const int64_t blocks = (g.K + bk - 1) / bk;
+  first = __builtin_amdgcn_readfirstlane((int)(blocks * split / g.nsplit));
+  last = __builtin_amdgcn_readfirstlane((int)(blocks * (split + 1) / g.nsplit));
+}
+
+// ----------------------------------------------------------------------------- 16-bit operands
+template <typename T>
+SGNN_DEV f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  if constexpr (std::is_same_v<T, bf16_t>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
+}
+
+// One operand's tile in LDS: R rows (m or n) by BK of k, in 16-byte chunks.
+//   rows layout (k contiguous in memory): row r's chunk c (8 k) at slot c ^ swizzle(r)
+//   cols layout (m / n contiguous): k's chunk c (8 rows) at slot c ^ 2 h(k); read back transposed
+// The swizzles put the pieces that one LDS instruction touches at a time on different banks.
+template <int R, int BK, bool COLS>
+struct Tile16 {
+  static constexpr int kChunks = COLS ? R / 8 : BK / 8;  // chunks per line of memory (a row, or a k)
+  static constexpr int kLines = COLS ? BK : R;
+  static constexpr int kBytes = R * BK * 2;
+  static SGNN_DEV int swizzle(int line) {
+    if constexpr (COLS) return (2 * ((line & 3) | ((line >> 1) & 4))) & (kChunks - 1);
+    return kChunks == 8 ? (line >> 1) & 7 : (line >> 2) & 3;
+  }
+
+  // Chunk q of the tile (in LDS order) holds memory's line q / kChunks, chunk (q % kChunks) ^ swizzle.  offsets():
+  // this lane's chunks' bytes from the tile's first element, the same for every block of k.  Lines and chunks past
+  // the last row read another one's data: their outputs are not stored.
+  template <int THREADS, int KPER>
+  static SGNN_DEV void offsets(uint32_t (&o)[KPER], int64_t ld, int64_t rows, int64_t r0) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      const int q = i * THREADS + threadIdx.x;
+      const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
+      const int left = (int)min(rows - r0, (int64_t)R);
+      o[i] = 2 * (COLS ? (uint32_t)line * (uint32_t)ld + min(8 * c, left - 8)
+                       : (uint32_t)min(line, left - 1) * (uint32_t)ld + 8 * c);
+    }
+  }
+  // first: the block's first element.  The loads' 64 x 16 bytes land at m0 in lane order; they are written as
+  // instructions, as the compiler makes every later LDS read wait for the builtin's.  The caller waits (vmcnt).
+  template <int THREADS, int KPER>
+  static SGNN_DEV void direct(const char* lds, const char* first, const uint32_t (&o)[KPER]) {
+    const uint64_t at = (uint64_t)first;
+    const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
+                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      const uint32_t to = __builtin_amdgcn_readfirstlane(
+          (uint32_t)(uintptr_t)(const SGNN_LDS char*)lds + (i * THREADS + threadIdx.x / 64 * 64) * 16);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                   :
+                   : "s"(to), "v"(o[i]), "s"(base)
+                   : "memory", "m0");
+    }
+  }
+
+  // The same through registers, at any alignment, with zeros past K (and past the last row, in cols).
+  template <int THREADS, int KPER>
+  static SGNN_DEV void fetch(u32x4 (&v)[KPER], const char* src, int64_t ld, int64_t rows, int64_t K, int64_t r0,
+                             int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      const int q = i * THREADS + threadIdx.x;
+      const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
+      const int64_t gl = (COLS ? k0 : r0) + line, gc = (COLS ? r0 : k0) + 8 * c;
+      const int64_t lines = COLS ? K : rows, most = COLS ? rows : K;
+      u32x4 t = {0, 0, 0, 0};
+      if (gl < lines && gc < most) {
+        const char* p = src + 2 * (gl * ld + gc);
+        if (gc + 8 <= most) {
+          t = *reinterpret_cast<const u32x4_any*>(p);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (gc + e < most) t[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
+        }
+      }
+      v[i] = t;
+    }
+  }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void put(char* lds, const u32x4 (&v)[KPER]) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) *reinterpret_cast<u32x4*>(lds + (i * THREADS + threadIdx.x) * 16) = v[i];
+  }
+
+  // Fragment of 16 rows from r (a multiple of 16) by 32 k from 32 kk: lane l has row l & 15, k 8 (l >> 4) .. + 7.
+  static SGNN_DEV s16x8 frag(const char* lds, int r, int kk) {
+    const int l = lane_id();
+    if constexpr (!COLS) {
+      const int row = r + (l & 15);
+      return *reinterpret_cast<const s16x8*>(lds + (row * kChunks + ((4 * kk + (l >> 4)) ^ swizzle(row))) * 16);
+    } else {
+      // ds_read_b64_tr_b16: lanes 4 j .. 4 j + 3 of a group of 16 read 16 rows of k + j, lane i gets row i of 4 k
+      const int k = 32 * kk + 8 * (l >> 4) + ((l & 15) >> 2);
+      const int at = (k * kChunks + ((r / 8 + ((l & 3) >> 1)) ^ swizzle(k))) * 16 + (l & 1) * 8;
+      // k + 4 has the same swizzle
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(lds + at));
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(lds + at + 4 * kChunks * 16));
+      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// BM x BN outputs per workgroup, WM x WN waves.  DIRECT: both operands' lines are 16-byte aligned (and in the cols
+// layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
+template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
+  constexpr int BK = 64, kThreads = 64 * WM * WN;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  using TA = Tile16<BM, BK, ACOLS>;
+  using TB = Tile16<BN, BK, BCOLS>;
+  constexpr int kStage = TA::kBytes + TB::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];  // two stages of A's and B's tiles
+  static_assert(16 * 16 * TN * 4 * WM * WN <= 2 * kStage, "the epilogue's buffers fit");
+  const int w = wave_id(), wm = w / WN, wn = w % WN;
+  int tm, tn;
+  tile_of(g, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int split = g.nsplit > 1 ? blockIdx.z : 0;
+  const int64_t batch = g.nsplit > 1 ? 0 : blockIdx.z;
+  const char* A = static_cast<const char*>(g.A) + 2 * batch * g.batch_a;
+  const char* B = static_cast<const char*>(g.B) + 2 * batch * g.batch_b;
+  int first, last;
+  blocks_of(g, BK, split, first, last);
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  const auto compute = [&](const char* a) {
+    const char* b = a + TA::kBytes;
+#pragma unroll
+    for (int kk = 0; kk < BK / 32; ++kk) {
+      s16x8 fa[TM], fb[TN];
+#pragma unroll
+      for (int j = 0; j < TN; ++j) fb[j] = TB::frag(b, (wn * TN + j) * 16, kk);
+#pragma unroll
+      for (int i = 0; i < TM; ++i) fa[i] = TA::frag(a, (wm * TM + i) * 16, kk);
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
+    }
+  };
+  constexpr int PA = BM * BK / 8 / kThreads, PB = BN * BK / 8 / kThreads;
+  u32x4 va[PA], vb[PB];
+  const auto fetch = [&](int blk) {
+    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
+  };
+  const auto put = [&](char* a) {
+    TA::template put<kThreads>(a, va);
+    TB::template put<kThreads>(a + TA::kBytes, vb);
+  };
+  char* here = lds;
+  char* there = lds + kStage;
+  // One barrier per block: past it, this block's tiles are whole and the other stage is read by no wave any more.
+  if constexpr (DIRECT) {
+    uint32_t oa[PA], ob[PB];
+    TA::template offsets<kThreads>(oa, g.lda, g.M, m0);
+    TB::template offsets<kThreads>(ob, g.ldb, g.N, n0);
+    const char* pa = A + 2 * (ACOLS ? m0 : m0 * g.lda);
+    const char* pb = B + 2 * (BCOLS ? n0 : n0 * g.ldb);
+    const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
+    const auto stage = [&](char* a, int blk) {
+      if ((int64_t)(blk + 1) * BK <= g.K) {
+        TA::template direct<kThreads>(a, pa + blk * sa, oa);
+        TB::template direct<kThreads>(a + TA::kBytes, pb + blk * sb, ob);
+      } else {
+        fetch(blk);
+        put(a);
+      }
+    };
+    if (first < last) stage(here, first);
+    for (int blk = first; blk < last; ++blk) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      if (blk + 1 < last) stage(there, blk + 1);
+      compute(here);
+      char* t = here;
+      here = there, there = t;
+    }
+  } else {
+    // the next block waits in registers while this one's products run
+    if (first < last) {
+      fetch(first);
+      put(here);
+    }
+    for (int blk = first; blk < last; ++blk) {
+      __syncthreads();
+      if (blk + 1 < last) fetch(blk + 1);
+      compute(here);
+      if (blk + 1 < last) put(there);
+      char* t = here;
+      here = there, there = t;
+    }
+  }
+  __syncthreads();
+  write_tile<T, TM, TN>(g, reinterpret_cast<float*>(lds) + w * 16 * 16 * TN, acc, batch, split, m0 + wm * TM * 16,
+                        n0 + wn * TN * 16);
+}
+
+// ----------------------------------------------------------------------------- fp32 operands
+// v = hi + mid + lo, each the leading 8 bits of what is left (truncated, so every difference is exact).
+SGNN_DEV void split3(f32x4 v, u32x2& hi, u32x2& mid, u32x2& lo) {
+  uint32_t h[4], m[4], q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float x = v[i];
+    h[i] = __builtin_bit_cast(uint32_t, x);
+    const float r = x - __builtin_bit_cast(float, h[i] & 0xffff0000u);
+    m[i] = __builtin_bit_cast(uint32_t, r);
+    q[i] = __builtin_bit_cast(uint32_t, r - __builtin_bit_cast(float, m[i] & 0xffff0000u));
+  }
+  // the upper halves of two words as one: bytes 2, 3 of the first, then of the second
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    hi[i] = __builtin_amdgcn_perm(h[2 * i + 1], h[2 * i], 0x07060302u);
+    mid[i] = __builtin_amdgcn_perm(m[2 * i + 1], m[2 * i], 0x07060302u);
+    lo[i] = __builtin_amdgcn_perm(q[2 * i + 1], q[2 * i], 0x07060302u);
+  }
+}
+
+// R rows by 32 k as three planes of bf16, row r's chunk c (8 k) at slot c ^ ((r >> 2) & 3): 16 rows' chunks of one
+// read cover all banks.
+template <int R, bool COLS>
+struct Tile32 {
+  static constexpr int BK = 32, kPlane = R * BK * 2, kBytes = 3 * kPlane;
+  static SGNN_DEV int at(int row, int k) {  // byte of element (row, k)
+    return row * 64 + (((k >> 3) ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
+  }
+  // Rows: KPER x four k of one row.  Cols: one block of KPER k (two or four) by four rows.
+  template <int THREADS, int KPER>
+  static SGNN_DEV void fetch(f32x4 (&v)[KPER], const float* src, int64_t ld, int64_t rows, int64_t K, int64_t r0,
+                             int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      int64_t line, col, lines, most;
+      if constexpr (COLS) {
+        line = k0 + threadIdx.x / (R / 4) * KPER + i, col = r0 + threadIdx.x % (R / 4) * 4, lines = K, most = rows;
+      } else {
+        const int q = i * THREADS + threadIdx.x;
+        line = r0 + q / 8, col = k0 + q % 8 * 4, lines = rows, most = K;
+      }
+      f32x4 t = {0, 0, 0, 0};
+      if (line < lines && col < most) {
+        const float* p = src + line * ld + col;
+        if (col + 4 <= most) {
+          t = __builtin_bit_cast(f32x4, (u32x4)*reinterpret_cast<const u32x4_any*>(p));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < most) t[e] = p[e];
+        }
+      }
+      v[i] = t;
+    }
+  }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void put(char* lds, const f32x4 (&v)[KPER]) {
+    u32x2 hi, mid, lo;
+    if constexpr (!COLS) {
+#pragma unroll
+      for (int i = 0; i < KPER; ++i) {
+        const int q = i * THREADS + threadIdx.x, o = at(q / 8, q % 8 * 4);
+        split3(v[i], hi, mid, lo);
+        *reinterpret_cast<u32x2*>(lds + o) = hi;
+        *reinterpret_cast<u32x2*>(lds + kPlane + o) = mid;
+        *reinterpret_cast<u32x2*>(lds + 2 * kPlane + o) = lo;
+      }
+    } else {
+      static_assert(KPER == 2 || KPER == 4, "a block's k fit one LDS word or two");
+      const int k = threadIdx.x / (R / 4) * KPER, r = threadIdx.x % (R / 4) * 4;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int o = at(r + e, k);
+        if constexpr (KPER == 4) {
+          split3(f32x4{v[0][e], v[1][e], v[2][e], v[3][e]}, hi, mid, lo);
+          *reinterpret_cast<u32x2*>(lds + o) = hi;
+          *reinterpret_cast<u32x2*>(lds + kPlane + o) = mid;
+          *reinterpret_cast<u32x2*>(lds + 2 * kPlane + o) = lo;
+        } else {
+          split3(f32x4{v[0][e], v[1][e], 0.0f, 0.0f}, hi, mid, lo);
+          *reinterpret_cast<uint32_t*>(lds + o) = hi[0];
+          *reinterpret_cast<uint32_t*>(lds + kPlane + o) = mid[0];
+          *reinterpret_cast<uint32_t*>(lds + 2 * kPlane + o) = lo[0];
+        }
+      }
+    }
+  }
+  static SGNN_DEV s16x8 frag(const char* lds, int plane, int r) {
+    const int l = lane_id();
+    return *reinterpret_cast<const s16x8*>(lds + plane * kPlane + at(r + (l & 15), 8 * (l >> 4)));
+  }
+};
+
+// a b = sum of the parts' products; left out are mid lo, lo mid and lo lo, below 2^-22 of |a b| together.
+// An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
+// are not finite are formed once more in plain fp32 (`again`).
+template <bool ACOLS, bool BCOLS, int BM, int BN>
+__global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
+  constexpr int BK = 32, kThreads = 256, WM = 2, WN = 2;
+  constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
+  using TA = Tile32<BM, ACOLS>;
+  using TB = Tile32<BN, BCOLS>;
+  __shared__ __attribute__((aligned(16))) char sa[TA::kBytes], sb[TB::kBytes];
+  static_assert(16 * 16 * TN * 4 * WM * WN <= TA::kBytes, "the epilogue's buffers fit one tile");
+  const int w = wave_id(), wm = w / WN, wn = w % WN, l = lane_id();
+  int tm, tn;
+  tile_of(g, tm, tn);
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int split = g.nsplit > 1 ? blockIdx.z : 0;
+  const int64_t batch = g.nsplit > 1 ? 0 : blockIdx.z;
+  const float* A = static_cast<const float*>(g.A) + batch * g.batch_a;
+  const float* B = static_cast<const float*>(g.B) + batch * g.batch_b;
+  int first, last;
+  blocks_of(g, BK, split, first, last);
+
+  f32x4 acc[TM][TN];
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  f32x4 va[BM * BK / 4 / kThreads], vb[BN * BK / 4 / kThreads];
+  const auto fetch = [&](int blk) {
+    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
+  };
+  if (first < last) fetch(first);
+  for (int blk = first; blk < last; ++blk) {
+    TA::template put<kThreads>(sa, va);
+    TB::template put<kThreads>(sb, vb);
     __syncthreads();
+    if (blk + 1 < last) fetch(blk + 1);
+    s16x8 fb[TN][3];
 #pragma unroll
-    for (int s = 0; s < kKc / 2; ++s) {
-      const int k = 2 * s + (l >> 5);
-      acc = mfma32(As[k * kLdT + wm * 32 + (l & 31)], Bs[k * kLdT + wn * 32 + (l & 31)], acc);
+    for (int j = 0; j < TN; ++j)
+#pragma unroll
+      for (int p = 0; p < 3; ++p) fb[j][p] = TB::frag(sb, p, (wn * TN + j) * 16);
+#pragma unroll
+    for (int i = 0; i < TM; ++i) {
+      s16x8 fa[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) fa[p] = TA::frag(sa, p, (wm * TM + i) * 16);
+      // smallest products first
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][2], fa[0], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[2], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][1], fa[1], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][1], fa[0], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[1], acc[i][j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[0], acc[i][j]);
     }
     __syncthreads();
   }
-  const int64_t n = n0 + wn * 32 + (l & 31);
-  const T* res = static_cast<const T*>(g.res);
+  const int64_t k0 = (int64_t)first * BK, k1 = min((int64_t)last * BK, g.K);
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int64_t m = m0 + wm * 32 + crow(r, l >> 5);
-    if (m >= g.M || n >= g.N) continue;
-    float v = g.alpha * acc[r];
-    if (g.bias) v += to_float(static_cast<const T*>(g.bias)[n]);
-    if (g.z) static_cast<T*>(g.z)[m * g.N + n] = from_float<T>(v);
-    v = act_value<ACT>(v);
-    if (res) v += g.beta * to_float(res[b * g.batch_r + m * g.ldr + n]);
-    static_cast<T*>(g.C)[b * g.batch_c + m * g.ldc + n] = from_float<T>(v);
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const f32x4 v = acc[i][j];
+      // x - x is 0 for finite x alone
+      const float odd = (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+      if (odd == 0.0f) continue;
+      const int64_t m = m0 + (wm * TM + i) * 16 + (l & 15);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int64_t n = n0 + (wn * TN + j) * 16 + 4 * (l >> 4) + r;
+        if (v[r] - v[r] == 0.0f || m >= g.M || n >= g.N) continue;
+        float s = 0.0f;
+#pragma unroll 1
+        for (int64_t k = k0; k < k1; ++k)
+          s = fmaf(A[ACOLS ? k * g.lda + m : m * g.lda + k], B[BCOLS ? k * g.ldb + n : n * g.ldb + k], s);
+        acc[i][j][r] = s;
+      }
+    }
+  write_tile<float, TM, TN>(g, reinterpret_cast<float*>(sa) + w * 16 * 16 * TN, acc, batch, split, m0 + wm * TM * 16,
+                            n0 + wn * TN * 16);
+}
+
+// ----------------------------------------------------------------------------- split k
+// Partials summed in split order, then the epilogue; one thread per 16 bytes of output.
+template <typename T>
+__global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
+  constexpr int V = 16 / sizeof(T);
+  const int64_t per = (g.N + V - 1) / V, total = g.M * per;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
+    const int64_t m = t / per, n = (t - m * per) * V;
+    const int cnt = (int)min((int64_t)V, g.N - n);
+    float v[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = 0.0f;
+    const float* p = g.part + m * g.N + n;
+    for (int s = 0; s < g.nsplit; ++s, p += g.M * g.N) {
+      if (cnt == V) {
+        float u[4];
+#pragma unroll
+        for (int q = 0; q < V / 4; ++q) {
+          load_vec(p + 4 * q, u);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[4 * q + i] += u[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (i < cnt) v[i] += p[i];
+      }
+    }
+    finish<T>(g, 0, m, n, v, cnt);
   }
 }
 
-template <typename T>
-void launch(const Gemm& g, hipStream_t s) {
-  const dim3 grid((unsigned)((g.M + kTile - 1) / kTile), (unsigned)((g.N + kTile - 1) / kTile), (unsigned)g.batch);
-  switch (g.act) {
-    case SGNN_ACT_RELU: hipLaunchKernelGGL((k_gemm_typed<T, SGNN_ACT_RELU>), grid, dim3(kThreads), 0, s, g); break;
-    case SGNN_ACT_GELU: hipLaunchKernelGGL((k_gemm_typed<T, SGNN_ACT_GELU>), grid, dim3(kThreads), 0, s, g); break;
-    case SGNN_ACT_GELU_TANH: hipLaunchKernelGGL((k_gemm_typed<T, SGNN_ACT_GELU_TANH>), grid, dim3(kThreads), 0, s, g); break;
-    case SGNN_ACT_SILU: hipLaunchKernelGGL((k_gemm_typed<T, SGNN_ACT_SILU>), grid, dim3(kThreads), 0, s, g); break;
-    default: hipLaunchKernelGGL((k_gemm_typed<T, SGNN_ACT_NONE>), grid, dim3(kThreads), 0, s, g);
+// ----------------------------------------------------------------------------- choice and launch
+struct Plan {
+  int bm, bn, nsplit;
+};
+
+// The larger tile moves fewer bytes per product through LDS and L2, the smaller ones fill the 256 CUs sooner; long
+// k is split over workgroups where the tiles alone leave CUs idle.
+Plan plan_of(const Gemm& g) {
+  const auto tiles = [&](int bm, int bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn) * g.batch; };
+  const int bk = g.dtype == SGNN_F32 ? 32 : 64;
+  Plan p{64, 64, 1};
+  if (g.dtype != SGNN_F32 && tiles(256, 256) >= 192) p = {256, 256, 1};
+  else if (tiles(128, 128) >= 128 || g.K >= 2048) p = {128, 128, 1};
+  if (g.batch > 1) return p;
+  const int64_t blocks = (g.K + bk - 1) / bk, wgs = p.bm == 256 ? 256 : 512;
+  const int64_t want = wgs / std::max<int64_t>(1, tiles(p.bm, p.bn));
+  p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, blocks / 8, 256}));
+  return p;
+}
+
+template <typename T, bool AC, bool BC, int BM, int BN, int WM, int WN>
+void launch16(const GemmArgs& g, dim3 grid, bool direct, hipStream_t s) {
+  if (direct)
+    hipLaunchKernelGGL((k_gemm16<T, AC, BC, BM, BN, WM, WN, true>), grid, dim3(64 * WM * WN), 0, s, g);
+  else
+    hipLaunchKernelGGL((k_gemm16<T, AC, BC, BM, BN, WM, WN, false>), grid, dim3(64 * WM * WN), 0, s, g);
+}
+
+template <typename T, bool AC, bool BC>
+void launch_tiles(const GemmArgs& g, const Plan& p, dim3 grid, bool direct, hipStream_t s) {
+  if constexpr (std::is_same_v<T, float>) {
+    if (p.bm == 128)
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 128, 128>), grid, dim3(256), 0, s, g);
+    else
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 64, 64>), grid, dim3(256), 0, s, g);
+  } else {
+    if (p.bm == 256 && direct)
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 256, 256, 2, 4, true>), grid, dim3(512), 0, s, g);
+    else if (p.bm == 128)
+      launch16<T, AC, BC, 128, 128, 2, 2>(g, grid, direct, s);
+    else
+      launch16<T, AC, BC, 64, 64, 2, 2>(g, grid, direct, s);
   }
+}
+
+// Whether the direct-to-LDS loads serve an operand: 16-byte lines whose offsets within a tile fit 32 bits.
+bool direct_ok(const void* p, int64_t ld, int64_t batch, bool cols, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && batch % 8 == 0 && ld < (1 << 22) &&
+         (!cols || rows % 8 == 0);
 }
 
 }  // namespace
 
 namespace sgnn {
 
-size_t gemm_workspace_bytes(const Gemm&) { return 0; }
+size_t gemm_workspace_bytes(const Gemm& g) {
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0) return 0;
+  const int s = plan_of(g).nsplit;
+  return s > 1 ? sizeof(float) * (size_t)s * (size_t)g.M * (size_t)g.N : 0;
+}
 
-int gemm_run(const Gemm& g, void*, size_t, void* stream) {
+int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* stream) {
   if (g.M == 0 || g.N == 0 || g.batch == 0) return SGNN_OK;
-  if ((g.N + kTile - 1) / kTile > 65535 || (g.M + kTile - 1) / kTile > INT32_MAX || g.batch > 65535)
-    return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 4M columns or 65535 matrices");
+  Plan p = plan_of(g);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool direct = direct_ok(g.A, g.lda, g.batch_a, g.a_cols, g.M) && direct_ok(g.B, g.ldb, g.batch_b, g.b_cols, g.N);
+  if (!direct && p.bm == 256) p.bm = p.bn = 128;
+  const int64_t tm = (g.M + p.bm - 1) / p.bm, tn = (g.N + p.bn - 1) / p.bn;
+  if (tm > INT32_MAX / tn || g.batch > 65535 || g.K > (int64_t)INT32_MAX * 32)
+    return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k, or 65535 matrices");
+  GemmArgs a{g.A, g.B, g.bias, g.res, g.z, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
+             g.batch_b, g.batch_r, g.batch_c, g.act, p.nsplit, (int32_t)tm, (int32_t)tn, g.alpha, g.beta};
+  if (p.nsplit > 1) {
+    if (!workspace || workspace_bytes < gemm_workspace_bytes(g))
+      return set_error(SGNN_ERR_INVALID, "gemm: workspace too small");
+    a.part = static_cast<float*>(workspace);
+  }
+  const dim3 grid((unsigned)(tm * tn), 1, (unsigned)(p.nsplit > 1 ? p.nsplit : g.batch));
   with_type(g.dtype, [&](auto* t) {
-    launch<std::remove_pointer_t<decltype(t)>>(g, s);
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (!g.a_cols && !g.b_cols) launch_tiles<T, false, false>(a, p, grid, direct, s);
+    else if (!g.a_cols) launch_tiles<T, false, true>(a, p, grid, direct, s);
+    else launch_tiles<T, true, true>(a, p, grid, direct, s);
+    if (p.nsplit > 1) {
+      const int64_t items = g.M * ((g.N + 16 / (int64_t)sizeof(T) - 1) / (16 / (int64_t)sizeof(T)));
+      hipLaunchKernelGGL(k_gemm_join<T>, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256), 0, s, a);
+    }
     return 0;
   });
   return check_launch("gemm");

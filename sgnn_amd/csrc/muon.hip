@@ -41,12 +41,21 @@ __global__ __launch_bounds__(kThreads) void k_ns_end(const float* x, int rows, i
 
 size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-struct NsLayout {  // X twice, G and b G + c G^2
-  size_t x, g, total;
+Gemm product(int64_t M, int64_t N, int64_t K, bool b_cols) {
+  Gemm g;
+  g.dtype = SGNN_F32;
+  g.M = M, g.N = N, g.K = K, g.b_cols = b_cols;
+  return g;
+}
+
+struct NsLayout {  // X twice, G and b G + c G^2, the products' own
+  size_t x, g, gemm, total;
   NsLayout(int64_t m, int64_t n) {
     x = pad256(sizeof(float) * m * n);
     g = pad256(sizeof(float) * m * m);
-    total = 2 * x + 2 * g;
+    gemm = std::max({gemm_workspace_bytes(product(m, m, n, false)), gemm_workspace_bytes(product(m, m, m, false)),
+                     gemm_workspace_bytes(product(m, n, m, true))});
+    total = 2 * x + 2 * g + gemm;
   }
 };
 
@@ -82,6 +91,7 @@ extern "C" int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_
     const int64_t m = std::min(t.rows, t.cols), n = std::max(t.rows, t.cols);
     const NsLayout at(m, n);
     char* ws = static_cast<char*>(workspace);
+    char* gws = ws + 2 * at.x + 2 * at.g;
     float *x = reinterpret_cast<float*>(ws), *next = reinterpret_cast<float*>(ws + at.x);
     float *gram = reinterpret_cast<float*>(ws + 2 * at.x), *poly = reinterpret_cast<float*>(ws + 2 * at.x + at.g);
     with_type(dtype, [&](auto* p) {
@@ -91,26 +101,24 @@ extern "C" int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_
       return 0;
     });
     for (int32_t k = 0; k < steps; ++k) {
-      Gemm g;
-      g.dtype = SGNN_F32;
-      g.M = g.N = m, g.K = n;
+      Gemm g = product(m, m, n, false);
       g.A = g.B = x, g.lda = g.ldb = n;
       g.C = gram, g.ldc = m;
-      int st = gemm_run(g, nullptr, 0, stream);
+      int st = gemm_run(g, gws, at.gemm, stream);
       if (st != SGNN_OK) return st;
-      g.K = m;
+      g = product(m, m, m, false);
       g.A = g.B = gram, g.lda = g.ldb = m;   // G is symmetric: its rows are its columns
       g.alpha = c, g.beta = b;
       g.res = gram, g.ldr = m;
-      g.C = poly;
-      if ((st = gemm_run(g, nullptr, 0, stream)) != SGNN_OK) return st;
-      g.N = n;
-      g.A = poly;
-      g.B = x, g.ldb = n, g.b_cols = true;
-      g.alpha = 1.0f, g.beta = a;
+      g.C = poly, g.ldc = m;
+      if ((st = gemm_run(g, gws, at.gemm, stream)) != SGNN_OK) return st;
+      g = product(m, n, m, true);
+      g.A = poly, g.lda = m;
+      g.B = x, g.ldb = n;
+      g.beta = a;
       g.res = x, g.ldr = n;
       g.C = next, g.ldc = n;
-      if ((st = gemm_run(g, nullptr, 0, stream)) != SGNN_OK) return st;
+      if ((st = gemm_run(g, gws, at.gemm, stream)) != SGNN_OK) return st;
       std::swap(x, next);
     }
     with_type(dtype, [&](auto* p) {
