@@ -18,10 +18,7 @@ using namespace sgnn;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-// 16 bytes at any element's alignment (one global_load/store_dwordx4: unaligned access is on for this target)
-typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
 #define SGNN_LDS __attribute__((address_space(3)))
 #define SGNN_GLB __attribute__((address_space(1)))
@@ -51,25 +48,6 @@ SGNN_DEV void act_any(int32_t act, float* v, int n) {  // act is the same for ev
     case SGNN_ACT_SILU: act_n<SGNN_ACT_SILU>(v, n); break;
     default: break;
   }
-}
-
-// 16 bytes of T at any alignment <-> floats
-template <typename T>
-SGNN_DEV void load_vec(const T* p, float* v) {
-  constexpr int V = 16 / sizeof(T);
-  typedef T TV __attribute__((ext_vector_type(V)));
-  const TV t = __builtin_bit_cast(TV, (u32x4)*reinterpret_cast<const u32x4_any*>(p));
-#pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = to_float(t[i]);
-}
-template <typename T>
-SGNN_DEV void store_vec(T* p, const float* v) {
-  constexpr int V = 16 / sizeof(T);
-  typedef T TV __attribute__((ext_vector_type(V)));
-  TV t;
-#pragma unroll
-  for (int i = 0; i < V; ++i) t[i] = from_float<T>(v[i]);
-  *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, t);
 }
 
 // V consecutive outputs (m, n ..) of one lane; cnt of them exist.

@@ -8,40 +8,77 @@ namespace {
 using namespace sgnn;
 
 constexpr int kThreads = 256;
-constexpr int kRows = 128;  // rows per partial sum of db
 
-// Workgroup (bx, by): columns [256 bx, +256), rows [128 by, +128): dz = dy act'(z), and those rows' column sums
-// in row order.
+// How the pass over dy is cut: `lanes` threads side by side take a 16-byte piece each of a row, 256 / lanes rows at
+// once; `strips` such column strips, `blocks` row blocks.  About 2048 workgroups (8 per CU) keep enough loads in
+// flight for the memory's rate; the row blocks are also the partial sums of db, so there are at most 512.
+struct ActCut {
+  int lanes;
+  int64_t strips, blocks;
+  ActCut(size_t size, int64_t M, int64_t N) {
+    const int64_t pieces = (N * (int64_t)size + 15) / 16;
+    lanes = 16;
+    while (lanes < kThreads && lanes < pieces) lanes *= 2;
+    strips = (pieces + lanes - 1) / lanes;
+    const int64_t passes = (M + kThreads / lanes - 1) / (kThreads / lanes);
+    blocks = std::max<int64_t>(1, std::min({passes, (int64_t)512, (2048 + strips - 1) / strips}));
+  }
+};
+
+// dz = dy act'(z), and the column sums of this workgroup's rows: every thread over its rows in order, then the
+// threads of one column in order.  Reads dy and z, writes dz: bounded by memory.
 template <typename T, int ACT>
 __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const T* z, int64_t M, int64_t N,
-                                                      T* dz, float* partial) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= N) return;
-  const int64_t r0 = (int64_t)blockIdx.y * kRows, r1 = min(r0 + kRows, M);
-  float s = 0.0f;
-  for (int64_t r = r0; r < r1; ++r) {
-    float v = to_float(dy[r * ldd + c]);
-    if constexpr (ACT != SGNN_ACT_NONE) v *= act_slope<ACT>(to_float(z[r * N + c]));
-    if (dz) dz[r * N + c] = from_float<T>(v);
-    s += v;
+                                                      int lanes, T* dz, float* partial) {
+  constexpr int V = 16 / sizeof(T);
+  __shared__ float sums[kThreads * V];
+  const int rows = kThreads / lanes, lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
+  const int64_t c = ((int64_t)blockIdx.x * lanes + lane) * V;
+  const int cnt = (int)min((int64_t)V, N - c);
+  float s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = 0.0f;
+  if (cnt > 0) {
+    const int64_t step = (int64_t)gridDim.y * rows;
+#pragma unroll 2
+    for (int64_t r = (int64_t)blockIdx.y * rows + row; r < M; r += step) {
+      float v[V], t[V];
+      load_some<V>(dy + r * ldd + c, cnt, v);
+      if constexpr (ACT != SGNN_ACT_NONE) {
+        load_some<V>(z + r * N + c, cnt, t);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] *= act_slope<ACT>(t[i]);
+        store_some<V>(dz + r * N + c, cnt, v);
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += v[i];
+    }
   }
-  if (partial) partial[(int64_t)blockIdx.y * N + c] = s;
+  if (!partial) return;
+#pragma unroll
+  for (int i = 0; i < V; ++i) sums[threadIdx.x * V + i] = s[i];
+  __syncthreads();
+  if (row != 0 || cnt <= 0) return;
+  for (int q = 1; q < rows; ++q)
+#pragma unroll
+    for (int i = 0; i < V; ++i) s[i] += sums[(q * lanes + lane) * V + i];
+  float* o = partial + (int64_t)blockIdx.y * N + c;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < cnt) o[i] = s[i];
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_sum_partials(const float* partial, int64_t nblk, int64_t N, T* out) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= N) return;
-  float s = 0.0f;
-  for (int64_t b = 0; b < nblk; ++b) s += partial[b * N + c];
-  out[c] = from_float<T>(s);
+__global__ __launch_bounds__(kSumThreads) void k_bias_grad(const float* partial, int64_t nblk, int64_t N, T* out) {
+  sum_partials(partial, nblk, N, [&](int64_t c, float s) { out[c] = from_float<T>(s); });
 }
 
 template <typename T>
-void launch_act_bwd(int32_t act, dim3 grid, hipStream_t s, const T* dy, int64_t ldd, const T* z, int64_t M, int64_t N,
-                    T* dz, float* partial) {
+void launch_act_bwd(int32_t act, const ActCut& cut, hipStream_t s, const T* dy, int64_t ldd, const T* z, int64_t M,
+                    int64_t N, T* dz, float* partial) {
   const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, s, dy, ldd, z, M, N, dz, partial);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)cut.strips, (unsigned)cut.blocks), dim3(kThreads), 0, s, dy, ldd, z, M,
+                       N, cut.lanes, dz, partial);
   };
   if (act == SGNN_ACT_RELU) go(k_act_bwd<T, SGNN_ACT_RELU>);
   else if (act == SGNN_ACT_GELU) go(k_act_bwd<T, SGNN_ACT_GELU>);
@@ -79,7 +116,7 @@ struct BwdLayout {
   size_t dz, partial, gemm, total;
   BwdLayout(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
     dz = act == SGNN_ACT_NONE ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
-    partial = pad256(sizeof(float) * (size_t)((M + kRows - 1) / kRows) * (size_t)N);
+    partial = pad256(sizeof(float) * (size_t)ActCut(dtype_size(dtype), M, N).blocks * (size_t)N);
     gemm = std::max(gemm_workspace_bytes(dgrad(dtype, M, N, K)), gemm_workspace_bytes(wgrad(dtype, M, N, K)));
     total = dz + partial + gemm;
   }
@@ -132,26 +169,21 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   hipStream_t s = static_cast<hipStream_t>(stream);
   const BwdLayout at(dtype, std::max<int64_t>(M, 0), N, K, act);
   char* ws = static_cast<char*>(workspace);
-  const int64_t nblk = (M + kRows - 1) / kRows;
   const void* up = dy;      // dz and its leading dimension
   int64_t ldu = ldd;
-  if (N > 0 && M > 0 && (act != SGNN_ACT_NONE || db)) {
-    if (nblk > 65535) return set_error(SGNN_ERR_UNSUPPORTED, "linear_bwd: more than 8M rows");
+  if (N > 0 && (act != SGNN_ACT_NONE || db))
     with_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
-      T* dz = act == SGNN_ACT_NONE ? nullptr : reinterpret_cast<T*>(ws);
-      launch_act_bwd<T>(act, dim3((unsigned)((N + kThreads - 1) / kThreads), (unsigned)nblk), s,
-                        static_cast<const T*>(dy), ldd, static_cast<const T*>(z), M, N, dz,
-                        db ? reinterpret_cast<float*>(ws + at.dz) : nullptr);
-      return 0;
-    });
-    if (act != SGNN_ACT_NONE) up = ws, ldu = N;
-  }
-  if (db && N > 0)
-    with_type(dtype, [&](auto* t) {
-      using T = std::remove_pointer_t<decltype(t)>;
-      hipLaunchKernelGGL(k_sum_partials<T>, dim3((unsigned)((N + kThreads - 1) / kThreads)), dim3(kThreads), 0, s,
-                         reinterpret_cast<const float*>(ws + at.dz), nblk, N, static_cast<T*>(db));
+      const ActCut cut(sizeof(T), M, N);
+      float* partial = db ? reinterpret_cast<float*>(ws + at.dz) : nullptr;
+      if (M > 0) {
+        launch_act_bwd<T>(act, cut, s, static_cast<const T*>(dy), ldd, static_cast<const T*>(z), M, N,
+                          reinterpret_cast<T*>(ws), partial);
+        if (act != SGNN_ACT_NONE) up = ws, ldu = N;
+      }
+      if (db)
+        hipLaunchKernelGGL(k_bias_grad<T>, dim3(sum_grid(N)), dim3(kSumThreads), 0, s, partial,
+                           M > 0 ? cut.blocks : 0, N, static_cast<T*>(db));
       return 0;
     });
   const int st = check_launch("linear_bwd");

@@ -5,41 +5,211 @@
 namespace {
 using namespace sgnn;
 
-constexpr int kThreads = 256;
-constexpr int kWavesPer = kThreads / 64;
+// Rows are held in registers: G lanes per row (16, 64, or a workgroup of 256 or 512), NC 16-byte pieces per lane,
+// piece j of lane i at column (j G + i) V.  Forward and backward read every input once and write every output once:
+// both are bounded by memory.
+constexpr int threads_of(int G) { return G > 256 ? G : 256; }
 
-SGNN_DEV float wave_sum(float v) {
+// Sum over a row's G lanes; `red` is 2 x 16 floats of LDS, `turn` the half to use (the other may still be read).
+template <int G>
+SGNN_DEV float group_sum(float v, float* red, int turn) {
+  if constexpr (G <= 64) return lanes_sum<G>(v);
+  v = lanes_sum<64>(v);
+  float* r = red + 16 * turn;
+  if (lane_id() == 0) r[wave_id()] = v;
+  __syncthreads();
+  float s = 0.0f;
 #pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o, 64);
-  return v;
+  for (int w = 0; w < G / 64; ++w) s += r[w];
+  return s;
 }
 
-// One wave per row: mean, then the variance of the differences (two passes), then the outputs.
+// Mean, then the variance of the differences (both from registers), then the outputs; kRows rows per group of lanes
+// in turn, so that gamma and beta are read once for them.
+template <typename T, typename W, int G, int NC>
+__global__ __launch_bounds__(threads_of(G)) void k_norm(const T* x, int64_t ldx, int64_t n, int width, const W* gamma,
+                                                        const W* beta, const T* residual, int64_t ldr, float eps, T* y,
+                                                        float* mean_out, float* rstd_out, int rows_per) {
+  constexpr int V = 16 / sizeof(T), kGroups = threads_of(G) / G;
+  __shared__ float red[32];
+  const int i = threadIdx.x % G;
+  float ga[NC][V], be[NC][V];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int c = (j * G + i) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ga[j][e] = 1.0f, be[j][e] = 0.0f;
+    if (gamma) load_some<V>(gamma + c, width - c, ga[j]);
+    if (beta) load_some<V>(beta + c, width - c, be[j]);
+  }
+  const int64_t r0 = (int64_t)blockIdx.x * rows_per * kGroups + threadIdx.x / G;
+  for (int q = 0; q < rows_per; ++q) {
+    const int64_t r = r0 + (int64_t)q * kGroups;
+    if (r >= n) break;  // the lanes of one row leave together
+    float v[NC][V];
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = (j * G + i) * V;
+      load_some<V>(x + r * ldx + c, width - c, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) s += v[j][e];
+    const float mean = group_sum<G>(s, red, 0) / width;
+    s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        v[j][e] -= mean;
+        if ((j * G + i) * V + e < width) s += v[j][e] * v[j][e];
+      }
+    const float rstd = 1.0f / sqrtf(group_sum<G>(s, red, 1) / width + eps);
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = (j * G + i) * V;
+      if (c >= width) continue;
+      float o[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = v[j][e] * rstd * ga[j][e] + be[j][e];
+      if (residual) {
+        float t[V];
+        load_some<V>(residual + r * ldr + c, width - c, t);
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] += t[e];
+      }
+      store_some<V>(y + r * width + c, width - c, o);
+    }
+    if (i == 0) {
+      if (mean_out) mean_out[r] = mean;
+      if (rstd_out) rstd_out[r] = rstd;
+    }
+  }
+}
+
+// dx, and this workgroup's share of dgamma and dbeta: every lane sums its own columns over its rows (rows blockIdx,
+// + gridDim ... in order), the groups of one workgroup are added in order in LDS, and the workgroups' sums go to
+// partial [workgroup][2][width].  The next row is loaded before this one's sums are waited for.
+template <typename T, typename W, int G, int NC>
+__global__ __launch_bounds__(threads_of(G)) void k_norm_bwd(const T* dy, int64_t ldd, const T* x, int64_t ldx,
+                                                            const float* mean, const float* rstd, const W* gamma,
+                                                            int64_t n, int width, T* dx, float* partial) {
+  constexpr int V = 16 / sizeof(T), kGroups = threads_of(G) / G;
+  __shared__ float red[2][32];
+  __shared__ float join[kGroups > 1 ? (kGroups - 1) * G * NC * V : 1];
+  const int i = threadIdx.x % G, grp = threadIdx.x / G;
+  float ga[NC][V], dg[NC][V], db[NC][V];
+#pragma unroll
+  for (int j = 0; j < NC; ++j) {
+    const int c = (j * G + i) * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) ga[j][e] = 1.0f, dg[j][e] = 0.0f, db[j][e] = 0.0f;
+    if (gamma) load_some<V>(gamma + c, width - c, ga[j]);
+  }
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  float xv[NC][V], up[NC][V], mu = 0.0f, rs = 0.0f;
+  const auto load = [&](int64_t r) {
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = (j * G + i) * V;
+      load_some<V>(x + r * ldx + c, width - c, xv[j]);
+      load_some<V>(dy + r * ldd + c, width - c, up[j]);
+    }
+    mu = mean[r], rs = rstd[r];
+  };
+  int64_t r = (int64_t)blockIdx.x * kGroups + grp;
+  if (r < n) load(r);
+  for (int turn = 0; r < n; r += step, turn ^= 1) {
+    float hat[NC][V], g[NC][V];
+    float sg = 0.0f, sgh = 0.0f;
+    const float rnow = rs;
+#pragma unroll
+    for (int j = 0; j < NC; ++j)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // columns past the row read as 0 in dy: nothing of theirs is summed
+        hat[j][e] = (xv[j][e] - mu) * rs;
+        g[j][e] = up[j][e] * ga[j][e];
+        dg[j][e] += up[j][e] * hat[j][e];
+        db[j][e] += up[j][e];
+        sg += g[j][e];
+        sgh += g[j][e] * hat[j][e];
+      }
+    if (r + step < n) load(r + step);
+    if (dx) {
+      sg = group_sum<G>(sg, red[0], turn) / width;
+      sgh = group_sum<G>(sgh, red[1], turn) / width;
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int c = (j * G + i) * V;
+        if (c >= width) continue;
+        float o[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) o[e] = rnow * (g[j][e] - sg - hat[j][e] * sgh);
+        store_some<V>(dx + r * width + c, width - c, o);
+      }
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    float(&a)[NC][V] = which == 0 ? dg : db;
+    if constexpr (kGroups > 1) {
+      if (grp > 0)
+#pragma unroll
+        for (int j = 0; j < NC; ++j)
+#pragma unroll
+          for (int e = 0; e < V; ++e) join[((grp - 1) * NC * V + j * V + e) * G + i] = a[j][e];
+      __syncthreads();
+      if (grp == 0)
+        for (int q = 0; q < kGroups - 1; ++q)
+#pragma unroll
+          for (int j = 0; j < NC; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) a[j][e] += join[(q * NC * V + j * V + e) * G + i];
+      __syncthreads();
+    }
+    if (grp == 0)
+#pragma unroll
+      for (int j = 0; j < NC; ++j) {
+        const int c = (j * G + i) * V;
+        if (c < width) store_some<V>(partial + ((int64_t)blockIdx.x * 2 + which) * width + c, width - c, a[j]);
+      }
+  }
+}
+
+// Rows longer than 512 lanes hold: a workgroup per row, read again for each of the steps (from L2 where it is still
+// there).
+constexpr int kMaxWidth = 8192, kWide = 1024;
+
+template <typename T>
+SGNN_DEV float at_or(const T* p, int c, float none) {
+  return p ? to_float(p[c]) : none;
+}
+
 template <typename T, typename W>
-__global__ __launch_bounds__(kThreads) void k_norm(const T* x, int64_t ldx, int64_t n, int width, const W* gamma,
-                                                   const W* beta, const T* residual, int64_t ldr, float eps, T* y,
-                                                   float* mean_out, float* rstd_out) {
-  const int l = lane_id();
-  const int64_t nw = (int64_t)gridDim.x * kWavesPer;
-  for (int64_t r = (int64_t)blockIdx.x * kWavesPer + wave_id(); r < n; r += nw) {
+__global__ __launch_bounds__(kWide) void k_norm_wide(const T* x, int64_t ldx, int64_t n, int width, const W* gamma,
+                                                     const W* beta, const T* residual, int64_t ldr, float eps, T* y,
+                                                     float* mean_out, float* rstd_out) {
+  __shared__ float red[32];
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const T* p = x + r * ldx;
     float s = 0.0f;
-    for (int c = l; c < width; c += 64) s += to_float(p[c]);
-    const float mean = wave_sum(s) / width;
-    float v = 0.0f;
-    for (int c = l; c < width; c += 64) {
+    for (int c = threadIdx.x; c < width; c += kWide) s += to_float(p[c]);
+    const float mean = group_sum<kWide>(s, red, 0) / width;
+    s = 0.0f;
+    for (int c = threadIdx.x; c < width; c += kWide) {
       const float d = to_float(p[c]) - mean;
-      v += d * d;
+      s += d * d;
     }
-    const float rstd = 1.0f / sqrtf(wave_sum(v) / width + eps);
-    for (int c = l; c < width; c += 64) {
-      float o = (to_float(p[c]) - mean) * rstd;
-      if (gamma) o *= to_float(gamma[c]);
-      if (beta) o += to_float(beta[c]);
-      if (residual) o += to_float(residual[r * ldr + c]);
-      y[r * width + c] = from_float<T>(o);
+    const float rstd = 1.0f / sqrtf(group_sum<kWide>(s, red, 1) / width + eps);
+    for (int c = threadIdx.x; c < width; c += kWide) {
+      const float o = (to_float(p[c]) - mean) * rstd * at_or(gamma, c, 1.0f) + at_or(beta, c, 0.0f);
+      y[r * width + c] = from_float<T>(o + (residual ? to_float(residual[r * ldr + c]) : 0.0f));
     }
-    if (l == 0) {
+    if (threadIdx.x == 0) {
       if (mean_out) mean_out[r] = mean;
       if (rstd_out) rstd_out[r] = rstd;
     }
@@ -47,39 +217,37 @@ __global__ __launch_bounds__(kThreads) void k_norm(const T* x, int64_t ldx, int6
 }
 
 template <typename T, typename W>
-__global__ __launch_bounds__(kThreads) void k_norm_dx(const T* dy, int64_t ldd, const T* x, int64_t ldx,
-                                                      const float* mean, const float* rstd, const W* gamma, int64_t n,
-                                                      int width, T* dx) {
-  const int l = lane_id();
-  const int64_t nw = (int64_t)gridDim.x * kWavesPer;
-  for (int64_t r = (int64_t)blockIdx.x * kWavesPer + wave_id(); r < n; r += nw) {
+__global__ __launch_bounds__(kWide) void k_norm_bwd_wide(const T* dy, int64_t ldd, const T* x, int64_t ldx,
+                                                         const float* mean, const float* rstd, const W* gamma,
+                                                         int64_t n, int width, T* dx) {
+  __shared__ float red[2][32];
+  int turn = 0;
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x, turn ^= 1) {
     const float mu = mean[r], rs = rstd[r];
     float sg = 0.0f, sgh = 0.0f;
-    for (int c = l; c < width; c += 64) {
-      const float g = to_float(dy[r * ldd + c]) * (gamma ? to_float(gamma[c]) : 1.0f);
+    for (int c = threadIdx.x; c < width; c += kWide) {
+      const float g = to_float(dy[r * ldd + c]) * at_or(gamma, c, 1.0f);
       sg += g;
       sgh += g * (to_float(x[r * ldx + c]) - mu) * rs;
     }
-    sg = wave_sum(sg) / width;
-    sgh = wave_sum(sgh) / width;
-    for (int c = l; c < width; c += 64) {
-      const float g = to_float(dy[r * ldd + c]) * (gamma ? to_float(gamma[c]) : 1.0f);
+    sg = group_sum<kWide>(sg, red[0], turn) / width;
+    sgh = group_sum<kWide>(sgh, red[1], turn) / width;
+    for (int c = threadIdx.x; c < width; c += kWide) {
+      const float g = to_float(dy[r * ldd + c]) * at_or(gamma, c, 1.0f);
       dx[r * width + c] = from_float<T>(rs * (g - sg - (to_float(x[r * ldx + c]) - mu) * rs * sgh));
     }
   }
 }
 
-constexpr int kRows = 128;  // rows per partial sum
-
+// One thread per column over every gridDim.x-th row.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_norm_partials(const T* dy, int64_t ldd, const T* x, int64_t ldx,
-                                                            const float* mean, const float* rstd, int64_t n, int width,
-                                                            float* partial) {
-  const int c = blockIdx.y * kThreads + threadIdx.x;
+__global__ __launch_bounds__(256) void k_norm_sums_wide(const T* dy, int64_t ldd, const T* x, int64_t ldx,
+                                                        const float* mean, const float* rstd, int64_t n, int width,
+                                                        float* partial) {
+  const int c = blockIdx.y * 256 + threadIdx.x;
   if (c >= width) return;
-  const int64_t r0 = (int64_t)blockIdx.x * kRows, r1 = min(r0 + kRows, n);
   float dg = 0.0f, db = 0.0f;
-  for (int64_t r = r0; r < r1; ++r) {
+  for (int64_t r = blockIdx.x; r < n; r += gridDim.x) {
     const float g = to_float(dy[r * ldd + c]);
     dg += g * (to_float(x[r * ldx + c]) - mean[r]) * rstd[r];
     db += g;
@@ -89,20 +257,48 @@ __global__ __launch_bounds__(kThreads) void k_norm_partials(const T* dy, int64_t
 }
 
 template <typename W>
-__global__ __launch_bounds__(kThreads) void k_norm_reduce(const float* partial, int64_t nblk, int width, W* dgamma,
-                                                          W* dbeta) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= 2 * width) return;
-  float s = 0.0f;
-  for (int64_t b = 0; b < nblk; ++b) s += partial[b * 2 * width + c];
-  if (c < width) {
-    if (dgamma) dgamma[c] = from_float<W>(s);
-  } else if (dbeta) {
-    dbeta[c - width] = from_float<W>(s);
-  }
+__global__ __launch_bounds__(kSumThreads) void k_norm_reduce(const float* partial, int64_t nblk, int width, W* dgamma,
+                                                             W* dbeta) {
+  sum_partials(partial, nblk, 2 * (int64_t)width, [&](int64_t c, float s) {
+    if (c < width) {
+      if (dgamma) dgamma[c] = from_float<W>(s);
+    } else if (dbeta) {
+      dbeta[c - width] = from_float<W>(s);
+    }
+  });
 }
 
-unsigned row_grid(int64_t n) { return (unsigned)std::min<int64_t>((n + kWavesPer - 1) / kWavesPer, 4096); }
+// Lanes per row and pieces per lane: the fewest lanes that leave a lane at most 16 values (the backward pass holds six
+// arrays of them: 150 registers, three waves per SIMD).
+struct NormCut {
+  int G, NC;  // G = 0: the wide kernels
+  NormCut(size_t size, int width) {
+    G = width <= 256 ? 16 : width <= 1024 ? 64 : width <= 4096 ? 256 : width <= kMaxWidth ? 512 : 0;
+    const int per = G ? (width + G - 1) / G * (int)size : 0;  // bytes per lane
+    NC = per <= 16 ? 1 : per <= 32 ? 2 : 4;
+  }
+};
+
+// Workgroups of the backward pass, which are also the partial sums: enough for the memory's rate (8 of 256 threads
+// per CU for short rows; 2 for long ones, whose partial rows are as long), never more than there are rows for.
+int64_t bwd_blocks(const NormCut& cut, int64_t n) {
+  const int64_t groups = cut.G == 0 || cut.G > 256 ? 1 : 256 / cut.G;
+  const int64_t most = cut.G == 16 ? 2048 : cut.G == 64 ? 1024 : cut.G == 256 ? 512 : 256;
+  return std::max<int64_t>(1, std::min(most, (n + groups - 1) / groups));
+}
+
+template <typename T, typename F>
+void with_cut(const NormCut& cut, F f) {
+  const auto nc = [&](auto g) {
+    if (cut.NC == 1) f(g, std::integral_constant<int, 1>{});
+    else if (cut.NC == 2) f(g, std::integral_constant<int, 2>{});
+    else if constexpr (sizeof(T) == 4) f(g, std::integral_constant<int, 4>{});  // 16 values are two pieces of 16 bits
+  };
+  if (cut.G == 16) nc(std::integral_constant<int, 16>{});
+  else if (cut.G == 64) nc(std::integral_constant<int, 64>{});
+  else if (cut.G == 256) nc(std::integral_constant<int, 256>{});
+  else nc(std::integral_constant<int, 512>{});
+}
 
 template <typename F>
 int with_types(int32_t dtype, int32_t wdtype, F f) {
@@ -125,10 +321,23 @@ extern "C" int sgnn_norm(int32_t dtype, int32_t wdtype, const void* x, int64_t l
   with_types(dtype, wdtype, [&](auto* t, auto* w) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
-    hipLaunchKernelGGL((k_norm<T, W>), dim3(row_grid(n)), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
-                       static_cast<const T*>(x), ldx, n, width, static_cast<const W*>(gamma),
-                       static_cast<const W*>(beta), static_cast<const T*>(residual), ldr, eps, static_cast<T*>(y),
-                       mean, rstd);
+    const NormCut cut(sizeof(T), width);
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const T *in = static_cast<const T*>(x), *res = static_cast<const T*>(residual);
+    const W *ga = static_cast<const W*>(gamma), *be = static_cast<const W*>(beta);
+    T* out = static_cast<T*>(y);
+    if (cut.G == 0) {
+      hipLaunchKernelGGL((k_norm_wide<T, W>), dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(kWide), 0, s, in, ldx, n,
+                         width, ga, be, res, ldr, eps, out, mean, rstd);
+      return 0;
+    }
+    with_cut<T>(cut, [&](auto g, auto nc) {
+      constexpr int G = decltype(g)::value, NC = decltype(nc)::value, kGroups = threads_of(G) / G;
+      // several rows per group once there are enough for 16 workgroups on every CU
+      const int64_t per = std::max<int64_t>(1, std::min<int64_t>(4, n / (kGroups * 4096)));
+      hipLaunchKernelGGL((k_norm<T, W, G, NC>), dim3((unsigned)((n + kGroups * per - 1) / (kGroups * per))),
+                         dim3(threads_of(G)), 0, s, in, ldx, n, width, ga, be, res, ldr, eps, out, mean, rstd, (int)per);
+    });
     return 0;
   });
   return check_launch("norm");
@@ -136,7 +345,8 @@ extern "C" int sgnn_norm(int32_t dtype, int32_t wdtype, const void* x, int64_t l
 
 extern "C" size_t sgnn_norm_bwd_workspace_bytes(int64_t n, int32_t width) {
   if (n <= 0 || width <= 0) return 0;
-  return sizeof(float) * 2 * (size_t)width * (size_t)((n + kRows - 1) / kRows);
+  const auto blocks = [&](size_t size) { return bwd_blocks(NormCut(size, width), n); };
+  return sizeof(float) * 2 * (size_t)width * (size_t)std::max(blocks(2), blocks(4));
 }
 
 extern "C" int sgnn_norm_bwd(int32_t dtype, int32_t wdtype, const void* dy, int64_t ldd, const void* x, int64_t ldx,
@@ -153,21 +363,32 @@ extern "C" int sgnn_norm_bwd(int32_t dtype, int32_t wdtype, const void* dy, int6
   if (sums && n > 0 && (!workspace || workspace_bytes < sgnn_norm_bwd_workspace_bytes(n, width)))
     return set_error(SGNN_ERR_INVALID, "norm_bwd: workspace smaller than sgnn_norm_bwd_workspace_bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t nblk = (n + kRows - 1) / kRows;
-  float* part = static_cast<float*>(workspace);
+  float* part = sums ? static_cast<float*>(workspace) : nullptr;
   with_types(dtype, wdtype, [&](auto* t, auto* w) {
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
+    const NormCut cut(sizeof(T), width);
+    const int64_t nblk = n > 0 ? bwd_blocks(cut, n) : 0;
     const T *up = static_cast<const T*>(dy), *in = static_cast<const T*>(x);
-    if (dx && n > 0)
-      hipLaunchKernelGGL((k_norm_dx<T, W>), dim3(row_grid(n)), dim3(kThreads), 0, s, up, ldd, in, ldx, mean, rstd,
-                         static_cast<const W*>(gamma), n, width, static_cast<T*>(dx));
-    if (sums && n > 0)
-      hipLaunchKernelGGL(k_norm_partials<T>, dim3((unsigned)nblk, (unsigned)((width + kThreads - 1) / kThreads)),
-                         dim3(kThreads), 0, s, up, ldd, in, ldx, mean, rstd, n, width, part);
+    const W* ga = static_cast<const W*>(gamma);
+    T* out = static_cast<T*>(dx);
+    if (n > 0 && cut.G == 0) {
+      if (dx)
+        hipLaunchKernelGGL((k_norm_bwd_wide<T, W>), dim3((unsigned)std::min<int64_t>(n, 4096)), dim3(kWide), 0, s, up,
+                           ldd, in, ldx, mean, rstd, ga, n, width, out);
+      if (sums)
+        hipLaunchKernelGGL(k_norm_sums_wide<T>, dim3((unsigned)nblk, (unsigned)((width + 255) / 256)), dim3(256), 0, s,
+                           up, ldd, in, ldx, mean, rstd, n, width, part);
+    } else if (n > 0 && (dx || sums)) {
+      with_cut<T>(cut, [&](auto g, auto nc) {
+        constexpr int G = decltype(g)::value, NC = decltype(nc)::value;
+        hipLaunchKernelGGL((k_norm_bwd<T, W, G, NC>), dim3((unsigned)nblk), dim3(threads_of(G)), 0, s, up, ldd, in, ldx,
+                           mean, rstd, ga, n, width, out, part);
+      });
+    }
     if (sums)
-      hipLaunchKernelGGL(k_norm_reduce<W>, dim3((unsigned)((2 * (int64_t)width + kThreads - 1) / kThreads)),
-                         dim3(kThreads), 0, s, part, nblk, width, static_cast<W*>(dgamma), static_cast<W*>(dbeta));
+      hipLaunchKernelGGL(k_norm_reduce<W>, dim3(sum_grid(2 * (int64_t)width)), dim3(kSumThreads), 0, s, part, nblk,
+                         width, static_cast<W*>(dgamma), static_cast<W*>(dbeta));
     return 0;
   });
   return check_launch("norm_bwd");

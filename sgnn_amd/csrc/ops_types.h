@@ -24,6 +24,103 @@ SGNN_DEV T from_float(float v) {
   return (T)v;
 }
 
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+// 16 bytes at any element's alignment (one global_load/store_dwordx4: unaligned access is on for this target)
+typedef u32x4 u32x4_any __attribute__((aligned(2)));
+
+// 16 bytes of T at any alignment <-> floats
+template <typename T>
+SGNN_DEV void load_vec(const T* p, float* v) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  const TV t = __builtin_bit_cast(TV, (u32x4)*reinterpret_cast<const u32x4_any*>(p));
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_float(t[i]);
+}
+template <typename T>
+SGNN_DEV void store_vec(T* p, const float* v) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  TV t;
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = from_float<T>(v[i]);
+  *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, t);
+}
+// N values of T, the first cnt of them there (the others read as 0, are not written).
+template <int N, typename T>
+SGNN_DEV void load_some(const T* p, int cnt, float (&v)[N]) {
+  constexpr int V = 16 / sizeof(T);
+  if (cnt >= N) {
+#pragma unroll
+    for (int i = 0; i < N; i += V) load_vec(p + i, v + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < cnt ? to_float(p[i]) : 0.0f;
+  }
+}
+template <int N, typename T>
+SGNN_DEV void store_some(T* p, int cnt, const float (&v)[N]) {
+  constexpr int V = 16 / sizeof(T);
+  if (cnt >= N) {
+#pragma unroll
+    for (int i = 0; i < N; i += V) store_vec(p + i, v + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (i < cnt) p[i] = from_float<T>(v[i]);
+  }
+}
+
+// Sum over groups of G consecutive lanes (16, 32 or 64), the same in each of them: within 16 lanes by DPP (xor 1, xor
+// 2, then the two mirrors), rows of 16 and halves of 32 by the swap instructions -- no LDS.
+template <int CTRL>
+SGNN_DEV float dpp_mov(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int G>
+SGNN_DEV float lanes_sum(float v) {
+  v += dpp_mov<0xb1>(v);   // quad_perm 1, 0, 3, 2
+  v += dpp_mov<0x4e>(v);   // quad_perm 2, 3, 0, 1
+  v += dpp_mov<0x141>(v);  // row_half_mirror
+  v += dpp_mov<0x140>(v);  // row_mirror
+  if constexpr (G >= 32) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a = s[0], b = s[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  if constexpr (G >= 64) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v);
+    const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t a = s[0], b = s[1];
+    v = __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+  }
+  return v;
+}
+
+// out[c] = sum over the nblk partial rows of `cols` fp32 values, 16 columns per workgroup of 1024 threads: each of 64
+// groups of 16 lanes takes every 64th row, then the groups' sums in group order.  Bounded by the latency of its
+// nblk / 64 dependent-free loads per lane: a few us up to 2048 rows.  f(c, sum) stores.
+constexpr int kSumThreads = 1024, kSumCols = 16;
+template <typename F>
+SGNN_DEV void sum_partials(const float* partial, int64_t nblk, int64_t cols, F f) {
+  __shared__ float part[kSumThreads / kSumCols][kSumCols + 1];
+  const int g = threadIdx.x / kSumCols, i = threadIdx.x % kSumCols;
+  const int64_t c = (int64_t)blockIdx.x * kSumCols + i;
+  float s = 0.0f;
+  if (c < cols)
+#pragma unroll 8
+    for (int64_t b = g; b < nblk; b += kSumThreads / kSumCols) s += partial[b * cols + c];
+  part[g][i] = s;
+  __syncthreads();
+  if (g != 0 || c >= cols) return;
+  s = 0.0f;
+#pragma unroll 8
+  for (int r = 0; r < kSumThreads / kSumCols; ++r) s += part[r][i];
+  f(c, s);
+}
+inline unsigned sum_grid(int64_t cols) { return (unsigned)((cols + kSumCols - 1) / kSumCols); }
+
 inline size_t dtype_size(int32_t dtype) { return dtype == SGNN_F32 ? 4 : 2; }
 inline bool dtype_ok(int32_t dtype) { return dtype == SGNN_F32 || dtype == SGNN_BF16 || dtype == SGNN_F16; }
 
