@@ -11,17 +11,12 @@
 // 16-byte pieces of rows at any alignment.
 #include "gemm.h"
 
-#include "ops_types.h"
+#include "gemm_tile.h"
 
 namespace {
 using namespace sgnn;
 
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-#define SGNN_LDS __attribute__((address_space(3)))
-#define SGNN_GLB __attribute__((address_space(1)))
 
 struct GemmArgs {
   const void *A, *B, *bias, *res;
@@ -180,109 +175,6 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 }
 
 // ----------------------------------------------------------------------------- 16-bit operands
-template <typename T>
-SGNN_DEV f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
-  typedef T T8 __attribute__((ext_vector_type(8)));
-  if constexpr (std::is_same_v<T, bf16_t>)
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
-}
-
-// One operand's tile in LDS: R rows (m or n) by BK of k, in 16-byte chunks.
-//   rows layout (k contiguous in memory): row r's chunk c (8 k) at slot c ^ swizzle(r)
-//   cols layout (m / n contiguous): k's chunk c (8 rows) at slot c ^ 2 h(k); read back transposed
-// The swizzles put the pieces that one LDS instruction touches at a time on different banks.
-template <int R, int BK, bool COLS>
-struct Tile16 {
-  static constexpr int kChunks = COLS ? R / 8 : BK / 8;  // chunks per line of memory (a row, or a k)
-  static constexpr int kLines = COLS ? BK : R;
-  static constexpr int kBytes = R * BK * 2;
-  static SGNN_DEV int swizzle(int line) {
-    if constexpr (COLS) return (2 * ((line & 3) | ((line >> 1) & 4))) & (kChunks - 1);
-    return kChunks == 8 ? (line >> 1) & 7 : (line >> 2) & 3;
-  }
-
-  // Chunk q of the tile (in LDS order) holds memory's line q / kChunks, chunk (q % kChunks) ^ swizzle.  offsets():
-  // this lane's chunks' bytes from the tile's first element, the same for every block of k.  Lines and chunks past
-  // the last row read another one's data: their outputs are not stored.
-  template <int THREADS, int KPER>
-  static SGNN_DEV void offsets(uint32_t (&o)[KPER], int64_t ld, int64_t rows, int64_t r0) {
-#pragma unroll
-    for (int i = 0; i < KPER; ++i) {
-      const int q = i * THREADS + threadIdx.x;
-      const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
-      const int left = (int)min(rows - r0, (int64_t)R);
-      o[i] = 2 * (COLS ? (uint32_t)line * (uint32_t)ld + min(8 * c, left - 8)
-                       : (uint32_t)min(line, left - 1) * (uint32_t)ld + 8 * c);
-    }
-  }
-  // first: the block's first element.  The loads' 64 x 16 bytes land at m0 in lane order; they are written as
-  // instructions, as the compiler makes every later LDS read wait for the builtin's.  The caller waits (vmcnt).
-  template <int THREADS, int KPER>
-  static SGNN_DEV void direct(const char* lds, const char* first, const uint32_t (&o)[KPER]) {
-    const uint64_t at = (uint64_t)first;
-    const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
-                          (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
-#pragma unroll
-    for (int i = 0; i < KPER; ++i) {
-      const uint32_t to = __builtin_amdgcn_readfirstlane(
-          (uint32_t)(uintptr_t)(const SGNN_LDS char*)lds + (i * THREADS + threadIdx.x / 64 * 64) * 16);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                   :
-                   : "s"(to), "v"(o[i]), "s"(base)
-                   : "memory", "m0");
-    }
-  }
-
-  // The same through registers, at any alignment, with zeros past K (and past the last row, in cols).
-  template <int THREADS, int KPER>
-  static SGNN_DEV void fetch(u32x4 (&v)[KPER], const char* src, int64_t ld, int64_t rows, int64_t K, int64_t r0,
-                             int64_t k0) {
-#pragma unroll
-    for (int i = 0; i < KPER; ++i) {
-      const int q = i * THREADS + threadIdx.x;
-      const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
-      const int64_t gl = (COLS ? k0 : r0) + line, gc = (COLS ? r0 : k0) + 8 * c;
-      const int64_t lines = COLS ? K : rows, most = COLS ? rows : K;
-      u32x4 t = {0, 0, 0, 0};
-      if (gl < lines && gc < most) {
-        const char* p = src + 2 * (gl * ld + gc);
-        if (gc + 8 <= most) {
-          t = *reinterpret_cast<const u32x4_any*>(p);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (gc + e < most) t[e >> 1] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e & 1));
-        }
-      }
-      v[i] = t;
-    }
-  }
-  template <int THREADS, int KPER>
-  static SGNN_DEV void put(char* lds, const u32x4 (&v)[KPER]) {
-#pragma unroll
-    for (int i = 0; i < KPER; ++i) *reinterpret_cast<u32x4*>(lds + (i * THREADS + threadIdx.x) * 16) = v[i];
-  }
-
-  // Fragment of 16 rows from r (a multiple of 16) by 32 k from 32 kk: lane l has row l & 15, k 8 (l >> 4) .. + 7.
-  static SGNN_DEV s16x8 frag(const char* lds, int r, int kk) {
-    const int l = lane_id();
-    if constexpr (!COLS) {
-      const int row = r + (l & 15);
-      return *reinterpret_cast<const s16x8*>(lds + (row * kChunks + ((4 * kk + (l >> 4)) ^ swizzle(row))) * 16);
-    } else {
-      // ds_read_b64_tr_b16: lanes 4 j .. 4 j + 3 of a group of 16 read 16 rows of k + j, lane i gets row i of 4 k
-      const int k = 32 * kk + 8 * (l >> 4) + ((l & 15) >> 2);
-      const int at = (k * kChunks + ((r / 8 + ((l & 3) >> 1)) ^ swizzle(k))) * 16 + (l & 1) * 8;
-      // k + 4 has the same swizzle
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(lds + at));
-      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(lds + at + 4 * kChunks * 16));
-      return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-    }
-  }
-};
-
 // BM x BN outputs per workgroup, WM x WN waves.  DIRECT: both operands' lines are 16-byte aligned (and in the cols
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT>
