@@ -554,23 +554,25 @@ typedef enum sgnn_act {
 
 /* y[M][N] = act(z) (+ residual), z = x[M][K] w[N][K]^T (+ bias[N]): one nn.Linear of build_mlp
  * (graph_network.py:7-45) with its activation and the block's residual (:176) in the epilogue.
- * bias, residual and z may be NULL; z (dense [M][N]) receives the pre-activation values the backward pass
- * reads.  K = 0 gives z = bias.  y and z may overlap no input; residual may be y itself.
+ * bias, residual and slope may be NULL.  slope (dense [M][N], elements of dtype's size) receives act'(z) for the
+ * backward pass: fp32 for SGNN_F32; for the 16-bit types a fixed-point number of 16 bits, act'(z) to 2^-16, which is
+ * 16 times finer than the type itself holds it.  K = 0 gives z = bias.  y and slope may overlap no input but that
+ * residual may be y itself.
  * workspace: sgnn_linear_workspace_bytes(dtype, M, N, K) bytes, 256-B aligned. */
 size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K);
 int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-                int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* z, void* y,
+                int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* slope, void* y,
                 int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Its backward pass from dy [M][N]: dz = dy act'(z), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = sum_m dz
- * (all dense; NULL skips one; the residual's gradient is dy).  z (dense) as saved by sgnn_linear; for
- * SGNN_ACT_RELU the output y of a call without residual serves as well; not read for SGNN_ACT_NONE.
+ * (all dense; NULL skips one; the residual's gradient is dy).  slope: as sgnn_linear wrote it for the same dtype;
+ * NULL: act'(z) = 1 (SGNN_ACT_NONE).
  * 16-bit types: dz is rounded once to the type before the two products, as their matrix instructions read it;
  * db sums the unrounded values.  M = 0 gives dw = db = 0.
- * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, act) bytes, 256-B aligned. */
-size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act);
-int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const void* z,
-                    int32_t act, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw,
-                    void* db, void* workspace, size_t workspace_bytes, void* stream);
+ * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != NULL) bytes, 256-B aligned. */
+size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope);
+int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const void* slope,
+                    const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw, void* db,
+                    void* workspace, size_t workspace_bytes, void* stream);
 
 /* y[n][width] = (x - mean) rstd gamma + beta (+ residual) per row, rstd = 1 / sqrt(var + eps) with the biased
  * variance (nn.LayerNorm, graph_network.py:86-96), x and residual rows at ldx / ldr, y dense.  gamma, beta and
@@ -598,11 +600,29 @@ typedef struct sgnn_matrix {
  * in / |in|_F goes through s <- a s + b s^3 + c s^5, which for (3.4445, -4.7750, 2.0315) brings it near 1 in
  * five steps (the update of the Muon optimiser).  `mats` is a HOST array of `count` matrices of any shapes
  * (read during the call only); matrices of one shape that stand next to each other share their launches.
- * Zero matrices give zeros.  Products are formed to fp32 accuracy whatever the type.
+ * Zero matrices give zeros.  Products: of fp32 and fp16 matrices to 22 bits of every operand, of bf16 ones to 11;
+ * sums in fp32.  X and its polynomials must stay below 63 in magnitude (the quintic above keeps them below 4); past
+ * that they become infinite.
  * workspace: sgnn_newton_schulz_workspace_bytes(mats, count) bytes (reads the shapes alone), 256-B aligned. */
 size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, int32_t count);
 int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_t count, int32_t steps, float a, float b,
                        float c, float eps, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The elementwise parts of a Muon step over flat fp32 buffers (training.FlatParams), around sgnn_newton_schulz.
+ * A segment is one parameter: `numel` elements from `offset`.  segs is a DEVICE array of nseg segments. */
+typedef struct sgnn_muon_seg {
+  int64_t offset, numel;
+  float scale;     /* matrix: factor of its orthogonalised update */
+  int32_t matrix;  /* 0: this parameter takes the Adam step */
+} sgnn_muon_seg;
+/* matrix: m = momentum m + grad, update = nesterov ? grad + momentum m : m.  Others: the step of sgnn_adam_step on
+ * param, m, v (update is not touched). */
+int sgnn_muon_moments(const sgnn_muon_seg* segs, int32_t nseg, float* param, const float* grad, float* m, float* v,
+                      float* update, float momentum, int32_t nesterov, float adam_lr, float beta1, float beta2,
+                      float adam_eps, int64_t step, void* stream);
+/* matrix: param = (1 - lr weight_decay) param - lr scale update.  Others: nothing. */
+int sgnn_muon_apply(const sgnn_muon_seg* segs, int32_t nseg, float* param, const float* update, float lr,
+                    float weight_decay, void* stream);
 
 #ifdef __cplusplus
 }

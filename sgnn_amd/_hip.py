@@ -203,8 +203,8 @@ SIGNATURES = {
                                    c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, ctypes.c_size_t,
                                    c_void_p]),
     "sgnn_linear_bwd_workspace_bytes": (ctypes.c_size_t, [c_int32, c_int64, c_int64, c_int64, c_int32]),
-    "sgnn_linear_bwd": (ctypes.c_int, [c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int32,
-                                       c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
+    "sgnn_linear_bwd": (ctypes.c_int, [c_int32, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                       c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_void_p,
                                        ctypes.c_size_t, c_void_p]),
     "sgnn_norm": (ctypes.c_int, [c_int32, c_int32, c_void_p, c_int64, c_int64, c_int32, c_void_p, c_void_p, c_void_p,
                                  c_int64, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
@@ -215,6 +215,9 @@ SIGNATURES = {
     "sgnn_newton_schulz_workspace_bytes": (ctypes.c_size_t, [P_MATRIX, c_int32]),
     "sgnn_newton_schulz": (ctypes.c_int, [c_int32, P_MATRIX, c_int32, c_int32, c_float, c_float, c_float, c_float,
                                           c_void_p, ctypes.c_size_t, c_void_p]),
+    "sgnn_muon_moments": (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_float,
+                                         c_int32, c_float, c_float, c_float, c_float, c_int64, c_void_p]),
+    "sgnn_muon_apply": (ctypes.c_int, [c_void_p, c_int32, c_void_p, c_void_p, c_float, c_float, c_void_p]),
 }
 
 # sgnn_dtype / sgnn_act (include/sgnn.h)
@@ -256,6 +259,26 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
 
 def lib() -> ctypes.CDLL:
     return _LIB if _LIB is not None else load_library()
+
+
+_TORCH_OPS = None
+
+
+def torch_ops():
+    """The torch binding of the typed operators (csrc/torch_ops.cpp), bound to the library load_library opened."""
+    global _TORCH_OPS
+    if _TORCH_OPS is None:
+        import importlib.util
+        lib()
+        path = os.path.join(HERE, "_lib", "_torch_ops.so")
+        if not os.path.exists(path):
+            raise SgnnError(f"{path} not built: run `python -c 'import __graft_entry__ as g; g.build()'`")
+        spec = importlib.util.spec_from_file_location("_torch_ops", path)
+        ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ops)
+        ops.bind(os.path.abspath(LIB_PATH))
+        _TORCH_OPS = ops
+    return _TORCH_OPS
 
 
 def check(status: int, what: str) -> None:

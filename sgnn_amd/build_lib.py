@@ -43,10 +43,36 @@ def deps():
 
 
 def needs_build() -> bool:
-    if not os.path.exists(LIB):
+    if not (os.path.exists(LIB) and os.path.exists(TORCH_OPS)):
         return True
     t = os.path.getmtime(LIB)
-    return any(os.path.getmtime(d) > t for d in deps())
+    return any(os.path.getmtime(d) > t for d in deps()) or torch_ops_stale()
+
+
+# the torch binding of the typed operators (host code alone; opens libsgnn_hip.so at run time)
+TORCH_OPS_SRC = os.path.join(CSRC, "torch_ops.cpp")
+TORCH_OPS = os.path.join(LIBDIR, "_torch_ops.so")
+
+
+def torch_ops_stale() -> bool:
+    return not os.path.exists(TORCH_OPS) or any(
+        os.path.getmtime(f) > os.path.getmtime(TORCH_OPS)
+        for f in (TORCH_OPS_SRC, os.path.join(ROOT, "include", "sgnn.h"), __file__))
+
+
+def start_torch_ops() -> subprocess.Popen:
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    rocm = os.path.dirname(os.path.dirname(os.path.realpath(HIPCC))) if os.path.exists(HIPCC) else "/opt/rocm"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1",
+           "-DUSE_ROCM=1", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *[f"-I{p}" for p in (*include_paths(), os.path.join(rocm, "include"), sysconfig.get_paths()["include"])],
+           TORCH_OPS_SRC, "-o", TORCH_OPS + ".tmp", f"-L{lib}", "-ltorch_python", "-ltorch_cpu", "-ltorch", "-lc10",
+           "-lc10_hip", "-ldl"]
+    return subprocess.Popen(cmd)
 
 
 OBJDIR = os.path.join(LIBDIR, "obj")   # per-source objects (git- and gpurun-ignored): incremental rebuilds
@@ -75,6 +101,10 @@ def build(force: bool = False, verbose: bool = False, defines=(), lib: str = LIB
         if verbose:
             print(" ".join(cmd))
         procs.append((subprocess.Popen(cmd), obj))
+    if lib == LIB and (force or torch_ops_stale()):
+        if start_torch_ops().wait() != 0:
+            raise RuntimeError("building the torch binding failed")
+        os.replace(TORCH_OPS + ".tmp", TORCH_OPS)
     for p, obj in procs:
         if p.wait() != 0:
             raise RuntimeError("hipcc failed")

@@ -22,7 +22,7 @@ struct Gemm {
   float alpha = 1.0f, beta = 1.0f;
   const void* res = nullptr;
   int64_t ldr = 0, batch_r = 0;
-  void* z = nullptr;   // dense [M][N], batch 1 only
+  void* slope = nullptr;   // act'(alpha sum + bias), dense [M][N] as sgnn_linear describes it; batch 1 only
   void* C = nullptr;
   int64_t ldc = 0, batch_c = 0;
 };

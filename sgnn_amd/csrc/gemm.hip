@@ -20,7 +20,7 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct GemmArgs {
   const void *A, *B, *bias, *res;
-  void *z, *C;
+  void *slope, *C;
   float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
   int64_t lda, ldb, ldr, ldc, M, N, K, batch_a, batch_b, batch_r, batch_c;
   int32_t act, nsplit, tiles_m, tiles_n;
@@ -28,114 +28,81 @@ struct GemmArgs {
 };
 
 // ----------------------------------------------------------------------------- epilogue
-template <int ACT>
-SGNN_DEV void act_n(float* v, int n) {
+template <int ACT, typename T, int V>
+SGNN_DEV void act_row(const GemmArgs& g, int64_t at, int cnt, float (&v)[V]) {
+  if (g.slope) {
+    float s[V];
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < n) v[i] = act_value<ACT>(v[i]);
-}
-
-SGNN_DEV void act_any(int32_t act, float* v, int n) {  // act is the same for every lane
-  switch (act) {
-    case SGNN_ACT_RELU: act_n<SGNN_ACT_RELU>(v, n); break;
-    case SGNN_ACT_GELU: act_n<SGNN_ACT_GELU>(v, n); break;
-    case SGNN_ACT_GELU_TANH: act_n<SGNN_ACT_GELU_TANH>(v, n); break;
-    case SGNN_ACT_SILU: act_n<SGNN_ACT_SILU>(v, n); break;
-    default: break;
+    for (int i = 0; i < V; ++i) act_both<ACT, true>(v[i], v[i], s[i]);
+    store_slopes<T>(g.slope, at, cnt, s);
+  } else {
+    float unused;
+#pragma unroll
+    for (int i = 0; i < V; ++i) act_both<ACT, false>(v[i], v[i], unused);
   }
 }
 
-// V consecutive outputs (m, n ..) of one lane; cnt of them exist.
-template <typename T>
-SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float* v, int cnt) {
-  constexpr int V = 16 / sizeof(T);
-  const bool whole = cnt >= V;
+// V = 16 bytes' consecutive outputs (m, n ..) of one lane; cnt of them exist.
+template <typename T, int V>
+SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float (&v)[V], int cnt) {
   float t[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) v[i] *= g.alpha;
   if (g.bias) {
-    const T* p = static_cast<const T*>(g.bias) + n;
-    if (whole) {
-      load_vec(p, t);
+    load_some<V>(static_cast<const T*>(g.bias) + n, cnt, t);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += t[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < cnt) v[i] += to_float(p[i]);
-    }
+    for (int i = 0; i < V; ++i) v[i] += t[i];
   }
-  if (g.z) {
-    T* p = static_cast<T*>(g.z) + m * g.N + n;
-    if (whole) {
-      store_vec(p, v);
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < cnt) p[i] = from_float<T>(v[i]);
-    }
+  switch (g.act) {  // the same for every lane
+    case SGNN_ACT_RELU: act_row<SGNN_ACT_RELU, T>(g, m * g.N + n, cnt, v); break;
+    case SGNN_ACT_GELU: act_row<SGNN_ACT_GELU, T>(g, m * g.N + n, cnt, v); break;
+    case SGNN_ACT_GELU_TANH: act_row<SGNN_ACT_GELU_TANH, T>(g, m * g.N + n, cnt, v); break;
+    case SGNN_ACT_SILU: act_row<SGNN_ACT_SILU, T>(g, m * g.N + n, cnt, v); break;
+    default: break;
   }
-  act_any(g.act, v, V);
   if (g.res) {
-    const T* p = static_cast<const T*>(g.res) + b * g.batch_r + m * g.ldr + n;
-    if (whole) {
-      load_vec(p, t);
+    load_some<V>(static_cast<const T*>(g.res) + b * g.batch_r + m * g.ldr + n, cnt, t);
 #pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += g.beta * t[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < cnt) v[i] += g.beta * to_float(p[i]);
-    }
+    for (int i = 0; i < V; ++i) v[i] += g.beta * t[i];
   }
-  T* p = static_cast<T*>(g.C) + b * g.batch_c + m * g.ldc + n;
-  if (whole) {
-    store_vec(p, v);
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < cnt) p[i] = from_float<T>(v[i]);
-  }
+  store_some<V>(static_cast<T*>(g.C) + b * g.batch_c + m * g.ldc + n, cnt, v);
 }
 
-// A wave's accumulators (TM x TN sub-tiles of 16 x 16, lane l: m = l & 15, n = 4 (l >> 4) + r) to memory, 16 rows
-// of m at a time through `buf` (16 x 16 TN floats of its own).  16-byte pieces are XORed with m, so that the 16
+// A wave's accumulators (TM x TN sub-tiles of 16 x 16, lane l: m = l & 15, n = 4 (l >> 4) + r) to memory, RP sub-tile
+// rows at a time through `buf` (16 RP x 16 TN floats of its own).  16-byte pieces are XORed with m, so that the 16
 // rows of one write, which are a multiple of all banks apart, fall on different ones.
-template <typename T, int TM, int TN>
+template <typename T, int RP, int TM, int TN>
 SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][TN], int64_t b, int split, int64_t m0,
                          int64_t n0) {
+  static_assert(TM % RP == 0, "whole rounds");
   const int l = lane_id();
   constexpr int kPieces = 4 * TN;  // 16-byte pieces per row of 16 TN floats
   constexpr int kMask = kPieces - 1 < 15 ? kPieces - 1 : 15;
-  const int lm = l & 15;
 #pragma unroll
-  for (int i = 0; i < TM; ++i) {
+  for (int round = 0; round < TM / RP; ++round) {
 #pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const int piece = (4 * j + (l >> 4)) ^ (lm & kMask);
-      *reinterpret_cast<f32x4*>(buf + lm * 16 * TN + piece * 4) = acc[i][j];
-    }
+    for (int i = 0; i < RP; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        const int r = 16 * i + (l & 15), piece = (4 * j + (l >> 4)) ^ (r & kMask);
+        *reinterpret_cast<f32x4*>(buf + r * 16 * TN + piece * 4) = acc[round * RP + i][j];
+      }
     __builtin_amdgcn_wave_barrier();
+    const int64_t mr = m0 + 16 * RP * round;
     if (g.part) {
 #pragma unroll 1
-      for (int t = l; t < 16 * kPieces; t += 64) {
+      for (int t = l; t < 16 * RP * kPieces; t += 64) {
         const int r = t / kPieces, p = t % kPieces;
-        const f32x4 v = *reinterpret_cast<const f32x4*>(buf + r * 16 * TN + (p ^ (r & kMask)) * 4);
-        const int64_t m = m0 + 16 * i + r, n = n0 + 4 * p;
-        if (m >= g.M || n >= g.N) continue;
-        float* o = g.part + ((int64_t)split * g.M + m) * g.N + n;
-        if (n + 4 <= g.N) {
-          *reinterpret_cast<u32x4_any*>(o) = __builtin_bit_cast(u32x4, v);
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            if (n + q < g.N) o[q] = v[q];
-        }
+        const f32x4 f = *reinterpret_cast<const f32x4*>(buf + r * 16 * TN + (p ^ (r & kMask)) * 4);
+        const int64_t m = mr + r, n = n0 + 4 * p;
+        const float v[4] = {f[0], f[1], f[2], f[3]};
+        if (m < g.M && n < g.N)
+          store_some<4>(g.part + ((int64_t)split * g.M + m) * g.N + n, (int)min((int64_t)4, g.N - n), v);
       }
     } else {
       constexpr int V = 16 / sizeof(T), kPer = V / 4;
 #pragma unroll 1
-      for (int t = l; t < 16 * kPieces / kPer; t += 64) {
+      for (int t = l; t < 16 * RP * kPieces / kPer; t += 64) {
         const int r = t / (kPieces / kPer), p = (t % (kPieces / kPer)) * kPer;
         float v[V];
 #pragma unroll
@@ -144,7 +111,7 @@ SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][T
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
         }
-        const int64_t m = m0 + 16 * i + r, n = n0 + 4 * p;
+        const int64_t m = mr + r, n = n0 + 4 * p;
         if (m < g.M && n < g.N) finish<T>(g, b, m, n, v, (int)min((int64_t)V, g.N - n));
       }
     }
@@ -185,7 +152,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   using TB = Tile16<BN, BK, BCOLS>;
   constexpr int kStage = TA::kBytes + TB::kBytes;
   __shared__ __attribute__((aligned(16))) char lds[2 * kStage];  // two stages of A's and B's tiles
-  static_assert(16 * 16 * TN * 4 * WM * WN <= 2 * kStage, "the epilogue's buffers fit");
+  constexpr int RP = TM < 4 ? TM : 4, kBuf = RP * 16 * 16 * TN;
+  static_assert(kBuf * 4 * WM * WN <= 2 * kStage, "the epilogue's buffers fit");
   const int w = wave_id(), wm = w / WN, wn = w % WN;
   int tm, tn;
   tile_of(g, tm, tn);
@@ -272,8 +240,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     }
   }
   __syncthreads();
-  write_tile<T, TM, TN>(g, reinterpret_cast<float*>(lds) + w * 16 * 16 * TN, acc, batch, split, m0 + wm * TM * 16,
-                        n0 + wn * TN * 16);
+  write_tile<T, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, batch, split, m0 + wm * TM * 16,
+                    n0 + wn * TN * 16);
 }
 
 // ----------------------------------------------------------------------------- fp32 operands
@@ -379,8 +347,10 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile32<BM, ACOLS>;
   using TB = Tile32<BN, BCOLS>;
-  __shared__ __attribute__((aligned(16))) char sa[TA::kBytes], sb[TB::kBytes];
-  static_assert(16 * 16 * TN * 4 * WM * WN <= TA::kBytes, "the epilogue's buffers fit one tile");
+  __shared__ __attribute__((aligned(16))) char lds[TA::kBytes + TB::kBytes];
+  char *sa = lds, *sb = lds + TA::kBytes;
+  constexpr int RP = 2, kBuf = RP * 16 * 16 * TN;
+  static_assert(kBuf * 4 * WM * WN <= TA::kBytes + TB::kBytes, "the epilogue's buffers fit");
   const int w = wave_id(), wm = w / WN, wn = w % WN, l = lane_id();
   int tm, tn;
   tile_of(g, tm, tn);
@@ -455,8 +425,8 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
         acc[i][j][r] = s;
       }
     }
-  write_tile<float, TM, TN>(g, reinterpret_cast<float*>(sa) + w * 16 * 16 * TN, acc, batch, split, m0 + wm * TM * 16,
-                            n0 + wn * TN * 16);
+  write_tile<float, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, batch, split, m0 + wm * TM * 16,
+                        n0 + wn * TN * 16);
 }
 
 // ----------------------------------------------------------------------------- split k
@@ -561,7 +531,7 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
   const int64_t tm = (g.M + p.bm - 1) / p.bm, tn = (g.N + p.bn - 1) / p.bn;
   if (tm > INT32_MAX / tn || g.batch > 65535 || g.K > (int64_t)INT32_MAX * 32)
     return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k, or 65535 matrices");
-  GemmArgs a{g.A, g.B, g.bias, g.res, g.z, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
+  GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
              g.batch_b, g.batch_r, g.batch_c, g.act, p.nsplit, (int32_t)tm, (int32_t)tn, g.alpha, g.beta};
   if (p.nsplit > 1) {
     if (!workspace || workspace_bytes < gemm_workspace_bytes(g))

@@ -47,7 +47,8 @@ struct Tile16 {
     }
   }
   // first: the block's first element.  The loads' 64 x 16 bytes land at m0 in lane order; they are written as
-  // instructions, as the compiler makes every later LDS read wait for the builtin's.  The caller waits (vmcnt).
+  // instructions, as the compiler makes every later LDS read wait for the builtin's.  The caller waits (vmcnt); no other code of
+  // these kernels has a value in m0.
   template <int THREADS, int KPER>
   static SGNN_DEV void direct(const char* lds, const char* first, const uint32_t (&o)[KPER]) {
     const uint64_t at = (uint64_t)first;
@@ -60,7 +61,7 @@ struct Tile16 {
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :
                    : "s"(to), "v"(o[i]), "s"(base)
-                   : "memory", "m0");
+                   : "memory");
     }
   }
 

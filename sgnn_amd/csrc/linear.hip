@@ -26,9 +26,9 @@ struct ActCut {
 };
 
 // dz = dy act'(z), and the column sums of this workgroup's rows: every thread over its rows in order, then the
-// threads of one column in order.  Reads dy and z, writes dz: bounded by memory.
-template <typename T, int ACT>
-__global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const T* z, int64_t M, int64_t N,
+// threads of one column in order.  Reads dy and the slopes, writes dz: bounded by memory.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const void* slope, int64_t M, int64_t N,
                                                       int lanes, T* dz, float* partial) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float sums[kThreads * V];
@@ -44,10 +44,10 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
     for (int64_t r = (int64_t)blockIdx.y * rows + row; r < M; r += step) {
       float v[V], t[V];
       load_some<V>(dy + r * ldd + c, cnt, v);
-      if constexpr (ACT != SGNN_ACT_NONE) {
-        load_some<V>(z + r * N + c, cnt, t);
+      if (slope) {
+        load_slopes<T>(slope, r * N + c, cnt, t);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= act_slope<ACT>(t[i]);
+        for (int i = 0; i < V; ++i) v[i] *= t[i];
         store_some<V>(dz + r * N + c, cnt, v);
       }
 #pragma unroll
@@ -71,20 +71,6 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
 template <typename T>
 __global__ __launch_bounds__(kSumThreads) void k_bias_grad(const float* partial, int64_t nblk, int64_t N, T* out) {
   sum_partials(partial, nblk, N, [&](int64_t c, float s) { out[c] = from_float<T>(s); });
-}
-
-template <typename T>
-void launch_act_bwd(int32_t act, const ActCut& cut, hipStream_t s, const T* dy, int64_t ldd, const T* z, int64_t M,
-                    int64_t N, T* dz, float* partial) {
-  const auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)cut.strips, (unsigned)cut.blocks), dim3(kThreads), 0, s, dy, ldd, z, M,
-                       N, cut.lanes, dz, partial);
-  };
-  if (act == SGNN_ACT_RELU) go(k_act_bwd<T, SGNN_ACT_RELU>);
-  else if (act == SGNN_ACT_GELU) go(k_act_bwd<T, SGNN_ACT_GELU>);
-  else if (act == SGNN_ACT_GELU_TANH) go(k_act_bwd<T, SGNN_ACT_GELU_TANH>);
-  else if (act == SGNN_ACT_SILU) go(k_act_bwd<T, SGNN_ACT_SILU>);
-  else go(k_act_bwd<T, SGNN_ACT_NONE>);
 }
 
 bool act_ok(int32_t act) { return act >= SGNN_ACT_NONE && act <= SGNN_ACT_SILU; }
@@ -114,8 +100,8 @@ Gemm wgrad(int32_t dtype, int64_t M, int64_t N, int64_t K) {  // dw[N][K] = dz^T
 // Workspace of the backward pass: dz, the partial sums of db, and the products' own.
 struct BwdLayout {
   size_t dz, partial, gemm, total;
-  BwdLayout(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
-    dz = act == SGNN_ACT_NONE ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
+  BwdLayout(int32_t dtype, int64_t M, int64_t N, int64_t K, bool has_slope) {
+    dz = !has_slope ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
     partial = pad256(sizeof(float) * (size_t)ActCut(dtype_size(dtype), M, N).blocks * (size_t)N);
     gemm = std::max(gemm_workspace_bytes(dgrad(dtype, M, N, K)), gemm_workspace_bytes(wgrad(dtype, M, N, K)));
     total = dz + partial + gemm;
@@ -130,7 +116,7 @@ extern "C" size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t 
 }
 
 extern "C" int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-                           int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* z,
+                           int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* slope,
                            void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sgnn;
   if (!dtype_ok(dtype) || !act_ok(act)) return set_error(SGNN_ERR_INVALID, "linear: unknown dtype or activation");
@@ -145,41 +131,40 @@ extern "C" int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const
   g.B = w, g.ldb = ldw;
   g.bias = bias, g.act = act;
   g.res = residual, g.ldr = ldr;
-  g.z = z, g.C = y, g.ldc = ldy;
+  g.slope = slope, g.C = y, g.ldc = ldy;
   return gemm_run(g, workspace, workspace_bytes, stream);
 }
 
-extern "C" size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t act) {
-  if (!sgnn::dtype_ok(dtype) || !act_ok(act) || M <= 0 || N <= 0 || K < 0) return 0;
-  return BwdLayout(dtype, M, N, K, act).total;
+extern "C" size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope) {
+  if (!sgnn::dtype_ok(dtype) || M <= 0 || N <= 0 || K < 0) return 0;
+  return BwdLayout(dtype, M, N, K, has_slope != 0).total;
 }
 
 extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd,
-                               const void* z, int32_t act, const void* x, int64_t ldx, const void* w, int64_t ldw,
-                               void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream) {
+                               const void* slope, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx,
+                               void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sgnn;
-  if (!dtype_ok(dtype) || !act_ok(act)) return set_error(SGNN_ERR_INVALID, "linear_bwd: unknown dtype or activation");
+  if (!dtype_ok(dtype)) return set_error(SGNN_ERR_INVALID, "linear_bwd: unknown dtype");
   if (M < 0 || N < 0 || K < 0) return set_error(SGNN_ERR_INVALID, "linear_bwd: negative size");
-  if (M > 0 && N > 0 && (!dy || ldd < N || (act != SGNN_ACT_NONE && !z)))
-    return set_error(SGNN_ERR_INVALID, "linear_bwd: bad dy or z");
+  if (M > 0 && N > 0 && (!dy || ldd < N)) return set_error(SGNN_ERR_INVALID, "linear_bwd: bad dy");
   if (K > 0 && ((dx && N > 0 && (!w || ldw < K)) || (dw && M > 0 && (!x || ldx < K))))
     return set_error(SGNN_ERR_INVALID, "linear_bwd: bad operand");
-  if (workspace_bytes < sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, act))
+  if (workspace_bytes < sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != nullptr))
     return set_error(SGNN_ERR_INVALID, "linear_bwd: workspace smaller than sgnn_linear_bwd_workspace_bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const BwdLayout at(dtype, std::max<int64_t>(M, 0), N, K, act);
+  const BwdLayout at(dtype, M, N, K, slope != nullptr);
   char* ws = static_cast<char*>(workspace);
   const void* up = dy;      // dz and its leading dimension
   int64_t ldu = ldd;
-  if (N > 0 && (act != SGNN_ACT_NONE || db))
+  if (N > 0 && (slope || db))
     with_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const ActCut cut(sizeof(T), M, N);
       float* partial = db ? reinterpret_cast<float*>(ws + at.dz) : nullptr;
       if (M > 0) {
-        launch_act_bwd<T>(act, cut, s, static_cast<const T*>(dy), ldd, static_cast<const T*>(z), M, N,
-                          reinterpret_cast<T*>(ws), partial);
-        if (act != SGNN_ACT_NONE) up = ws, ldu = N;
+        hipLaunchKernelGGL(k_act_bwd<T>, dim3((unsigned)cut.strips, (unsigned)cut.blocks), dim3(kThreads), 0, s,
+                           static_cast<const T*>(dy), ldd, slope, M, N, cut.lanes, reinterpret_cast<T*>(ws), partial);
+        if (slope) up = ws, ldu = N;
       }
       if (db)
         hipLaunchKernelGGL(k_bias_grad<T>, dim3(sum_grid(N)), dim3(kSumThreads), 0, s, partial,

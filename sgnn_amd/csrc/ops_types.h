@@ -139,35 +139,74 @@ constexpr float kGeluCubic = 0.044715f;
 
 SGNN_DEV float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
 
-// act(z).  ReLU keeps a NaN (a comparison, not a maximum).
-template <int ACT>
-SGNN_DEV float act_value(float z) {
-  if constexpr (ACT == SGNN_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if constexpr (ACT == SGNN_ACT_GELU) return 0.5f * z * (1.0f + erff(z * kInvSqrt2));
-  // 0.5 (1 + tanh u) = sigmoid(2 u)
-  if constexpr (ACT == SGNN_ACT_GELU_TANH) return z * sigmoid(2.0f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
-  if constexpr (ACT == SGNN_ACT_SILU) return z * sigmoid(z);
-  return z;
-}
-
-// d act / d z.  ReLU's slope at 0 is 0.  Far out, where the smooth ones' second terms are 0 in fp32 but for the
-// products of 0 and infinity in them, the first terms alone.
-template <int ACT>
-SGNN_DEV float act_slope(float z) {
-  if constexpr (ACT == SGNN_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+// act(z) and, where SLOPE, d act / d z, which share their functions.  ReLU keeps a NaN (a comparison, not a maximum);
+// its slope at 0 is 0.  Far out, where the smooth ones' second terms are 0 in fp32 but for the products of 0 and
+// infinity in them, the slopes are the first terms alone.
+template <int ACT, bool SLOPE>
+SGNN_DEV void act_both(float z, float& value, float& slope) {
+  value = z, slope = 1.0f;
+  if constexpr (ACT == SGNN_ACT_RELU) {
+    value = z < 0.0f ? 0.0f : z;
+    slope = z > 0.0f ? 1.0f : 0.0f;
+  }
   if constexpr (ACT == SGNN_ACT_GELU) {
     const float phi = 0.5f * (1.0f + erff(z * kInvSqrt2));
-    return fabsf(z) > 20.0f ? phi : phi + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    value = z * phi;
+    if constexpr (SLOPE) slope = fabsf(z) > 20.0f ? phi : phi + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
   }
-  if constexpr (ACT == SGNN_ACT_GELU_TANH) {
+  if constexpr (ACT == SGNN_ACT_GELU_TANH) {  // 0.5 (1 + tanh u) = sigmoid(2 u)
     const float s = sigmoid(2.0f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
-    return fabsf(z) > 20.0f ? s : s + z * s * (1.0f - s) * 2.0f * kSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * z * z);
+    value = z * s;
+    if constexpr (SLOPE)
+      slope = fabsf(z) > 20.0f ? s : s + z * s * (1.0f - s) * 2.0f * kSqrt2OverPi * (1.0f + 3.0f * kGeluCubic * z * z);
   }
   if constexpr (ACT == SGNN_ACT_SILU) {
     const float s = sigmoid(z);
-    return fabsf(z) > 88.0f ? s : s * (1.0f + z * (1.0f - s));
+    value = z * s;
+    if constexpr (SLOPE) slope = fabsf(z) > 88.0f ? s : s * (1.0f + z * (1.0f - s));
   }
-  return 1.0f;
+}
+
+// A slope in 16 bits: all of them lie in [-0.13, 1.13]; (slope + 1/4) 2^15 is a whole number below 2^16 - 1, which
+// marks a NaN.  0 and 1 are exact.
+SGNN_DEV uint16_t slope_to_bits(float s) { return s == s ? (uint16_t)rintf((s + 0.25f) * 32768.0f) : 0xffffu; }
+SGNN_DEV float slope_from_bits(uint16_t b) {
+  return b == 0xffffu ? __builtin_nanf("") : (float)b * (1.0f / 32768.0f) - 0.25f;
+}
+// V slopes (16 bytes of T's size) at any alignment.
+template <typename T, int V>
+SGNN_DEV void store_slopes(void* base, int64_t at, int cnt, const float (&s)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    store_some<V>(static_cast<float*>(base) + at, cnt, s);
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(base) + at;
+    if (cnt >= V) {
+      u32x4 t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t[i] = slope_to_bits(s[2 * i]) | (uint32_t)slope_to_bits(s[2 * i + 1]) << 16;
+      *reinterpret_cast<u32x4_any*>(p) = t;
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (i < cnt) p[i] = slope_to_bits(s[i]);
+    }
+  }
+}
+template <typename T, int V>
+SGNN_DEV void load_slopes(const void* base, int64_t at, int cnt, float (&s)[V]) {
+  if constexpr (sizeof(T) == 4) {
+    load_some<V>(static_cast<const float*>(base) + at, cnt, s);
+  } else {
+    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
+    if (cnt >= V) {
+      const u32x4 t = *reinterpret_cast<const u32x4_any*>(p);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = slope_from_bits((uint16_t)(t[i >> 1] >> (16 * (i & 1))));
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] = i < cnt ? slope_from_bits(p[i]) : 0.0f;
+    }
+  }
 }
 
 }  // namespace sgnn

@@ -37,13 +37,13 @@ def test_empty_calls_need_no_device(lib):
     assert lib.sgnn_newton_schulz(0, empty, 1, 5, 1.0, 0.0, 0.0, 0.0, None, 0, None) == _hip.SGNN_OK
 
 
-def _linear_bwd(lib, dtype=0, M=4, N=4, K=4, dy=P, ldd=4, z=P, act=3, x=P, ldx=4, w=P, ldw=4, dx=P, dw=P, db=P,
+def _linear_bwd(lib, dtype=0, M=4, N=4, K=4, dy=P, ldd=4, slope=P, x=P, ldx=4, w=P, ldw=4, dx=P, dw=P, db=P,
                 nws=1 << 30):
-    return lib.sgnn_linear_bwd(dtype, M, N, K, dy, ldd, z, act, x, ldx, w, ldw, dx, dw, db, P, nws, None)
+    return lib.sgnn_linear_bwd(dtype, M, N, K, dy, ldd, slope, x, ldx, w, ldw, dx, dw, db, P, nws, None)
 
 
 @pytest.mark.parametrize("bad", [
-    dict(dtype=7), dict(act=9), dict(M=-1), dict(dy=None), dict(ldd=3), dict(z=None), dict(x=None), dict(ldx=3),
+    dict(dtype=7), dict(M=-1), dict(dy=None), dict(ldd=3), dict(x=None), dict(ldx=3),
     dict(w=None), dict(ldw=3), dict(nws=0)])
 def test_linear_bwd_refuses(lib, bad):
     assert _linear_bwd(lib, **bad) == INVALID
