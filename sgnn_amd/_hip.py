@@ -78,6 +78,11 @@ class SgnnMatrix(ctypes.Structure):
                 ("cols", c_int32)]
 
 
+class SgnnMuonSeg(ctypes.Structure):
+    """struct sgnn_muon_seg (include/sgnn.h)."""
+    _fields_ = [("offset", c_int64), ("numel", c_int64), ("scale", c_float), ("matrix", c_int32)]
+
+
 P_SAVES = ctypes.POINTER(SgnnSaves)
 P_MATRIX = ctypes.POINTER(SgnnMatrix)
 SLAB_EDGE, SLAB_NODE, SLAB_UV, SLAB_DECODER, SLAB_ENC_NODE, SLAB_ENC_EDGE = range(6)

@@ -32,7 +32,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 import torch.nn as nn
 
-from . import engine
+from . import engine, functional
 from ._hip import check, lib, require_gpu_tensor, stream_ptr
 
 
@@ -249,8 +249,45 @@ class _MLP(torch.autograd.Function):
         return (None, None, dx, dres, *grads)
 
 
+_ACTIVATION_NAMES = {nn.ReLU: "relu", nn.SiLU: "silu", nn.Identity: "none"}
+
+
+def _activation_name(m: nn.Module) -> str:
+    if isinstance(m, nn.GELU):
+        return "gelu" if m.approximate == "none" else "gelu_tanh"
+    name = _ACTIVATION_NAMES.get(type(m))
+    if name is None:
+        raise NotImplementedError(f"no kernel for the activation {m}")
+    return name
+
+
+def needs_typed(module: nn.Module) -> bool:
+    """Whether an MLP (or a module of them) is one the fp32 ReLU kernels do not compute: 16-bit
+    parameters, or build_mlp's `activation` (graph_network.py:7-45) set to GELU or SiLU."""
+    return (any(isinstance(m, (nn.GELU, nn.SiLU)) for m in module.modules())
+            or any(p.dtype in (torch.bfloat16, torch.float16) for p in module.parameters()))
+
+
+def _typed_mlp(body: nn.Module, ln: Optional[nn.Module], x: torch.Tensor, residual: Optional[torch.Tensor]):
+    """The same MLP on the typed operators, in the type of its parameters (x and residual are cast to it)."""
+    layers = [m for m in body.modules() if not list(m.children())]   # Linear, activation, Linear, activation ...
+    lins = [m for m in layers if isinstance(m, nn.Linear)]
+    t = lins[0].weight.dtype
+    h = x.to(t)
+    for i, m in enumerate(layers):
+        if isinstance(m, nn.Linear):
+            after = layers[i + 1] if i + 1 < len(layers) and not isinstance(layers[i + 1], nn.Linear) else nn.Identity()
+            h = functional.linear(h, m.weight, m.bias, _activation_name(after))
+    if ln is not None:
+        return functional.layer_norm(h, ln.weight, ln.bias, residual.to(t) if residual is not None else None, ln.eps)
+    if residual is not None:
+        raise ValueError("a residual needs the LayerNorm form")
+    return h
+
+
 def mlp(seq: nn.Module, has_ln: bool, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """A reference-layout Sequential(build_mlp[, LayerNorm]) on rows x (any widths / depth)."""
+    """A reference-layout Sequential(build_mlp[, LayerNorm]) on rows x (any widths / depth).  fp32 with ReLU:
+    the chain above; 16-bit parameters, GELU or SiLU: functional.linear / layer_norm in the parameters' type."""
     if has_ln:
         lins, ln = _linears(seq[0]), seq[1]
         params = [t for l in lins for t in (l.weight, l.bias)] + [ln.weight, ln.bias]
@@ -261,6 +298,9 @@ def mlp(seq: nn.Module, has_ln: bool, x: torch.Tensor, residual: Optional[torch.
         require_gpu_tensor(p, "parameter")
     if x.shape[1] != lins[0].in_features:
         raise ValueError(f"MLP input width {x.shape[1]} != {lins[0].in_features}")
+    body = seq[0] if has_ln else seq
+    if params[0].dtype in (torch.bfloat16, torch.float16) or any(type(m) in (nn.GELU, nn.SiLU) for m in body.children()):
+        return _typed_mlp(body, seq[1] if has_ln else None, x, residual)
     return _MLP.apply(len(lins), has_ln, _c(x), residual, *params)
 
 
@@ -351,7 +391,7 @@ def message_passing(block: nn.Module, x: torch.Tensor, graph: EdgeGraph, e: torc
     msg_in = gather_cat(graph.E, [(x, graph.recv, 1.0, graph.by_recv), (x, graph.send, 1.0, graph.by_send),
                                   (e, None, 1.0, None)])
     m = mlp(block.edge_fn, True, msg_in)
-    agg = _SegmentSum.apply(graph, m)
+    agg = _SegmentSum.apply(graph, _c(m))
     x_new = mlp(block.node_fn, True, gather_cat(graph.n, [(agg, None, 1.0, None), (x, None, 1.0, None)]),
                 residual=x)
     return x_new, gather_cat(graph.E, [(e, None, 2.0, None)])

@@ -312,13 +312,17 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor&
 }
 
 // ----------------------------------------------------------------------------- newton-schulz
-std::vector<Tensor> newton_schulz(const std::vector<Tensor>& gs, int64_t steps, double a, double b, double c,
-                                  double eps) {
+// given: as many outputs as inputs, or none.
+std::vector<Tensor> newton_schulz(const std::vector<Tensor>& gs, const std::vector<Tensor>& given, int64_t steps,
+                                  double a, double b, double c, double eps) {
   at::NoGradGuard no_grad;
   TORCH_CHECK_VALUE(steps >= 0 && steps <= INT32_MAX && eps >= 0.0, "newton_schulz: steps ", steps, ", eps ", eps);
+  TORCH_CHECK_VALUE(given.empty() || given.size() == gs.size(), "newton_schulz: ", given.size(), " outputs for ",
+                    gs.size(), " inputs");
   std::vector<Tensor> ins, outs;
   std::vector<sgnn_matrix> mats;
-  for (const Tensor& g : gs) {
+  for (size_t k = 0; k < gs.size(); ++k) {
+    const Tensor& g = gs[k];
     supported(g, "g");
     like(g, "g", gs[0]);
     TORCH_CHECK_VALUE((g.dim() == 2 || g.dim() == 3) && g.size(-1) <= INT32_MAX && g.size(-2) <= INT32_MAX,
@@ -326,15 +330,24 @@ std::vector<Tensor> newton_schulz(const std::vector<Tensor>& gs, int64_t steps, 
     c10::DeviceGuard guard(g.device());
     const int64_t m = g.size(-2), n = g.size(-1);
     ins.push_back((g.stride(-1) == 1 && g.stride(-2) >= n) || g.is_contiguous() ? g : g.contiguous());
-    outs.push_back(at::empty(g.sizes(), g.options()));
+    if (given.empty()) {
+      outs.push_back(at::empty(g.sizes(), g.options()));
+    } else {
+      like(given[k], "out", g);
+      TORCH_CHECK_VALUE(given[k].sizes() == g.sizes() &&
+                            ((given[k].stride(-1) == 1 && given[k].stride(-2) >= n) || given[k].is_contiguous()),
+                        "newton_schulz: out ", given[k].sizes(), " with strides ", given[k].strides(), " for ", g.sizes());
+      outs.push_back(given[k]);
+    }
     const Tensor &in = ins.back(), &out = outs.back();
     if (g.numel() == 0) continue;
     const char* pi = static_cast<const char*>(in.data_ptr());
     char* po = static_cast<char*>(out.data_ptr());
     const int64_t count = g.dim() == 3 ? g.size(0) : 1, size = g.element_size();
-    const int64_t bi = g.dim() == 3 ? in.stride(0) : 0, bo = m * n;
+    const int64_t bi = g.dim() == 3 ? in.stride(0) : 0, bo = g.dim() == 3 ? out.stride(0) : 0;
     for (int64_t i = 0; i < count; ++i)
-      mats.push_back({pi + size * i * bi, po + size * i * bo, std::max(in.stride(-2), n), n, (int32_t)m, (int32_t)n});
+      mats.push_back({pi + size * i * bi, po + size * i * bo, std::max(in.stride(-2), n), std::max(out.stride(-2), n),
+                      (int32_t)m, (int32_t)n});
   }
   TORCH_CHECK_VALUE(mats.size() <= INT32_MAX, "newton_schulz: too many matrices");
   if (!mats.empty()) {

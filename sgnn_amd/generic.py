@@ -82,7 +82,9 @@ def ms_fast_shapes(gnn: nn.Module) -> bool:
 def block_fast_shapes(block: nn.Module) -> bool:
     """One InteractionNetwork / G2M / M2M / M2G block the fused edge / node kernels
     implement: node and edge latents and the MLP hidden width all 64 or 128,
-    nmlp_layers 1 or 2."""
+    nmlp_layers 1 or 2, fp32 with ReLU."""
+    if autograd.needs_typed(block):
+        return False
     lin = [m for m in block.edge_fn.modules() if isinstance(m, nn.Linear)]
     nlin = [m for m in block.node_fn.modules() if isinstance(m, nn.Linear)]
     H = lin[0].out_features
@@ -112,14 +114,14 @@ def processor_forward(proc: nn.Module, x, edge_index, edge_features):
 def epd_forward(epd: nn.Module, x, edge_index, edge_features) -> torch.Tensor:
     """EncodeProcessDecode.forward (graph_network.py:388-406): the fused chain in
     inference at the fast widths, else module by module (differentiable)."""
-    if not needs_grad(epd, x, edge_features) and fast_shapes(epd):
+    if not needs_grad(epd, x, edge_features) and fast_shapes(epd) and not autograd.needs_typed(epd):
         return engine.epd_forward(epd, x, edge_index, edge_features)
     return autograd.epd_forward(epd, x, edge_index, edge_features)
 
 
 def ms_gnn_forward(gnn: nn.Module, *args) -> torch.Tensor:
     """MultiScaleGNN.forward (multi_scale_gnn.py:277-326)."""
-    if not needs_grad(gnn, *args) and ms_fast_shapes(gnn):
+    if not needs_grad(gnn, *args) and ms_fast_shapes(gnn) and not autograd.needs_typed(gnn):
         from .multi_scale import ms_engine
         return ms_engine.gnn_forward(gnn, *args)
     return autograd.ms_gnn_forward(gnn, *args)

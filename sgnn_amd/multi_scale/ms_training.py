@@ -24,8 +24,9 @@ import torch
 
 from .. import _hip, engine
 from .._hip import check, lib, stream_ptr
+from ..muon import make_optimizer
 from ..train import DataParallel, block_buckets, device_random_walk_noise
-from ..training import (MAX_TYPES, MS_NSLAB, Adam, FlatParams, SlabArena, _saves, _Timer, emb_args,
+from ..training import (MAX_TYPES, MS_NSLAB, FlatParams, SlabArena, _saves, _Timer, emb_args,
                         embedding_backward, encode_nodes_backward, nslab_table, typed_embedding)
 from . import ms_engine
 from .ms_engine import EDGE_TYPES
@@ -285,12 +286,12 @@ class MultiScaleTrainer:
     def __init__(self, simulator, lr_init: float = 1e-3, lr_decay: float = 0.1,
                  lr_decay_steps: int = 15000, noise_std: float = 0.02,
                  loss_weight_position: float = 1.0, loss_weight_strain: float = 1.0,
-                 group=None, nslab: int = MS_NSLAB):
+                 group=None, nslab: int = MS_NSLAB, optimizer: str = "adam"):
         self.fused = fused_trainable(simulator)
         self.sim = simulator
         self.gnn = simulator._multi_scale_gnn
         self.flat = FlatParams(simulator)
-        self.opt = Adam(self.flat, lr_init)
+        self.opt = make_optimizer(optimizer, self.flat, simulator, lr_init)
         self.grads = {k: p.grad for k, p in simulator.named_parameters()}
         self.lr_init, self.lr_decay, self.lr_decay_steps = lr_init, lr_decay, lr_decay_steps
         self.noise_std = noise_std

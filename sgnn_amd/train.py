@@ -22,6 +22,7 @@ import torch
 import torch.distributed as dist
 
 from . import engine, training
+from .muon import make_optimizer
 
 
 def device_random_walk_noise(position_sequence: torch.Tensor, noise_std_last_step: float,
@@ -221,13 +222,13 @@ class Trainer:
     def __init__(self, simulator, lr_init: float = 1e-3, lr_decay: float = 0.1,
                  lr_decay_steps: int = 30000, noise_std: float = 0.02,
                  loss_weight_position: float = 1.0, loss_weight_strain: float = 1.0,
-                 group=None, nslab: Optional[int] = None):
+                 group=None, nslab: Optional[int] = None, optimizer: str = "adam"):
         self.sim = simulator
         self.epd = simulator._encode_process_decode
         # the fused kernels where they are built for the widths, else the width-generic autograd path
         self.fused = training.fused_trainable(self.epd, simulator._nparticle_types)
         self.flat = training.FlatParams(simulator)
-        self.opt = training.Adam(self.flat, lr_init)
+        self.opt = make_optimizer(optimizer, self.flat, simulator, lr_init)   # "adam" (train.py:199) or "muon"
         self.grads: Dict[str, torch.Tensor] = {k: p.grad for k, p in simulator.named_parameters()}
         self.lr_init, self.lr_decay, self.lr_decay_steps = lr_init, lr_decay, lr_decay_steps
         self.noise_std = noise_std
@@ -474,7 +475,8 @@ def train(simulator, metadata: dict, device, config: dict, group=None, log_every
     trainer = Trainer(simulator, lr_init=config["lr_init"], lr_decay=config["lr_decay"],
                       lr_decay_steps=config["lr_decay_steps"], noise_std=config["noise_std"],
                       loss_weight_position=config.get("loss_weight_position", 1.0),
-                      loss_weight_strain=config.get("loss_weight_strain", 1.0), group=group)
+                      loss_weight_strain=config.get("loss_weight_strain", 1.0), group=group,
+                      optimizer=config.get("optimizer", "adam"))
     if config.get("model_file"):
         model_dir = os.path.join(config["model_path"], config["run_name"]) + "/"
         checkpoint_utils.load_model(simulator, model_dir, config["model_file"], config["train_state_file"],

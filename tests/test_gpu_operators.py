@@ -568,3 +568,127 @@ def test_runs_repeat_bit_for_bit():
         runs.append([y.detach(), *grads, muon.newton_schulz(grads[0])])
     for other in runs[1:]:
         assert all(torch.equal(a, c) for a, c in zip(runs[0], other))
+
+
+# ----------------------------------------------------------------------------- the framework's paths
+@pytest.mark.parametrize("dtype,activation", [(torch.float32, torch.nn.GELU), (torch.float32, torch.nn.SiLU),
+                                              (torch.bfloat16, torch.nn.ReLU), (torch.float16, torch.nn.GELU)],
+                         ids=["f32-gelu", "f32-silu", "bf16-relu", "f16-gelu"])
+def test_modules_run_on_the_typed_operators(dtype, activation):
+    """build_mlp's other activations and 16-bit parameters: an Encoder and an InteractionNetwork block, forward and
+    every parameter's gradient against the same modules in float64 (norm-wise: fp32 1e-5; 16-bit types 12 roundings
+    of the type along the chain)."""
+    from sgnn_amd import graph_network as G
+    torch.manual_seed(3)
+
+    def mlp(i, h, o):
+        return torch.nn.Sequential(G.build_mlp(i, [h], o, activation=activation), torch.nn.LayerNorm(o))
+    enc, net = G.Encoder(7, 40, 3, 40, 1, 40), G.InteractionNetwork(40, 40, 40, 40, 1, 40)
+    enc.node_fn, enc.edge_fn, net.node_fn, net.edge_fn = mlp(7, 40, 40), mlp(3, 40, 40), mlp(80, 40, 40), mlp(120, 40, 40)
+    mods = torch.nn.ModuleList([enc, net]).to(dtype)
+    ref = {k: v.detach().double().requires_grad_(True) for k, v in mods.state_dict().items()}
+    mods = mods.cuda()
+    n, E = 60, 300
+    x, e = normal((n, 7), 1).to(dtype).float(), normal((E, 3), 2).to(dtype).float()
+    ei = torch.from_numpy(np.random.default_rng(3).integers(0, n, (2, E)))
+    w = normal((n, 40), 4)
+
+    def mlp64(p, v):
+        h = torch.nn.functional.linear(v, ref[p + "0.NN-0.weight"], ref[p + "0.NN-0.bias"])
+        h = torch.nn.functional.linear(activation()(h), ref[p + "0.NN-1.weight"], ref[p + "0.NN-1.bias"])
+        return torch.nn.functional.layer_norm(h, (h.shape[1],), ref[p + "1.weight"], ref[p + "1.bias"])
+    hx, he = mlp64("0.node_fn.", x.double()), mlp64("0.edge_fn.", e.double())
+    m = mlp64("1.edge_fn.", torch.cat([hx[ei[1]], hx[ei[0]], he], 1))
+    want = hx + mlp64("1.node_fn.", torch.cat([torch.zeros(n, 40, dtype=torch.float64).index_add(0, ei[1], m), hx], 1))
+    (want * w.double()).sum().backward()
+    h0, e0 = enc(x.cuda(), e.cuda())
+    got, _ = net(h0, ei.cuda(), e0)
+    (got.float() * w.cuda()).sum().backward()
+    h = half_step(dtype)
+    tol = 1e-5 if dtype == torch.float32 else 12 * h
+    got, want = got.detach(), want.detach()
+    assert float((got.double().cpu() - want).norm() / want.norm()) <= tol
+    if activation is torch.nn.ReLU:
+        # ReLU's slope jumps: after eight roundings of h / sqrt 3 (rms) each, z is off by a relative e = h sqrt(8 / 3);
+        # of two normal variables that far apart a share e / pi have different signs, and as half of the slopes are 1,
+        # the dz of one layer are off by sqrt(2 e / pi) in the norm; two such layers lie on the path
+        tol += (2 * 2 * h * (8 / 3) ** 0.5 / np.pi) ** 0.5
+    for k, p in mods.named_parameters():
+        assert float((p.grad.double().cpu() - ref[k].grad).norm() / ref[k].grad.norm()) <= tol, k
+
+
+def _adam64(p, g, m, v, t, lr, b1=0.9, b2=0.999, eps=1e-8):
+    m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    return p - lr / (1 - b1 ** t) * m / ((v / (1 - b2 ** t)).sqrt() + eps), m, v
+
+
+def test_muon_steps_against_64_bits():
+    """Three steps on a module of several shapes (the update's formula in muon.Muon's docstring); a state_dict taken
+    after two of them continues to the same bits."""
+    from sgnn_amd import muon, training
+    def make():
+        torch.manual_seed(1)
+        return torch.nn.Sequential(torch.nn.Linear(5, 40), torch.nn.Linear(40, 40), torch.nn.LayerNorm(40),
+                                   torch.nn.Linear(40, 72), torch.nn.Linear(72, 3)).cuda()
+    module = make()
+    flat = training.FlatParams(module)
+    opt = muon.Muon(flat, module, lr=0.01, weight_decay=0.1)
+    params = list(module.parameters())
+    matrix = [p.dim() == 2 and min(p.shape) >= 16 for p in params]
+    assert sum(matrix) == 2 and opt.is_matrix == matrix
+    p64 = [p.detach().double().cpu() for p in params]
+    m64, v64 = [torch.zeros_like(p) for p in p64], [torch.zeros_like(p) for p in p64]
+    for t in range(1, 4):
+        for i, p in enumerate(params):
+            g = normal(tuple(p.shape), 100 * t + i, 0.1)
+            p.grad.copy_(g)
+            g = g.double()
+            if matrix[i]:
+                m64[i] = 0.95 * m64[i] + g
+                o = ns64(g + 0.95 * m64[i])
+                p64[i] = p64[i] - 0.01 * (0.2 * max(p.shape) ** 0.5 * o + 0.1 * p64[i])
+            else:
+                p64[i], m64[i], v64[i] = _adam64(p64[i], g, m64[i], v64[i], t, 0.01)
+        if t == 3:
+            saved, grads = opt.state_dict(), flat.grad.clone()
+            other = make()
+            flat2 = training.FlatParams(other)
+            flat2.param.copy_(flat.param)
+            opt2 = muon.Muon(flat2, other, lr=9.0)
+            opt2.load_state_dict(saved)
+            flat2.grad.copy_(grads)
+        opt.step()
+        for i, (p, ref) in enumerate(zip(params, p64)):
+            # the update's own tolerance (ns_tol at 40 + 72), on an update of lr * 0.2 * sqrt(72); Adam: a few u
+            tol = ns_tol(ref, torch.float32, 40, 72) * 3 if matrix[i] else 1e-4
+            assert float((p.detach().double().cpu() - ref).norm()) <= tol * (0.02 * ref.numel() ** 0.5) + 8 * U * float(ref.norm()), (t, i)
+    opt2.step()
+    assert torch.equal(flat2.param, flat.param)
+
+
+def test_trainer_takes_muon(tmp_path):
+    """Trainer(optimizer="muon") trains, checkpoints and resumes; an unknown name and another optimiser's state are
+    refused."""
+    from sgnn_amd import data as D, train as T
+    from tests.test_gpu_harness import _config, _dataset
+    md = _dataset(str(tmp_path))
+    cfg = dict(_config(tmp_path), optimizer="muon")
+    dev = torch.device("cuda")
+    torch.manual_seed(0)
+    sim = T._get_simulator(D.read_metadata(str(tmp_path)), 0.02, 0.02, dev, cfg).to(dev)
+    before = {k: v.clone() for k, v in sim.state_dict().items()}
+    res = T.train(sim, md, dev, cfg, log_every=1)
+    assert res["step"] == 4 and all(np.isfinite(l) for _, l in res["history"])
+    # (the embedding of the one particle type is not read and keeps its values)
+    assert all(not torch.equal(before[k], v) for k, v in sim.state_dict().items()
+               if k.endswith("weight") and "embedding" not in k)
+    cfg2 = dict(cfg, model_file="model-best-000002.pt", train_state_file="train_state-best-000002.pt",
+                ntraining_steps=5, nsave_steps=0)
+    sim2 = T._get_simulator(md, 0.02, 0.02, dev, cfg).to(dev)
+    res2 = T.train(sim2, md, dev, cfg2, log_every=1)
+    assert res2["step"] == 5 and res2["trainer"].opt.step_count == 5
+    with pytest.raises(ValueError, match="optimizer"):
+        T.Trainer(sim2, optimizer="sgd")
+    adam = T.Trainer(sim2)
+    with pytest.raises(ValueError, match="Muon"):
+        T.Trainer(sim2, optimizer="muon").opt.load_state_dict(adam.opt.state_dict())

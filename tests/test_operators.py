@@ -96,3 +96,18 @@ def test_python_entry_points_refuse_cpu_tensors():
         functional.layer_norm(x)
     with pytest.raises(ValueError, match="GPU"):
         muon.newton_schulz(x)
+
+
+@pytest.mark.parametrize("bad", [dict(nseg=-1), dict(segs=None), dict(param=None), dict(update=None), dict(step=0)])
+def test_muon_kernels_refuse(lib, bad):
+    a = dict(segs=P, nseg=2, param=P, update=P, step=1)
+    a.update(bad)
+    assert lib.sgnn_muon_moments(a["segs"], a["nseg"], a["param"], P, P, P, a["update"], 0.95, 1, 0.1, 0.9, 0.999, 1e-8,
+                                 a["step"], None) == INVALID
+    if "step" not in bad:
+        assert lib.sgnn_muon_apply(a["segs"], a["nseg"], a["param"], a["update"], 0.1, 0.0, None) == INVALID
+
+
+def test_optimizer_names():
+    with pytest.raises(ValueError, match="adam"):
+        muon.make_optimizer("sgd", None, None, 0.1)
