@@ -14,11 +14,12 @@ LIBDIR = os.path.join(HERE, "_lib")
 LIB = os.path.join(LIBDIR, "libsgnn_hip.so")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-shared",
-         "-ffp-contract=fast", "-munsafe-fp-atomics", "-Wno-unused-result"]
+         "-ffp-contract=fast", "-munsafe-fp-atomics", "-Wno-unused-result",
+         # no packed fp32 instructions: some of their forms have given wrong results now and then (the host pass
+         # says that it does not know the feature)
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
-# packed fp32 instructions stay off in the typed operators' units (some of their forms have given wrong results)
-NO_PACKED_FP32 = {"gemm.hip", "linear.hip", "norm.hip", "muon.hip"}
 # the radius search's translation unit without FMA contraction: its graphs are bit-exact against the
 # oracle's `dims summed in order, no contraction` rule (the distance blocks of the other units carry
 # `#pragma clang fp contract(off)` as well)
@@ -29,8 +30,6 @@ def flags_for(src: str):
     f = [x for x in FLAGS if x != "-shared"]
     if os.path.basename(src) in NO_CONTRACT:
         f = ["-ffp-contract=off" if x == "-ffp-contract=fast" else x for x in f]
-    if os.path.basename(src) in NO_PACKED_FP32:
-        f += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
     return f
 
 
