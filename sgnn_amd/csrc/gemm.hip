@@ -1,10 +1,10 @@
 // One matrix product for every operand type and storage order (gemm.h).
 //
-//   k_gemm16   bf16 / fp16 operands on v_mfma_f32_16x16x32: double-buffered LDS tiles of 64 k, filled by the
-//              direct-to-LDS loads where the operands' rows are 16-byte aligned, through registers elsewhere
-//   k_gemm32   fp32 operands as three bf16 parts each (8 + 8 + 8 bits, split exactly while they are staged), six
-//              bf16 products per fp32 one
-//   k_gemm_row few rows of x: each wave streams its share of w's rows into registers, LDS only for the join
+//   k_gemm16     bf16 / fp16 operands on v_mfma_f32_16x16x32: double-buffered LDS tiles of 64 k, filled by the
+//                direct-to-LDS loads where the operands' rows are 16-byte aligned, through registers elsewhere
+//   k_gemm32     fp32 operands as three bf16 parts each (8 + 8 + 8 bits, split exactly while they are staged), six
+//                bf16 products per fp32 one
+//   k_gemm_rows  up to 32 rows of x: the waves stream their shares of w's rows into registers, LDS only for the join
 //
 // Both tiled kernels hold D[n][m] (w's rows on the accumulators' rows, x's on the lanes): a lane then has four
 // consecutive n of one m, which go through LDS once more so that the epilogue's loads and stores are whole
@@ -144,16 +144,18 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 // ----------------------------------------------------------------------------- 16-bit operands
 // BM x BN outputs per workgroup, WM x WN waves.  DIRECT: both operands' lines are 16-byte aligned (and in the cols
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
-template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT>
+// NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
+// longer than memory; the small tile has four.
+template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT, int NST>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   constexpr int BK = 64, kThreads = 64 * WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile16<BM, BK, ACOLS>;
   using TB = Tile16<BN, BK, BCOLS>;
   constexpr int kStage = TA::kBytes + TB::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];  // two stages of A's and B's tiles
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStage];  // stages of A's and B's tiles
   constexpr int RP = TM < 4 ? TM : 4, kBuf = RP * 16 * 16 * TN;
-  static_assert(kBuf * 4 * WM * WN <= 2 * kStage, "the epilogue's buffers fit");
+  static_assert(kBuf * 4 * WM * WN <= NST * kStage, "the epilogue's buffers fit");
   const int w = wave_id(), wm = w / WN, wn = w % WN;
   int tm, tn;
   tile_of(g, tm, tn);
@@ -187,18 +189,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     }
   };
   constexpr int PA = BM * BK / 8 / kThreads, PB = BN * BK / 8 / kThreads;
-  u32x4 va[PA], vb[PB];
-  const auto fetch = [&](int blk) {
+  const auto fetch = [&](u32x4(&va)[PA], u32x4(&vb)[PB], int blk) {
     TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
     TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
   };
-  const auto put = [&](char* a) {
+  const auto put = [&](char* a, const u32x4(&va)[PA], const u32x4(&vb)[PB]) {
     TA::template put<kThreads>(a, va);
     TB::template put<kThreads>(a + TA::kBytes, vb);
   };
-  char* here = lds;
-  char* there = lds + kStage;
-  // One barrier per block: past it, this block's tiles are whole and the other stage is read by no wave any more.
+  // One barrier per block: past it, this block's tiles are whole and the stage before it is read by no wave any more.
   if constexpr (DIRECT) {
     uint32_t oa[PA], ob[PB];
     TA::template offsets<kThreads>(oa, g.lda, g.M, m0);
@@ -210,33 +209,66 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
       if ((int64_t)(blk + 1) * BK <= g.K) {
         TA::template direct<kThreads>(a, pa + blk * sa, oa);
         TB::template direct<kThreads>(a + TA::kBytes, pb + blk * sb, ob);
-      } else {
-        fetch(blk);
-        put(a);
+      } else {  // its loads are waited for here, and with them all before them
+        u32x4 va[PA], vb[PB];
+        fetch(va, vb, blk);
+        put(a, va, vb);
       }
     };
-    if (first < last) stage(here, first);
+#pragma unroll
+    for (int i = 0; i < NST - 1; ++i)
+      if (first + i < last) stage(lds + i * kStage, first + i);
+    int at = 0;
     for (int blk = first; blk < last; ++blk) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      wait_stages<PA + PB, NST - 2>(last - 1 - blk);
       __syncthreads();
-      if (blk + 1 < last) stage(there, blk + 1);
-      compute(here);
-      char* t = here;
-      here = there, there = t;
+      if (blk + NST - 1 < last) stage(lds + (at == 0 ? NST - 1 : at - 1) * kStage, blk + NST - 1);
+      compute(lds + at * kStage);
+      at = at == NST - 1 ? 0 : at + 1;
     }
   } else {
-    // the next block waits in registers while this one's products run
-    if (first < last) {
-      fetch(first);
-      put(here);
-    }
-    for (int blk = first; blk < last; ++blk) {
+    // The partial block of k (or all, of an operand too narrow for 16 bytes) one after the other; then whole blocks,
+    // DEPTH of them waiting in registers.  Their loads stand outside any branch (past the end the last block is
+    // loaded again), or the compiler waits for all of them at each use.
+    static_assert(NST == 2, "two stages");
+    constexpr int DEPTH = BM > 64 ? 2 : 4;
+    const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
+    const int whole = plain ? min(last, (int)(g.K / BK)) : first;
+    u32x4 va[DEPTH][PA], vb[DEPTH][PB];
+    for (int blk = max(whole, first); blk < last; ++blk) {
+      fetch(va[0], vb[0], blk);
+      put(lds, va[0], vb[0]);
       __syncthreads();
-      if (blk + 1 < last) fetch(blk + 1);
-      compute(here);
-      if (blk + 1 < last) put(there);
-      char* t = here;
-      here = there, there = t;
+      compute(lds);
+      __syncthreads();
+    }
+    if (first < whole) {
+      uint32_t oa[PA], ob[PB], move_a, move_b;
+      TA::template places<kThreads>(oa, move_a, g.lda, g.M, m0);
+      TB::template places<kThreads>(ob, move_b, g.ldb, g.N, n0);
+      const char* pa = A + 2 * (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda);
+      const char* pb = B + 2 * (BCOLS ? n0 - TB::lead(n0) : n0 * g.ldb);
+      const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
+      const bool edge_a = m0 + BM > g.M, edge_b = n0 + BN > g.N;
+      const auto get = [&](u32x4(&a)[PA], u32x4(&b)[PB], int blk) {
+        blk = min(blk, whole - 1);
+        TA::fetch_whole(a, pa + blk * sa, oa);
+        TB::fetch_whole(b, pb + blk * sb, ob);
+      };
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) get(va[u], vb[u], first + u);
+      for (int blk = first; blk < whole; blk += DEPTH) {
+#pragma unroll
+        for (int u = 0; u < DEPTH; ++u) {
+          // past the end: the same block once more, whose products are not formed
+          char* a = lds + (u & 1) * kStage;
+          TA::template put_moved<kThreads>(a, va[u], move_a, edge_a);
+          TB::template put_moved<kThreads>(a + TA::kBytes, vb[u], move_b, edge_b);
+          get(va[u], vb[u], blk + u + DEPTH);
+          __syncthreads();
+          if (blk + u < whole) compute(a);
+        }
+      }
     }
   }
   __syncthreads();
@@ -265,15 +297,56 @@ SGNN_DEV void split3(f32x4 v, u32x2& hi, u32x2& mid, u32x2& lo) {
   }
 }
 
-// R rows by 32 k as three planes of bf16, row r's chunk c (8 k) at slot c ^ ((r >> 2) & 3): 16 rows' chunks of one
-// read cover all banks.
+// R rows by 32 k as three planes of bf16, 64 bytes a row.  Rows layout: row r's chunk c (8 k) at slot c ^ ((r >> 2) & 3).
+// Cols layout, whose writers hold four rows each and write one of them at a time: the rows 4 i + e of one e stand next
+// to each other, chunk c at slot c ^ e.  In both the 16 rows' chunks of one read, and 32 lanes' pieces of one write,
+// cover all banks.
 template <int R, bool COLS>
 struct Tile32 {
   static constexpr int BK = 32, kPlane = R * BK * 2, kBytes = 3 * kPlane;
   static SGNN_DEV int at(int row, int k) {  // byte of element (row, k)
+    if constexpr (COLS) return ((row & 3) * (R / 4) + (row >> 2)) * 64 + (((k >> 3) ^ (row & 3)) * 16) + (k & 7) * 2;
     return row * 64 + (((k >> 3) ^ ((row >> 2) & 3)) * 16) + (k & 7) * 2;
   }
-  // Rows: KPER x four k of one row.  Cols: one block of KPER k (two or four) by four rows.
+  // Cols: this thread's block of KPER k by four rows.  Four threads side by side read 64 bytes of a line; the next bits
+  // are the k, so that 32 lanes write 32 different 8 (4) byte pieces of 256 bytes.
+  template <int KPER>
+  static SGNN_DEV int block_k() { return (threadIdx.x >> 2) % (BK / KPER) * KPER; }
+  template <int KPER>
+  static SGNN_DEV int block_row() { return ((threadIdx.x >> 2) / (BK / KPER) * 4 + (threadIdx.x & 3)) * 4; }
+  // Rows: KPER x four k of one row.  Cols: one block of KPER k (two or four) by four rows.  Whole blocks as Tile16's.
+  static SGNN_DEV bool plain(int64_t ld, int64_t rows) { return ld < kNear && (!COLS || rows >= 4); }
+  static SGNN_DEV int lead(int64_t r0) { return COLS && r0 > 0 ? 4 : 0; }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void places(uint32_t (&o)[KPER], int& move, int64_t ld, int64_t rows, int64_t r0) {
+    const int left = (int)min(rows - r0, (int64_t)R);
+    move = 0;
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      if constexpr (COLS) {
+        const int line = block_k<KPER>() + i, col = block_row<KPER>(), from = min(col, left - 4);
+        move = min(col - from, 4);
+        o[i] = 4 * ((uint32_t)line * (uint32_t)ld + (uint32_t)(lead(r0) + from));
+      } else {
+        const int q = i * THREADS + threadIdx.x;
+        o[i] = 4 * ((uint32_t)min(q / 8, left - 1) * (uint32_t)ld + q % 8 * 4);
+      }
+    }
+  }
+  template <int KPER>
+  static SGNN_DEV void fetch_whole(f32x4 (&v)[KPER], const char* first, const uint32_t (&o)[KPER]) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i)
+      v[i] = __builtin_bit_cast(f32x4, (u32x4)*reinterpret_cast<const u32x4_any*>(first + o[i]));
+  }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void put_moved(char* lds, const f32x4 (&v)[KPER], int move, bool edge) {
+    if (!COLS || !edge) return put<THREADS>(lds, v);
+    f32x4 t[KPER];
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) t[i] = __builtin_bit_cast(f32x4, move_down(__builtin_bit_cast(u32x4, v[i]), 4 * move));
+    put<THREADS>(lds, t);
+  }
   template <int THREADS, int KPER>
   static SGNN_DEV void fetch(f32x4 (&v)[KPER], const float* src, int64_t ld, int64_t rows, int64_t K, int64_t r0,
                              int64_t k0) {
@@ -281,7 +354,7 @@ struct Tile32 {
     for (int i = 0; i < KPER; ++i) {
       int64_t line, col, lines, most;
       if constexpr (COLS) {
-        line = k0 + threadIdx.x / (R / 4) * KPER + i, col = r0 + threadIdx.x % (R / 4) * 4, lines = K, most = rows;
+        line = k0 + block_k<KPER>() + i, col = r0 + block_row<KPER>(), lines = K, most = rows;
       } else {
         const int q = i * THREADS + threadIdx.x;
         line = r0 + q / 8, col = k0 + q % 8 * 4, lines = rows, most = K;
@@ -314,7 +387,7 @@ struct Tile32 {
       }
     } else {
       static_assert(KPER == 2 || KPER == 4, "a block's k fit one LDS word or two");
-      const int k = threadIdx.x / (R / 4) * KPER, r = threadIdx.x % (R / 4) * 4;
+      const int k = block_k<KPER>(), r = block_row<KPER>();
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int o = at(r + e, k);
@@ -341,16 +414,17 @@ struct Tile32 {
 // a b = sum of the parts' products; left out are mid lo, lo mid and lo lo, below 2^-22 of |a b| together.
 // An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
 // are not finite are formed once more in plain fp32 (`again`).
-template <bool ACOLS, bool BCOLS, int BM, int BN>
+// DEPTH blocks of k wait in registers; NST stages of LDS (with two, one barrier per block).
+template <bool ACOLS, bool BCOLS, int BM, int BN, int DEPTH, int NST>
 __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
   constexpr int BK = 32, kThreads = 256, WM = 2, WN = 2;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile32<BM, ACOLS>;
   using TB = Tile32<BN, BCOLS>;
-  __shared__ __attribute__((aligned(16))) char lds[TA::kBytes + TB::kBytes];
-  char *sa = lds, *sb = lds + TA::kBytes;
+  constexpr int kStage = TA::kBytes + TB::kBytes;
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
   constexpr int RP = 2, kBuf = RP * 16 * 16 * TN;
-  static_assert(kBuf * 4 * WM * WN <= TA::kBytes + TB::kBytes, "the epilogue's buffers fit");
+  static_assert(kBuf * 4 * WM * WN <= NST * kStage, "the epilogue's buffers fit");
   const int w = wave_id(), wm = w / WN, wn = w % WN, l = lane_id();
   int tm, tn;
   tile_of(g, tm, tn);
@@ -367,17 +441,10 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  f32x4 va[BM * BK / 4 / kThreads], vb[BN * BK / 4 / kThreads];
-  const auto fetch = [&](int blk) {
-    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
-    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
-  };
-  if (first < last) fetch(first);
-  for (int blk = first; blk < last; ++blk) {
-    TA::template put<kThreads>(sa, va);
-    TB::template put<kThreads>(sb, vb);
-    __syncthreads();
-    if (blk + 1 < last) fetch(blk + 1);
+  constexpr int PA = BM * BK / 4 / kThreads, PB = BN * BK / 4 / kThreads;
+  f32x4 va[DEPTH][PA], vb[DEPTH][PB];
+  const auto compute = [&](const char* sa) {
+    const char* sb = sa + TA::kBytes;
     s16x8 fb[TN][3];
 #pragma unroll
     for (int j = 0; j < TN; ++j)
@@ -402,8 +469,49 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
 #pragma unroll
       for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[0], acc[i][j]);
     }
+  };
+  // As in k_gemm16: the partial block (or all, of an operand too narrow) first, then whole blocks without branches.
+  const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
+  const int whole = plain ? min(last, (int)(g.K / BK)) : first;
+  for (int blk = max(whole, first); blk < last; ++blk) {
+    TA::template fetch<kThreads>(va[0], A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+    TB::template fetch<kThreads>(vb[0], B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
+    TA::template put<kThreads>(lds, va[0]);
+    TB::template put<kThreads>(lds + TA::kBytes, vb[0]);
+    __syncthreads();
+    compute(lds);
     __syncthreads();
   }
+  if (first < whole) {
+    uint32_t oa[PA], ob[PB];
+    int move_a, move_b;
+    TA::template places<kThreads>(oa, move_a, g.lda, g.M, m0);
+    TB::template places<kThreads>(ob, move_b, g.ldb, g.N, n0);
+    const char* pa = reinterpret_cast<const char*>(A + (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda));
+    const char* pb = reinterpret_cast<const char*>(B + (BCOLS ? n0 - TB::lead(n0) : n0 * g.ldb));
+    const int64_t step_a = 4 * BK * (ACOLS ? g.lda : 1), step_b = 4 * BK * (BCOLS ? g.ldb : 1);
+    const bool edge_a = m0 + BM > g.M, edge_b = n0 + BN > g.N;
+    const auto get = [&](f32x4(&a)[PA], f32x4(&b)[PB], int blk) {
+      blk = min(blk, whole - 1);
+      TA::fetch_whole(a, pa + blk * step_a, oa);
+      TB::fetch_whole(b, pb + blk * step_b, ob);
+    };
+#pragma unroll
+    for (int u = 0; u < DEPTH; ++u) get(va[u], vb[u], first + u);
+    for (int blk = first; blk < whole; blk += DEPTH) {
+#pragma unroll
+      for (int u = 0; u < DEPTH; ++u) {
+        char* a = lds + (NST == 2 ? (u & 1) * kStage : 0);
+        TA::template put_moved<kThreads>(a, va[u], move_a, edge_a);
+        TB::template put_moved<kThreads>(a + TA::kBytes, vb[u], move_b, edge_b);
+        get(va[u], vb[u], blk + u + DEPTH);
+        __syncthreads();
+        if (blk + u < whole) compute(a);
+        if constexpr (NST == 1) __syncthreads();
+      }
+    }
+  }
+  __syncthreads();
   const int64_t k0 = (int64_t)first * BK, k1 = min((int64_t)last * BK, g.K);
 #pragma unroll
   for (int i = 0; i < TM; ++i)
@@ -427,6 +535,93 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
     }
   write_tile<float, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, batch, split, m0 + wm * TM * 16,
                         n0 + wn * TN * 16);
+}
+
+// ----------------------------------------------------------------------------- few rows
+// M <= 16 MT rows of x, both operands with k contiguous: a workgroup takes 16 MT columns n, its W waves every W-th block
+// of k, straight from memory into the matrix instructions' registers (a lane reads 32 or 64 bytes of one row of w at a
+// time, a row's four lanes 128 or 256), and the waves' sums are added in order through LDS.  Bounded by w's bytes.
+template <typename T, int MT, int W>
+__global__ __launch_bounds__(64 * W) void k_gemm_rows(GemmArgs g) {
+  constexpr bool k32 = sizeof(T) == 4;
+  constexpr int BK = 64, V = 16 / sizeof(T), kLoads = 16 / V, U = MT == 1 ? 2 : 1;  // a lane's 16 k of a block
+  __shared__ float part[W][16 * MT][16 * MT + 4];
+  const int l = lane_id(), w = wave_id(), i = l & 15, kl = 16 * (l >> 4);
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * MT;
+  const T* A = static_cast<const T*>(g.A);
+  const T* B = static_cast<const T*>(g.B);
+  f32x4 acc[MT][MT];
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int b = 0; b < MT; ++b) acc[a][b] = f32x4{0, 0, 0, 0};
+  // 16 k of a row from k, as loaded; zeros past K and for rows that are not there
+  const auto load = [&](u32x4(&v)[kLoads], const T* p, int64_t k, bool there) {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      const int64_t c = k + q * V;
+      v[q] = u32x4{0, 0, 0, 0};
+      if (!there || c >= g.K) continue;
+      if (c + V <= g.K) {
+        v[q] = *reinterpret_cast<const u32x4_any*>(p + c);
+      } else {
+        typedef T TV __attribute__((ext_vector_type(V)));
+        TV t = __builtin_bit_cast(TV, v[q]);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (c + e < g.K) t[e] = p[c + e];
+        v[q] = __builtin_bit_cast(u32x4, t);
+      }
+    }
+  };
+  for (int64_t k0 = (int64_t)w * BK; k0 < g.K; k0 += (int64_t)W * BK * U) {
+    u32x4 xa[U][MT][kLoads], wb[U][MT][kLoads];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = k0 + (int64_t)u * W * BK + kl;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        const int64_t n = n0 + 16 * t + i, m = 16 * t + i;
+        load(wb[u][t], B + n * g.ldb, k, n < g.N);
+        load(xa[u][t], A + m * g.lda, k, m < g.M);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < kLoads; ++q)
+#pragma unroll
+        for (int a = 0; a < MT; ++a)
+#pragma unroll
+          for (int b = 0; b < MT; ++b) {
+            if constexpr (k32) {
+              const f32x4 p = __builtin_bit_cast(f32x4, wb[u][b][q]), x = __builtin_bit_cast(f32x4, xa[u][a][q]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                acc[a][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(p[e], x[e], acc[a][b], 0, 0, 0);
+            } else {
+              acc[a][b] = mfma16<T>(__builtin_bit_cast(s16x8, wb[u][b][q]), __builtin_bit_cast(s16x8, xa[u][a][q]), acc[a][b]);
+            }
+          }
+  }
+#pragma unroll
+  for (int a = 0; a < MT; ++a)
+#pragma unroll
+    for (int b = 0; b < MT; ++b)
+      *reinterpret_cast<f32x4*>(&part[w][16 * a + i][16 * b + 4 * (l >> 4)]) = acc[a][b];
+  __syncthreads();
+  constexpr int kPer = 16 * MT / V;  // 16-byte pieces of an output row
+  for (int t = threadIdx.x; t < 16 * MT * kPer; t += 64 * W) {
+    const int m = t / kPer, c = t % kPer * V;
+    if (m >= g.M || n0 + c >= g.N) continue;
+    float v[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = 0.0f;
+    for (int q = 0; q < W; ++q)
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] += part[q][m][c + e];
+    finish<T>(g, 0, m, n0 + c, v, (int)min((int64_t)V, g.N - n0 - c));
+  }
 }
 
 // ----------------------------------------------------------------------------- split k
@@ -481,34 +676,49 @@ Plan plan_of(const Gemm& g) {
   return p;
 }
 
-template <typename T, bool AC, bool BC, int BM, int BN, int WM, int WN>
-void launch16(const GemmArgs& g, dim3 grid, bool direct, hipStream_t s) {
-  if (direct)
-    hipLaunchKernelGGL((k_gemm16<T, AC, BC, BM, BN, WM, WN, true>), grid, dim3(64 * WM * WN), 0, s, g);
-  else
-    hipLaunchKernelGGL((k_gemm16<T, AC, BC, BM, BN, WM, WN, false>), grid, dim3(64 * WM * WN), 0, s, g);
-}
-
 template <typename T, bool AC, bool BC>
 void launch_tiles(const GemmArgs& g, const Plan& p, dim3 grid, bool direct, hipStream_t s) {
   if constexpr (std::is_same_v<T, float>) {
     if (p.bm == 128)
-      hipLaunchKernelGGL((k_gemm32<AC, BC, 128, 128>), grid, dim3(256), 0, s, g);
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 128, 128, 1, 1>), grid, dim3(256), 0, s, g);
     else
-      hipLaunchKernelGGL((k_gemm32<AC, BC, 64, 64>), grid, dim3(256), 0, s, g);
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 64, 64, 4, 2>), grid, dim3(256), 0, s, g);
   } else {
-    if (p.bm == 256 && direct)
-      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 256, 256, 2, 4, true>), grid, dim3(512), 0, s, g);
+    if (p.bm == 256)
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 256, 256, 2, 4, true, 2>), grid, dim3(512), 0, s, g);
+    else if (p.bm == 128 && direct)
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 128, 128, 2, 2, true, 2>), grid, dim3(256), 0, s, g);
     else if (p.bm == 128)
-      launch16<T, AC, BC, 128, 128, 2, 2>(g, grid, direct, s);
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 128, 128, 2, 2, false, 2>), grid, dim3(256), 0, s, g);
+    else if (direct)
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 64, 64, 2, 2, true, 4>), grid, dim3(256), 0, s, g);
     else
-      launch16<T, AC, BC, 64, 64, 2, 2>(g, grid, direct, s);
+      hipLaunchKernelGGL((k_gemm16<T, AC, BC, 64, 64, 2, 2, false, 2>), grid, dim3(256), 0, s, g);
+  }
+}
+
+// The row kernel: 32 rows at most, and few enough columns per row of x that x's repeated reads stay below w's.
+bool rows_ok(const Gemm& g) { return !g.a_cols && !g.b_cols && g.batch == 1 && g.M <= 32; }
+
+template <typename T>
+void launch_rows(const GemmArgs& g, hipStream_t s) {
+  // a wave per 128 of k, up to eight
+  const bool many = g.K > 512;
+  const auto go = [&](auto kernel, int mt, int w) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)((g.N + 16 * mt - 1) / (16 * mt))), dim3(64 * w), 0, s, g);
+  };
+  if (g.M <= 16) {
+    if (many) go(k_gemm_rows<T, 1, 8>, 1, 8);
+    else go(k_gemm_rows<T, 1, 4>, 1, 4);
+  } else {
+    if (many) go(k_gemm_rows<T, 2, 8>, 2, 8);
+    else go(k_gemm_rows<T, 2, 4>, 2, 4);
   }
 }
 
 // Whether the direct-to-LDS loads serve an operand: 16-byte lines whose offsets within a tile fit 32 bits.
 bool direct_ok(const void* p, int64_t ld, int64_t batch, bool cols, int64_t rows) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && batch % 8 == 0 && ld < (1 << 22) &&
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && batch % 8 == 0 && ld < kNear &&
          (!cols || rows % 8 == 0);
 }
 
@@ -517,22 +727,30 @@ bool direct_ok(const void* p, int64_t ld, int64_t batch, bool cols, int64_t rows
 namespace sgnn {
 
 size_t gemm_workspace_bytes(const Gemm& g) {
-  if (g.M <= 0 || g.N <= 0 || g.K <= 0) return 0;
+  if (g.M <= 0 || g.N <= 0 || g.K <= 0 || rows_ok(g)) return 0;
   const int s = plan_of(g).nsplit;
   return s > 1 ? sizeof(float) * (size_t)s * (size_t)g.M * (size_t)g.N : 0;
 }
 
 int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* stream) {
   if (g.M == 0 || g.N == 0 || g.batch == 0) return SGNN_OK;
-  Plan p = plan_of(g);
   hipStream_t s = static_cast<hipStream_t>(stream);
+  GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
+             g.batch_b, g.batch_r, g.batch_c, g.act, 1, 0, 0, g.alpha, g.beta};
+  if (rows_ok(g)) {
+    with_type(g.dtype, [&](auto* t) {
+      launch_rows<std::remove_pointer_t<decltype(t)>>(a, s);
+      return 0;
+    });
+    return check_launch("gemm");
+  }
+  Plan p = plan_of(g);
   const bool direct = direct_ok(g.A, g.lda, g.batch_a, g.a_cols, g.M) && direct_ok(g.B, g.ldb, g.batch_b, g.b_cols, g.N);
   if (!direct && p.bm == 256) p.bm = p.bn = 128;
   const int64_t tm = (g.M + p.bm - 1) / p.bm, tn = (g.N + p.bn - 1) / p.bn;
   if (tm > INT32_MAX / tn || g.batch > 65535 || g.K > (int64_t)INT32_MAX * 32)
     return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k, or 65535 matrices");
-  GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
-             g.batch_b, g.batch_r, g.batch_c, g.act, p.nsplit, (int32_t)tm, (int32_t)tn, g.alpha, g.beta};
+  a.nsplit = p.nsplit, a.tiles_m = (int32_t)tm, a.tiles_n = (int32_t)tn;
   if (p.nsplit > 1) {
     if (!workspace || workspace_bytes < gemm_workspace_bytes(g))
       return set_error(SGNN_ERR_INVALID, "gemm: workspace too small");

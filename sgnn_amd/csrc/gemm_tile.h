@@ -18,6 +18,9 @@ SGNN_DEV f32x4 mfma16(s16x8 a, s16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(T8, a), __builtin_bit_cast(T8, b), c, 0, 0, 0);
 }
 
+// Leading dimensions below this keep a tile's byte offsets in 32 bits (256 lines of 4 bytes a value at most).
+constexpr int64_t kNear = 1 << 22;
+
 // One operand's tile in LDS: R rows (m or n) by BK of k, in 16-byte chunks.
 //   rows layout (k contiguous in memory): row r's chunk c (8 k) at slot c ^ swizzle(r)
 //   cols layout (m / n contiguous): k's chunk c (8 rows) at slot c ^ 2 h(k); read back transposed
@@ -65,7 +68,42 @@ struct Tile16 {
     }
   }
 
-  // The same through registers, at any alignment, with zeros past K (and past the last row, in cols).
+  // The same through registers, at any alignment: whole blocks of k by places(), like offsets().  In cols the chunks that
+  // the last row cuts, or that lie past it, are read 8 rows from the end and moved into place by put_moved(); `move`
+  // holds their distances, 4 bits each.  first: `lead` rows (0 or 8, as places() says) before the tile's first.
+  static SGNN_DEV bool plain(int64_t ld, int64_t rows) { return ld < kNear && (!COLS || rows >= 8); }
+  static SGNN_DEV int lead(int64_t r0) { return COLS && r0 > 0 ? 8 : 0; }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void places(uint32_t (&o)[KPER], uint32_t& move, int64_t ld, int64_t rows, int64_t r0) {
+    const int left = (int)min(rows - r0, (int64_t)R);
+    move = 0;
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) {
+      const int q = i * THREADS + threadIdx.x;
+      const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
+      if constexpr (COLS) {
+        const int from = min(8 * c, left - 8);  // down to -7 where r0 > 0
+        move |= (uint32_t)min(8 * c - from, 8) << (4 * i);
+        o[i] = 2 * ((uint32_t)line * (uint32_t)ld + (uint32_t)(lead(r0) + from));
+      } else {
+        o[i] = 2 * ((uint32_t)min(line, left - 1) * (uint32_t)ld + 8 * c);
+      }
+    }
+  }
+  template <int KPER>
+  static SGNN_DEV void fetch_whole(u32x4 (&v)[KPER], const char* first, const uint32_t (&o)[KPER]) {
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) v[i] = *reinterpret_cast<const u32x4_any*>(first + o[i]);
+  }
+  template <int THREADS, int KPER>
+  static SGNN_DEV void put_moved(char* lds, const u32x4 (&v)[KPER], uint32_t move, bool edge) {
+    if (!COLS || !edge) return put<THREADS>(lds, v);
+    u32x4 t[KPER];
+#pragma unroll
+    for (int i = 0; i < KPER; ++i) t[i] = move_down(v[i], 2 * (move >> (4 * i) & 15));
+    put<THREADS>(lds, t);
+  }
+  // Any block, with zeros past K (and past the last row, in cols).
   template <int THREADS, int KPER>
   static SGNN_DEV void fetch(u32x4 (&v)[KPER], const char* src, int64_t ld, int64_t rows, int64_t K, int64_t r0,
                              int64_t k0) {
@@ -112,5 +150,14 @@ struct Tile16 {
     }
   }
 };
+
+// Waits until at most `keep` stages' direct loads (PER of this wave each) are under way.
+template <int PER, int MOST>
+SGNN_DEV void wait_stages(int keep) {
+  static_assert(MOST <= 2 && PER * MOST < 64, "vmcnt's range");
+  if (MOST >= 2 && keep >= 2) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER * 2) : "memory");
+  else if (MOST >= 1 && keep >= 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"(PER) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+}
 
 }  // namespace sgnn

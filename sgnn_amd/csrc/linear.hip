@@ -11,7 +11,8 @@ constexpr int kThreads = 256;
 
 // How the pass over dy is cut: `lanes` threads side by side take a 16-byte piece each of a row, 256 / lanes rows at
 // once; `strips` such column strips, `blocks` row blocks.  About 2048 workgroups (8 per CU) keep enough loads in
-// flight for the memory's rate; the row blocks are also the partial sums of db, so there are at most 512.
+// flight for the memory's rate; the row blocks are also the partial sums of db, so there are at most 512, of four
+// passes at least.
 struct ActCut {
   int lanes;
   int64_t strips, blocks;
@@ -21,7 +22,7 @@ struct ActCut {
     while (lanes < kThreads && lanes < pieces) lanes *= 2;
     strips = (pieces + lanes - 1) / lanes;
     const int64_t passes = (M + kThreads / lanes - 1) / (kThreads / lanes);
-    blocks = std::max<int64_t>(1, std::min({passes, (int64_t)512, (2048 + strips - 1) / strips}));
+    blocks = std::max<int64_t>(1, std::min({(passes + 3) / 4, (int64_t)512, (2048 + strips - 1) / strips}));
   }
 };
 
@@ -39,19 +40,34 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
 #pragma unroll
   for (int i = 0; i < V; ++i) s[i] = 0.0f;
   if (cnt > 0) {
+    // four rows are loaded before the first is used
+    constexpr int U = 4;
     const int64_t step = (int64_t)gridDim.y * rows;
-#pragma unroll 2
-    for (int64_t r = (int64_t)blockIdx.y * rows + row; r < M; r += step) {
-      float v[V], t[V];
-      load_some<V>(dy + r * ldd + c, cnt, v);
-      if (slope) {
-        load_slopes<T>(slope, r * N + c, cnt, t);
+    for (int64_t r0 = (int64_t)blockIdx.y * rows + row; r0 < M; r0 += U * step) {
+      u32x4 up[U];
+      float t[U][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= t[i];
-        store_some<V>(dz + r * N + c, cnt, v);
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = r0 + u * step;
+        up[u] = u32x4{0, 0, 0, 0};
+        if (r >= M) continue;
+        up[u] = load_raw(dy + r * ldd + c, cnt);
+        if (slope) load_slopes<T>(slope, r * N + c, cnt, t[u]);
       }
 #pragma unroll
-      for (int i = 0; i < V; ++i) s[i] += v[i];
+      for (int u = 0; u < U; ++u) {
+        const int64_t r = r0 + u * step;
+        if (r >= M) continue;
+        float v[V];
+        unpack<T>(up[u], v);
+        if (slope) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) v[i] *= t[u][i];
+          store_some<V>(dz + r * N + c, cnt, v);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) s[i] += v[i];
+      }
     }
   }
   if (!partial) return;

@@ -89,15 +89,31 @@ __global__ __launch_bounds__(threads_of(G)) void k_norm(const T* x, int64_t ldx,
   }
 }
 
+// Two sums over a row's G lanes at once; turn: as in group_sum.
+template <int G>
+SGNN_DEV void group_sum2(float& a, float& b, float* red, int turn) {
+  a = lanes_sum<G <= 64 ? G : 64>(a);
+  b = lanes_sum<G <= 64 ? G : 64>(b);
+  if constexpr (G > 64) {
+    float* r = red + 2 * (G / 64) * turn;
+    if (lane_id() == 0) r[2 * wave_id()] = a, r[2 * wave_id() + 1] = b;
+    __syncthreads();
+    a = b = 0.0f;
+#pragma unroll
+    for (int w = 0; w < G / 64; ++w) a += r[2 * w], b += r[2 * w + 1];
+  }
+}
+
 // dx, and this workgroup's share of dgamma and dbeta: every lane sums its own columns over its rows (rows blockIdx,
 // + gridDim ... in order), the groups of one workgroup are added in order in LDS, and the workgroups' sums go to
-// partial [workgroup][2][width].  The next row is loaded before this one's sums are waited for.
+// partial [workgroup][2][width].  A row waits in registers as it was loaded (16-bit values packed) and is unpacked for
+// its sums and again for dx; the next row is loaded before this one's sums are waited for.
 template <typename T, typename W, int G, int NC>
 __global__ __launch_bounds__(threads_of(G)) void k_norm_bwd(const T* dy, int64_t ldd, const T* x, int64_t ldx,
                                                             const float* mean, const float* rstd, const W* gamma,
                                                             int64_t n, int width, T* dx, float* partial) {
   constexpr int V = 16 / sizeof(T), kGroups = threads_of(G) / G;
-  __shared__ float red[2][32];
+  __shared__ float red[G > 64 ? 4 * G / 64 : 1];
   __shared__ float join[kGroups > 1 ? (kGroups - 1) * G * NC * V : 1];
   const int i = threadIdx.x % G, grp = threadIdx.x / G;
   float ga[NC][V], dg[NC][V], db[NC][V];
@@ -109,45 +125,55 @@ __global__ __launch_bounds__(threads_of(G)) void k_norm_bwd(const T* dy, int64_t
     if (gamma) load_some<V>(gamma + c, width - c, ga[j]);
   }
   const int64_t step = (int64_t)gridDim.x * kGroups;
-  float xv[NC][V], up[NC][V], mu = 0.0f, rs = 0.0f;
+  u32x4 nx[NC], nu[NC];
+  float nmu = 0.0f, nrs = 0.0f;
   const auto load = [&](int64_t r) {
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
       const int c = (j * G + i) * V;
-      load_some<V>(x + r * ldx + c, width - c, xv[j]);
-      load_some<V>(dy + r * ldd + c, width - c, up[j]);
+      nx[j] = load_raw(x + r * ldx + c, width - c);
+      nu[j] = load_raw(dy + r * ldd + c, width - c);
     }
-    mu = mean[r], rs = rstd[r];
+    nmu = mean[r], nrs = rstd[r];
   };
   int64_t r = (int64_t)blockIdx.x * kGroups + grp;
   if (r < n) load(r);
   for (int turn = 0; r < n; r += step, turn ^= 1) {
-    float hat[NC][V], g[NC][V];
-    float sg = 0.0f, sgh = 0.0f;
-    const float rnow = rs;
+    u32x4 vx[NC], vu[NC];
+    const float mu = nmu, rs = nrs;
 #pragma unroll
-    for (int j = 0; j < NC; ++j)
+    for (int j = 0; j < NC; ++j) vx[j] = nx[j], vu[j] = nu[j];
+    if (r + step < n) load(r + step);
+    float sg = 0.0f, sgh = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      float xv[V], up[V];
+      unpack<T>(vx[j], xv);
+      unpack<T>(vu[j], up);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         // columns past the row read as 0 in dy: nothing of theirs is summed
-        hat[j][e] = (xv[j][e] - mu) * rs;
-        g[j][e] = up[j][e] * ga[j][e];
-        dg[j][e] += up[j][e] * hat[j][e];
-        db[j][e] += up[j][e];
-        sg += g[j][e];
-        sgh += g[j][e] * hat[j][e];
+        const float hat = (xv[e] - mu) * rs, g = up[e] * ga[j][e];
+        dg[j][e] += up[e] * hat;
+        db[j][e] += up[e];
+        sg += g;
+        sgh += g * hat;
       }
-    if (r + step < n) load(r + step);
+    }
     if (dx) {
-      sg = group_sum<G>(sg, red[0], turn) / width;
-      sgh = group_sum<G>(sgh, red[1], turn) / width;
+      group_sum2<G>(sg, sgh, red, turn);
+      sg /= width, sgh /= width;
 #pragma unroll
       for (int j = 0; j < NC; ++j) {
         const int c = (j * G + i) * V;
         if (c >= width) continue;
-        float o[V];
+        float xv[V], o[V];
+        // unpacked anew: the floats of the first time would be twice the registers across the barrier
+        asm volatile("" : "+v"(vx[j]), "+v"(vu[j]));
+        unpack<T>(vx[j], xv);
+        unpack<T>(vu[j], o);
 #pragma unroll
-        for (int e = 0; e < V; ++e) o[e] = rnow * (g[j][e] - sg - hat[j][e] * sgh);
+        for (int e = 0; e < V; ++e) o[e] = rs * (o[e] * ga[j][e] - sg - (xv[e] - mu) * rs * sgh);
         store_some<V>(dx + r * width + c, width - c, o);
       }
     }
@@ -268,8 +294,8 @@ __global__ __launch_bounds__(kSumThreads) void k_norm_reduce(const float* partia
   });
 }
 
-// Lanes per row and pieces per lane: the fewest lanes that leave a lane at most 16 values (the backward pass holds six
-// arrays of them: 150 registers, three waves per SIMD).
+// Lanes per row and pieces per lane: the fewest lanes that leave a lane at most 16 values (the backward pass holds
+// gamma and its two sums of them).
 struct NormCut {
   int G, NC;  // G = 0: the wide kernels
   NormCut(size_t size, int width) {
@@ -283,7 +309,7 @@ struct NormCut {
 // per CU for short rows; 2 for long ones, whose partial rows are as long), never more than there are rows for.
 int64_t bwd_blocks(const NormCut& cut, int64_t n) {
   const int64_t groups = cut.G == 0 || cut.G > 256 ? 1 : 256 / cut.G;
-  const int64_t most = cut.G == 16 ? 2048 : cut.G == 64 ? 1024 : cut.G == 256 ? 512 : 256;
+  const int64_t most = cut.G == 16 ? 2048 : cut.G <= 256 ? 1024 : 512;
   return std::max<int64_t>(1, std::min(most, (n + groups - 1) / groups));
 }
 

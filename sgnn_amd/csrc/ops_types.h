@@ -28,6 +28,16 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 // 16 bytes at any element's alignment (one global_load/store_dwordx4: unaligned access is on for this target)
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 
+// The 16 bytes n (0 .. 16, even) bytes further on; zeros move in.
+SGNN_DEV u32x4 move_down(u32x4 v, int n) {
+  if (n & 8) v = u32x4{v[2], v[3], 0, 0};
+  if (n & 4) v = u32x4{v[1], v[2], v[3], 0};
+  if (n & 2)
+    v = u32x4{v[0] >> 16 | v[1] << 16, v[1] >> 16 | v[2] << 16, v[2] >> 16 | v[3] << 16, v[3] >> 16};
+  if (n & 16) v = u32x4{0, 0, 0, 0};
+  return v;
+}
+
 // 16 bytes of T at any alignment <-> floats
 template <typename T>
 SGNN_DEV void load_vec(const T* p, float* v) {
@@ -45,6 +55,26 @@ SGNN_DEV void store_vec(T* p, const float* v) {
 #pragma unroll
   for (int i = 0; i < V; ++i) t[i] = from_float<T>(v[i]);
   *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, t);
+}
+// 16 bytes of T as they are in memory, the first cnt values there (the others 0), and their floats.
+template <typename T>
+SGNN_DEV u32x4 load_raw(const T* p, int cnt) {
+  constexpr int V = 16 / sizeof(T);
+  if (cnt >= V) return *reinterpret_cast<const u32x4_any*>(p);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  TV t = __builtin_bit_cast(TV, u32x4{0, 0, 0, 0});
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < cnt) t[i] = p[i];
+  return __builtin_bit_cast(u32x4, t);
+}
+template <typename T>
+SGNN_DEV void unpack(u32x4 raw, float* v) {
+  constexpr int V = 16 / sizeof(T);
+  typedef T TV __attribute__((ext_vector_type(V)));
+  const TV t = __builtin_bit_cast(TV, raw);
+#pragma unroll
+  for (int i = 0; i < V; ++i) v[i] = to_float(t[i]);
 }
 // N values of T, the first cnt of them there (the others read as 0, are not written).
 template <int N, typename T>
