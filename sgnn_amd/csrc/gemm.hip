@@ -414,10 +414,14 @@ struct Tile32 {
 // a b = sum of the parts' products; left out are mid lo, lo mid and lo lo, below 2^-22 of |a b| together.
 // An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
 // are not finite are formed once more in plain fp32 (`again`).
-// DEPTH blocks of k wait in registers; NST stages of LDS (with two, one barrier per block).
-template <bool ACOLS, bool BCOLS, int BM, int BN, int DEPTH, int NST>
-__global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
-  constexpr int BK = 32, kThreads = 256, WM = 2, WN = 2;
+// NST = 2 stages of LDS: the next block is split and written while this one's products run; a matrix instruction takes
+// 16 cycles, in which a wave issues three others (4096^3: 695 us, 198 TFLOP/s; 765 with one stage, where split and
+// products take turns and the two waves of a SIMD fall into step; other mixtures asked of the scheduler: 704 to 733).
+// NST = 1: half the LDS, so two workgroups per CU, one's epilogue beside the other's products: better where k is short
+// (200003 x 384 x 128, silu: 180 us against 211).
+template <bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, int NST>
+__global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
+  constexpr int BK = 32, kThreads = 64 * WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile32<BM, ACOLS>;
   using TB = Tile32<BN, BCOLS>;
@@ -442,7 +446,7 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
   constexpr int PA = BM * BK / 4 / kThreads, PB = BN * BK / 4 / kThreads;
-  f32x4 va[DEPTH][PA], vb[DEPTH][PB];
+  f32x4 va[PA], vb[PB];
   const auto compute = [&](const char* sa) {
     const char* sb = sa + TA::kBytes;
     s16x8 fb[TN][3];
@@ -474,10 +478,10 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
   const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
   const int whole = plain ? min(last, (int)(g.K / BK)) : first;
   for (int blk = max(whole, first); blk < last; ++blk) {
-    TA::template fetch<kThreads>(va[0], A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
-    TB::template fetch<kThreads>(vb[0], B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
-    TA::template put<kThreads>(lds, va[0]);
-    TB::template put<kThreads>(lds + TA::kBytes, vb[0]);
+    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
+    TA::template put<kThreads>(lds, va);
+    TB::template put<kThreads>(lds + TA::kBytes, vb);
     __syncthreads();
     compute(lds);
     __syncthreads();
@@ -496,18 +500,32 @@ __global__ __launch_bounds__(256) void k_gemm32(GemmArgs g) {
       TA::fetch_whole(a, pa + blk * step_a, oa);
       TB::fetch_whole(b, pb + blk * step_b, ob);
     };
-#pragma unroll
-    for (int u = 0; u < DEPTH; ++u) get(va[u], vb[u], first + u);
-    for (int blk = first; blk < whole; blk += DEPTH) {
-#pragma unroll
-      for (int u = 0; u < DEPTH; ++u) {
-        char* a = lds + (NST == 2 ? (u & 1) * kStage : 0);
-        TA::template put_moved<kThreads>(a, va[u], move_a, edge_a);
-        TB::template put_moved<kThreads>(a + TA::kBytes, vb[u], move_b, edge_b);
-        get(va[u], vb[u], blk + u + DEPTH);
+    const auto place = [&](char* a, const f32x4(&x)[PA], const f32x4(&y)[PB]) {
+      TA::template put_moved<kThreads>(a, x, move_a, edge_a);
+      TB::template put_moved<kThreads>(a + TA::kBytes, y, move_b, edge_b);
+    };
+    get(va, vb, first);
+    if constexpr (NST == 1) {
+      for (int blk = first; blk < whole; ++blk) {
+        place(lds, va, vb);
+        get(va, vb, blk + 1);
         __syncthreads();
-        if (blk + u < whole) compute(a);
-        if constexpr (NST == 1) __syncthreads();
+        compute(lds);
+        __syncthreads();
+      }
+    } else {
+      place(lds, va, vb);
+      get(va, vb, first + 1);
+      __syncthreads();
+      char *here = lds, *there = lds + kStage;
+      for (int blk = first; blk < whole; ++blk) {
+        // after the last block: it once more, into the stage that is not read again
+        compute(here);
+        place(there, va, vb);
+        get(va, vb, blk + 2);
+        __syncthreads();
+        char* t = here;
+        here = there, there = t;
       }
     }
   }
@@ -625,35 +643,40 @@ __global__ __launch_bounds__(64 * W) void k_gemm_rows(GemmArgs g) {
 }
 
 // ----------------------------------------------------------------------------- split k
-// Partials summed in split order, then the epilogue; one thread per 16 bytes of output.
+// Partials summed, then the epilogue: 32 pieces of 16 output bytes per workgroup, eight threads per piece that sum an
+// eighth of the splits each, in order, and are added in order.
+constexpr int kJoinParts = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void k_gemm_join(GemmArgs g) {
+__global__ __launch_bounds__(32 * kJoinParts) void k_gemm_join(GemmArgs g) {
   constexpr int V = 16 / sizeof(T);
+  __shared__ float sums[kJoinParts][32][V + 1];
   const int64_t per = (g.N + V - 1) / V, total = g.M * per;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
-    const int64_t m = t / per, n = (t - m * per) * V;
-    const int cnt = (int)min((int64_t)V, g.N - n);
-    float v[V];
+  const int i = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int64_t t = (int64_t)blockIdx.x * 32 + i;
+  const int64_t m = t / per, n = (t - m * per) * V;
+  const int cnt = t < total ? (int)min((int64_t)V, g.N - n) : 0;
+  float v[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = 0.0f;
-    const float* p = g.part + m * g.N + n;
-    for (int s = 0; s < g.nsplit; ++s, p += g.M * g.N) {
-      if (cnt == V) {
-        float u[4];
+  for (int e = 0; e < V; ++e) v[e] = 0.0f;
+  if (cnt > 0) {
+    const int s0 = g.nsplit * part / kJoinParts, s1 = g.nsplit * (part + 1) / kJoinParts;
+    const float* p = g.part + ((int64_t)s0 * g.M + m) * g.N + n;
+#pragma unroll 4
+    for (int s = s0; s < s1; ++s, p += g.M * g.N) {
+      float u[V];
+      load_some<V>(p, cnt, u);
 #pragma unroll
-        for (int q = 0; q < V / 4; ++q) {
-          load_vec(p + 4 * q, u);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * q + i] += u[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (i < cnt) v[i] += p[i];
-      }
+      for (int e = 0; e < V; ++e) v[e] += u[e];
     }
-    finish<T>(g, 0, m, n, v, cnt);
   }
+#pragma unroll
+  for (int e = 0; e < V; ++e) sums[part][i][e] = v[e];
+  __syncthreads();
+  if (part != 0 || cnt <= 0) return;
+  for (int q = 1; q < kJoinParts; ++q)
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += sums[q][i][e];
+  finish<T>(g, 0, m, n, v, cnt);
 }
 
 // ----------------------------------------------------------------------------- choice and launch
@@ -668,8 +691,10 @@ Plan plan_of(const Gemm& g) {
   const int bk = g.dtype == SGNN_F32 ? 32 : 64;
   Plan p{64, 64, 1};
   if (g.dtype != SGNN_F32 && tiles(256, 256) >= 192) p = {256, 256, 1};
+  else if (g.dtype == SGNN_F32 && tiles(256, 128) >= 256 && g.K >= 1024) p = {256, 128, 1};
   else if (tiles(128, 128) >= 128 || g.K >= 2048) p = {128, 128, 1};
   if (g.batch > 1) return p;
+  // what is resident at once: one workgroup per CU of the large tiles, two of the others
   const int64_t blocks = (g.K + bk - 1) / bk, wgs = p.bm == 256 ? 256 : 512;
   const int64_t want = wgs / std::max<int64_t>(1, tiles(p.bm, p.bn));
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, blocks / 8, 256}));
@@ -679,10 +704,12 @@ Plan plan_of(const Gemm& g) {
 template <typename T, bool AC, bool BC>
 void launch_tiles(const GemmArgs& g, const Plan& p, dim3 grid, bool direct, hipStream_t s) {
   if constexpr (std::is_same_v<T, float>) {
-    if (p.bm == 128)
-      hipLaunchKernelGGL((k_gemm32<AC, BC, 128, 128, 1, 1>), grid, dim3(256), 0, s, g);
+    if (p.bm == 256)
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 256, 128, 4, 2, 2>), grid, dim3(512), 0, s, g);
+    else if (p.bm == 128)
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 128, 128, 2, 2, 1>), grid, dim3(256), 0, s, g);
     else
-      hipLaunchKernelGGL((k_gemm32<AC, BC, 64, 64, 4, 2>), grid, dim3(256), 0, s, g);
+      hipLaunchKernelGGL((k_gemm32<AC, BC, 64, 64, 2, 2, 2>), grid, dim3(256), 0, s, g);
   } else {
     if (p.bm == 256)
       hipLaunchKernelGGL((k_gemm16<T, AC, BC, 256, 256, 2, 4, true, 2>), grid, dim3(512), 0, s, g);
@@ -746,7 +773,7 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
   }
   Plan p = plan_of(g);
   const bool direct = direct_ok(g.A, g.lda, g.batch_a, g.a_cols, g.M) && direct_ok(g.B, g.ldb, g.batch_b, g.b_cols, g.N);
-  if (!direct && p.bm == 256) p.bm = p.bn = 128;
+  if (!direct && p.bm == 256 && g.dtype != SGNN_F32) p.bm = p.bn = 128;
   const int64_t tm = (g.M + p.bm - 1) / p.bm, tn = (g.N + p.bn - 1) / p.bn;
   if (tm > INT32_MAX / tn || g.batch > 65535 || g.K > (int64_t)INT32_MAX * 32)
     return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k, or 65535 matrices");
@@ -764,7 +791,7 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
     else launch_tiles<T, true, true>(a, p, grid, direct, s);
     if (p.nsplit > 1) {
       const int64_t items = g.M * ((g.N + 16 / (int64_t)sizeof(T) - 1) / (16 / (int64_t)sizeof(T)));
-      hipLaunchKernelGGL(k_gemm_join<T>, dim3((unsigned)std::min<int64_t>((items + 255) / 256, 4096)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL(k_gemm_join<T>, dim3((unsigned)((items + 31) / 32)), dim3(32 * kJoinParts), 0, s, a);
     }
     return 0;
   });
