@@ -15,7 +15,7 @@ using namespace sgnn;
 
 constexpr float kScale = 1024.0f, kInvScale = 1.0f / 1024.0f;
 constexpr int kMaxGroup = 32;  // matrices of one shape per launch (their pointers are kernel arguments)
-constexpr int kNormParts = 64; // partial sums of squares per matrix
+constexpr int kNormParts = 256; // partial sums of squares per matrix, at most
 
 struct Group {
   int32_t rows, cols, count;
@@ -69,9 +69,14 @@ SGNN_DEV void put_planes(f16_t* p, int64_t plane, const float* v, float scale) {
 template <typename T, int P>
 __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, int nparts, float eps, f16_t* x,
                                                   int64_t plane, int64_t batch, int64_t ld, int64_t rows_padded) {
+  __shared__ double red[4];
   const int b = blockIdx.y;
-  double s = 0.0;
-  for (int i = 0; i < nparts; ++i) s += part[b * nparts + i];
+  double s = (int)threadIdx.x < nparts ? part[b * nparts + threadIdx.x] : 0.0;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane_id() == 0) red[wave_id()] = s;
+  __syncthreads();
+  s = red[0] + red[1] + red[2] + red[3];
   const float norm = (float)sqrt(s) + eps;
   const T* in = static_cast<const T*>(g.in[b]);
   const int64_t per = ld / 8, total = rows_padded * per;
@@ -257,6 +262,267 @@ void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
   else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM>), grid, dim3(256), 0, s, g);
 }
 
+// ----------------------------------------------------------------------------- small matrices
+// All steps of one matrix in one workgroup of eight waves, for sides that fit its LDS: X [m][n] and G / Q [m][m] as planes
+// with rows of n + 8 and m + 8 values (an odd number of 16-byte pieces, so that 16 rows' pieces fall on different banks),
+// m <= n in whole 32s, zeros in the padding.  A tall matrix is laid down transposed.  Each wave has up to NB blocks of
+// 32 x 32 of a product in registers; G and X are read along k from their rows, X as the second factor transposed
+// (ds_read_b64_tr_b16).  One launch instead of 2 + 3 per step, whose latency is all a small matrix costs.
+constexpr int kMaxSmall = 48, kSmallThreads = 512, kSmallWaves = kSmallThreads / 64, kMaxLds = 160 * 1024 - 256;
+struct SmallArgs {
+  sgnn_matrix mats[kMaxSmall];
+};
+
+inline int pad32(int v) { return (v + 31) & ~31; }
+inline size_t small_lds(int planes, int rows, int cols) {
+  const size_t m = pad32(std::min(rows, cols)), n = pad32(std::max(rows, cols));
+  return 2 * (size_t)planes * m * ((n + 8) + (m + 8));
+}
+inline int small_blocks(int rows, int cols) { return pad32(std::min(rows, cols)) / 32 * (pad32(std::max(rows, cols)) / 32); }
+inline bool small_ok(int planes, int rows, int cols) {
+  return std::min(rows, cols) <= 128 && std::max(rows, cols) <= 4096 && small_blocks(rows, cols) <= 6 * kSmallWaves &&
+         small_lds(planes, rows, cols) <= kMaxLds;
+}
+
+// acc = the 32 x 32 block (a0, b0) of A B^T, A's rows from LDS, B's from LDS (BT: its columns), over K.
+template <int P, bool BT>
+SGNN_DEV void small_block(f32x4 (&acc)[2][2], const char* A, int lda, int plane_a, const char* B, int ldb, int plane_b,
+                          int a0, int b0, int K) {
+  const int l = lane_id();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  for (int k0 = 0; k0 < K; k0 += 32) {
+    s16x8 fa[P][2], fb[P][2];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fa[p][i] = *reinterpret_cast<const s16x8*>(A + p * plane_a + 2 * ((a0 + 16 * i + (l & 15)) * lda + k0 + 8 * (l >> 4)));
+        if constexpr (!BT) {
+          fb[p][i] = *reinterpret_cast<const s16x8*>(B + p * plane_b + 2 * ((b0 + 16 * i + (l & 15)) * ldb + k0 + 8 * (l >> 4)));
+        } else {
+          const char* at = B + p * plane_b + 2 * ((k0 + 8 * (l >> 4) + ((l & 15) >> 2)) * ldb + b0 + 16 * i + 4 * (l & 3));
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(at));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(at + 8 * ldb));
+          fb[p][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+      }
+    if constexpr (P == 2) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
+  }
+}
+
+// The block's values times scale into planes of LDS.
+template <int P>
+SGNN_DEV void small_put(char* C, int ldc, int plane, const f32x4 (&acc)[2][2], int a0, int b0, float scale) {
+  typedef f16_t h4 __attribute__((ext_vector_type(4)));
+  const int l = lane_id();
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      h4 hi, lo;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v = acc[i][j][r] * scale;
+        const f16_t h = (f16_t)v;
+        hi[r] = h, lo[r] = (f16_t)(v - (float)h);
+      }
+      char* at = C + 2 * ((a0 + 16 * i + (l & 15)) * ldc + b0 + 16 * j + 4 * (l >> 4));
+      *reinterpret_cast<h4*>(at) = hi;
+      if constexpr (P == 2) *reinterpret_cast<h4*>(at + plane) = lo;
+    }
+}
+
+// A wave's q-th block, computed where it is used (hoisted out of the steps, all blocks' addresses at once would not fit
+// the registers).
+SGNN_DEV int block_of(int w, int q) {
+  int b = w + q * kSmallWaves;
+  asm volatile("" : "+s"(b));
+  return b;
+}
+
+template <typename T, int P, int NB>
+__global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int steps, float ca, float cb, float cc,
+                                                            float eps) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ double red[kSmallWaves];
+  constexpr int V = 16 / sizeof(T), NG = 2;
+  const sgnn_matrix& mat = args.mats[blockIdx.x];
+  const bool tall = mat.rows > mat.cols;
+  const int m = (min(mat.rows, mat.cols) + 31) & ~31, n = (max(mat.rows, mat.cols) + 31) & ~31;
+  const int ldx = n + 8, ldg = m + 8, plane_x = 2 * m * ldx, plane_g = 2 * m * ldg;
+  char *X = lds, *G = lds + P * plane_x;
+  const int w = wave_id(), l = lane_id();
+  const T* in = static_cast<const T*>(mat.in);
+
+  for (int t = threadIdx.x; t < P * plane_x / 16; t += kSmallThreads)
+    *reinterpret_cast<u32x4*>(X + 16 * t) = u32x4{0, 0, 0, 0};
+  __syncthreads();
+  // the elements' bits into their places (upper halves in the hi plane, lower ones in the lo plane) and the sum of
+  // squares, in 64 bits as in k_ns_norm
+  const int per = (mat.cols + V - 1) / V, pieces = mat.rows * per;
+  double s = 0.0;
+#pragma unroll 4
+  for (int t = threadIdx.x; t < pieces; t += kSmallThreads) {
+    const int r = t / per, c = (t - r * per) * V;
+    float v[V];
+    load_some<V>(in + (int64_t)r * mat.ld_in + c, mat.cols - c, v);
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      s += (double)v[e] * (double)v[e];
+      if (c + e >= mat.cols) continue;
+      char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
+      const uint32_t bits = __builtin_bit_cast(uint32_t, v[e]);
+      *reinterpret_cast<uint16_t*>(at) = bits >> 16;
+      if constexpr (P == 2) *reinterpret_cast<uint16_t*>(at + plane_x) = bits;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (l == 0) red[w] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int i = 0; i < kSmallWaves; ++i) s += red[i];
+  const float norm = (float)sqrt(s) + eps;
+  // the bits into the planes of the value / norm
+  for (int t = threadIdx.x; t < plane_x / 16; t += kSmallThreads) {
+    u32x4 hi = *reinterpret_cast<u32x4*>(X + 16 * t), lo = {0, 0, 0, 0};
+    if constexpr (P == 2) lo = *reinterpret_cast<u32x4*>(X + plane_x + 16 * t);
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t up = hi[e >> 1] >> (16 * (e & 1)) << 16, low = lo[e >> 1] >> (16 * (e & 1)) & 0xffffu;
+      const float x = __builtin_bit_cast(float, up | low);
+      v[e] = norm == 0.0f ? 0.0f : x / norm;
+    }
+    put_planes<P>(reinterpret_cast<f16_t*>(X + 16 * t), plane_x / 2, v, kScale);
+  }
+  __syncthreads();
+
+  if (steps == 0) {
+    T* out = static_cast<T*>(mat.out);
+    for (int t = threadIdx.x; t < mat.rows * mat.cols; t += kSmallThreads) {
+      const int r = t / mat.cols, c = t - r * mat.cols;
+      const f16_t* at = reinterpret_cast<const f16_t*>(X) + (tall ? c * ldx + r : r * ldx + c);
+      out[(int64_t)r * mat.ld_out + c] = from_float<T>((to_float(at[0]) + (P == 2 ? to_float(at[plane_x / 2]) : 0.0f)) * kInvScale);
+    }
+  }
+  const int mb = m / 32, gblocks = mb * mb, xblocks = mb * (n / 32);
+  constexpr float kDown = kInvScale * kInvScale;
+  for (int step = 0; step < steps; ++step) {
+    f32x4 g[NG][2][2], x[NB][2][2];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b < gblocks) {
+        small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b / mb * 32, b % mb * 32, n);
+        small_put<P>(G, ldg, plane_g, g[q], b / mb * 32, b % mb * 32, kInvScale);
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b < gblocks) {
+        f32x4 h[2][2];
+        const int a0 = b / mb * 32, b0 = b % mb * 32;
+        small_block<P, false>(h, G, ldg, plane_g, G, ldg, plane_g, a0, b0, m);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const bool diag = a0 + 16 * i + (l & 15) == b0 + 16 * j + 4 * (l >> 4) + r;
+              g[q][i][j][r] = cb * (g[q][i][j][r] * kDown) + cc * (h[i][j][r] * kDown) + (diag ? ca : 0.0f);
+            }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b / mb * 32, b % mb * 32, kScale);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NB; ++q) {
+      const int b = block_of(w, q);
+      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 32, b / mb * 32, m);
+    }
+    if (step + 1 < steps) {
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        const int b = block_of(w, q);
+        if (b < xblocks) small_put<P>(X, ldx, plane_x, x[q], b % mb * 32, b / mb * 32, kInvScale);
+      }
+      __syncthreads();
+    } else {
+      T* out = static_cast<T*>(mat.out);
+#pragma unroll
+      for (int q = 0; q < NB; ++q) {
+        const int b = block_of(w, q);
+        if (b >= xblocks) continue;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = b % mb * 32 + 16 * i + (l & 15), c = b / mb * 32 + 16 * j + 4 * (l >> 4);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float v = x[q][i][j][e] * kDown;
+              if (tall) {
+                if (r < mat.cols && c + e < mat.rows) out[(int64_t)(c + e) * mat.ld_out + r] = from_float<T>(v);
+              } else if (r < mat.rows && c + e < mat.cols) {
+                out[(int64_t)r * mat.ld_out + c + e] = from_float<T>(v);
+              }
+            }
+          }
+      }
+    }
+  }
+}
+
+template <typename T>
+int launch_small(const sgnn_matrix* mats, int count, int32_t steps, float a, float b, float c, float eps, hipStream_t s) {
+  constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
+  SmallArgs args;
+  size_t bytes = 0;
+  int blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    args.mats[i] = mats[i];
+    bytes = std::max(bytes, small_lds(P, mats[i].rows, mats[i].cols));
+    blocks = std::max(blocks, small_blocks(mats[i].rows, mats[i].cols));
+  }
+  const auto go = [&](auto kernel) {
+    // the attribute belongs to the device that is current
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds) !=
+        hipSuccess)
+      return check_launch("newton_schulz");
+    hipLaunchKernelGGL(kernel, dim3((unsigned)count), dim3(kSmallThreads), bytes, s, args, steps, a, b, c, eps);
+    return check_launch("newton_schulz");
+  };
+  return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2>) : go(k_ns_small<T, P, 6>);
+}
+
+// ----------------------------------------------------------------------------- large matrices
 size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 // A group's workspace: the norms' partial sums, X twice, G and Q, each two planes.
@@ -276,9 +542,16 @@ struct NsLayout {
   }
 };
 
-// The matrices from i on that share a launch: one shape, next to each other.
-int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i) {
+// The matrices from i on that share a launch: small ones of any shape, or large ones of one shape.  planes 1 (bf16) makes
+// more of them small than 2; the workspace is sized by 2.
+int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i, int planes) {
   int32_t n = 1;
+  if (small_ok(planes, mats[i].rows, mats[i].cols)) {
+    while (i + n < count && n < kMaxSmall && mats[i + n].rows > 0 && mats[i + n].cols > 0 &&
+           small_ok(planes, mats[i + n].rows, mats[i + n].cols))
+      ++n;
+    return n;
+  }
   while (i + n < count && n < kMaxGroup && mats[i + n].rows == mats[i].rows && mats[i + n].cols == mats[i].cols) ++n;
   return n;
 }
@@ -297,7 +570,7 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
   const auto blocks = [](int64_t items, int64_t most) {
     return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, most));
   };
-  const int parts = (int)blocks((int64_t)grp.rows * grp.cols / 8, kNormParts);
+  const int parts = (int)blocks((int64_t)grp.rows * grp.cols / 16, kNormParts);
   hipLaunchKernelGGL(k_ns_norm<T>, dim3(parts, grp.count), dim3(256), 0, s, grp, norms);
   constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
   hipLaunchKernelGGL((k_ns_begin<T, P>), dim3(blocks(batch_x / 8, 4096), grp.count), dim3(256), 0, s, grp, norms, parts,
@@ -342,8 +615,9 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
 extern "C" size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, int32_t count) {
   size_t most = 0;
   for (int32_t i = 0, n; mats && i < count; i += n) {
-    n = run_of(mats, count, i);
-    if (mats[i].rows > 0 && mats[i].cols > 0) most = std::max(most, NsLayout(mats[i].rows, mats[i].cols, n).total);
+    n = run_of(mats, count, i, 2);
+    if (mats[i].rows > 0 && mats[i].cols > 0 && !small_ok(2, mats[i].rows, mats[i].cols))
+      most = std::max(most, NsLayout(mats[i].rows, mats[i].cols, n).total);
   }
   return most;
 }
@@ -365,8 +639,17 @@ extern "C" int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_
   if (workspace_bytes < sgnn_newton_schulz_workspace_bytes(mats, count))
     return set_error(SGNN_ERR_INVALID, "newton_schulz: workspace smaller than sgnn_newton_schulz_workspace_bytes");
   for (int32_t i = 0, n; i < count; i += n) {
-    n = run_of(mats, count, i);
+    const int planes = dtype == SGNN_BF16 ? 1 : 2;
+    n = run_of(mats, count, i, planes);
     if (mats[i].rows == 0 || mats[i].cols == 0) continue;
+    if (small_ok(planes, mats[i].rows, mats[i].cols)) {
+      const int st = with_type(dtype, [&](auto* t) {
+        return launch_small<std::remove_pointer_t<decltype(t)>>(mats + i, n, steps, a, b, c, eps,
+                                                                static_cast<hipStream_t>(stream));
+      });
+      if (st != SGNN_OK) return st;
+      continue;
+    }
     Group grp;
     grp.rows = mats[i].rows, grp.cols = mats[i].cols, grp.count = n;
     for (int32_t k = 0; k < n; ++k) {
