@@ -106,13 +106,13 @@ struct NsGemm {
 
 // BT x BT outputs by four waves.  P planes per operand (1: hi alone).  SYM: the product is symmetric; only the tiles
 // on and above the diagonal are formed and each is written to both sides.
-template <int P, bool AC, bool BC, int BT, bool SYM>
+template <int P, bool AC, bool BC, int BT, bool SYM, int NST>
 __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
   constexpr int BK = 64 / P, kThreads = 256, TT = BT / 2 / 16;
   using TA = Tile16<BT, BK, AC>;
   using TB = Tile16<BT, BK, BC>;
   constexpr int kStage = 2 * P * TA::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[2 * kStage];
+  __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
   const int w = wave_id(), wm = w >> 1, wn = w & 1, l = lane_id();
   int tm, tn;
   if constexpr (SYM) {  // row tm of the triangle holds tiles_n - tm tiles
@@ -149,13 +149,16 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
     }
   };
   const int blocks = g.K / BK;
-  char* here = lds;
-  char* there = lds + kStage;
-  stage(here, 0);
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (i < blocks) stage(lds + i * kStage, i);
+  int turn = 0;
   for (int blk = 0; blk < blocks; ++blk) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    wait_stages<2 * P * PER, NST - 2>(blocks - 1 - blk);
     __syncthreads();
-    if (blk + 1 < blocks) stage(there, blk + 1);
+    if (blk + NST - 1 < blocks) stage(lds + (turn == 0 ? NST - 1 : turn - 1) * kStage, blk + NST - 1);
+    const char* here = lds + turn * kStage;
+    turn = turn == NST - 1 ? 0 : turn + 1;
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       s16x8 fa[P][TT], fb[P][TT];
@@ -181,8 +184,6 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
 #pragma unroll
         for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
     }
-    char* t = here;
-    here = there, there = t;
   }
   __syncthreads();
   // through LDS by 16 rows of m (as in gemm.hip), so that every load and store is 16 bytes of a row
@@ -258,15 +259,15 @@ template <int P, bool AC, bool BC, bool SYM>
 void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
   const int tiles = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
   const dim3 grid((unsigned)tiles, 1, (unsigned)count);
-  if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM>), grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM>), grid, dim3(256), 0, s, g);
+  if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 2>), grid, dim3(256), 0, s, g);
+  else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 4>), grid, dim3(256), 0, s, g);
 }
 
 // ----------------------------------------------------------------------------- small matrices
 // All steps of one matrix in one workgroup of eight waves, for sides that fit its LDS: X [m][n] and G / Q [m][m] as planes
 // with rows of n + 8 and m + 8 values (an odd number of 16-byte pieces, so that 16 rows' pieces fall on different banks),
-// m <= n in whole 32s, zeros in the padding.  A tall matrix is laid down transposed.  Each wave has up to NB blocks of
-// 32 x 32 of a product in registers; G and X are read along k from their rows, X as the second factor transposed
+// m <= n in whole 32s, zeros in the padding.  A tall matrix is laid down transposed.  Each wave has up to NB times
+// 32 x 32 of a product in registers, in blocks of 16 BI x 32; G and X are read along k from their rows, X as the second factor transposed
 // (ds_read_b64_tr_b16).  One launch instead of 2 + 3 per step, whose latency is all a small matrix costs.
 constexpr int kMaxSmall = 48, kSmallThreads = 512, kSmallWaves = kSmallThreads / 64, kMaxLds = 160 * 1024 - 256;
 struct SmallArgs {
@@ -279,27 +280,31 @@ inline size_t small_lds(int planes, int rows, int cols) {
   return 2 * (size_t)planes * m * ((n + 8) + (m + 8));
 }
 inline int small_blocks(int rows, int cols) { return pad32(std::min(rows, cols)) / 32 * (pad32(std::max(rows, cols)) / 32); }
+// A short side of 128 fills the waves with blocks of 64 x 32, which read a quarter less of LDS than those of 32 x 32.
+inline bool full_side(int rows, int cols) { return pad32(std::min(rows, cols)) == 128; }
 inline bool small_ok(int planes, int rows, int cols) {
   return std::min(rows, cols) <= 128 && std::max(rows, cols) <= 4096 && small_blocks(rows, cols) <= 6 * kSmallWaves &&
          small_lds(planes, rows, cols) <= kMaxLds;
 }
 
-// acc = the 32 x 32 block (a0, b0) of A B^T, A's rows from LDS, B's from LDS (BT: its columns), over K.
-template <int P, bool BT>
-SGNN_DEV void small_block(f32x4 (&acc)[2][2], const char* A, int lda, int plane_a, const char* B, int ldb, int plane_b,
+// acc = the 16 BI x 32 block (a0, b0) of A B^T, A's rows from LDS, B's from LDS (BT: its columns), over K.
+template <int P, bool BT, int BI>
+SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane_a, const char* B, int ldb, int plane_b,
                           int a0, int b0, int K) {
   const int l = lane_id();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < BI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
   for (int k0 = 0; k0 < K; k0 += 32) {
-    s16x8 fa[P][2], fb[P][2];
+    s16x8 fa[P][BI], fb[P][2];
 #pragma unroll
-    for (int p = 0; p < P; ++p)
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int i = 0; i < BI; ++i)
+        fa[p][i] = *reinterpret_cast<const s16x8*>(A + p * plane_a + 2 * ((a0 + 16 * i + (l & 15)) * lda + k0 + 8 * (l >> 4)));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        fa[p][i] = *reinterpret_cast<const s16x8*>(A + p * plane_a + 2 * ((a0 + 16 * i + (l & 15)) * lda + k0 + 8 * (l >> 4)));
         if constexpr (!BT) {
           fb[p][i] = *reinterpret_cast<const s16x8*>(B + p * plane_b + 2 * ((b0 + 16 * i + (l & 15)) * ldb + k0 + 8 * (l >> 4)));
         } else {
@@ -309,30 +314,31 @@ SGNN_DEV void small_block(f32x4 (&acc)[2][2], const char* A, int lda, int plane_
           fb[p][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
       }
+    }
     if constexpr (P == 2) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < BI; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+      for (int i = 0; i < BI; ++i)
 #pragma unroll
         for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
     }
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < BI; ++i)
 #pragma unroll
       for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
   }
 }
 
 // The block's values times scale into planes of LDS.
-template <int P>
-SGNN_DEV void small_put(char* C, int ldc, int plane, const f32x4 (&acc)[2][2], int a0, int b0, float scale) {
+template <int P, int BI>
+SGNN_DEV void small_put(char* C, int ldc, int plane, const f32x4 (&acc)[BI][2], int a0, int b0, float scale) {
   typedef f16_t h4 __attribute__((ext_vector_type(4)));
   const int l = lane_id();
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < BI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       h4 hi, lo;
@@ -356,12 +362,72 @@ SGNN_DEV int block_of(int w, int q) {
   return b;
 }
 
-template <typename T, int P, int NB>
+constexpr float kDown = kInvScale * kInvScale;  // of a product of two scaled planes
+
+// The planes of Q = ca I + cb G + cc G^2 into LDS at G, from this wave's blocks g of kScale^2 G.
+template <int P, int NG, int BI>
+SGNN_DEV void small_poly(f32x4 (&g)[NG][BI][2], char* G, int ldg, int plane_g, int m, float ca, float cb, float cc) {
+  const int l = lane_id(), w = wave_id(), mb = m / (16 * BI), gblocks = mb * (m / 32);
+#pragma unroll
+  for (int q = 0; q < NG; ++q) {
+    const int b = block_of(w, q);
+    if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NG; ++q) {
+    const int b = block_of(w, q);
+    if (b < gblocks) {
+      f32x4 h[BI][2];
+      const int a0 = b % mb * 16 * BI, b0 = b / mb * 32;
+      small_block<P, false>(h, G, ldg, plane_g, G, ldg, plane_g, a0, b0, m);
+#pragma unroll
+      for (int i = 0; i < BI; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const bool diag = a0 + 16 * i + (l & 15) == b0 + 16 * j + 4 * (l >> 4) + r;
+            g[q][i][j][r] = cb * (g[q][i][j][r] * kDown) + cc * (h[i][j][r] * kDown) + (diag ? ca : 0.0f);
+          }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < NG; ++q) {
+    const int b = block_of(w, q);
+    if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kScale);
+  }
+  __syncthreads();
+}
+
+// A block of kScale^2 X, at (r0, c0) of the matrix as it lies in LDS, into the caller's matrix.
+template <typename T, int BI>
+SGNN_DEV void small_out(const f32x4 (&x)[BI][2], T* out, int64_t ld, int rows, int cols, bool tall, int r0, int c0) {
+  const int l = lane_id();
+#pragma unroll
+  for (int i = 0; i < BI; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const int r = r0 + 16 * i + (l & 15), c = c0 + 16 * j + 4 * (l >> 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v = x[i][j][e] * kDown;
+        if (tall) {
+          if (r < cols && c + e < rows) out[(int64_t)(c + e) * ld + r] = from_float<T>(v);
+        } else if (r < rows && c + e < cols) {
+          out[(int64_t)r * ld + c + e] = from_float<T>(v);
+        }
+      }
+    }
+}
+
+template <typename T, int P, int NB, int BI>
 __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int steps, float ca, float cb, float cc,
                                                             float eps) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ double red[kSmallWaves];
-  constexpr int V = 16 / sizeof(T), NG = 2;
+  constexpr int V = 16 / sizeof(T);
   const sgnn_matrix& mat = args.mats[blockIdx.x];
   const bool tall = mat.rows > mat.cols;
   const int m = (min(mat.rows, mat.cols) + 31) & ~31, n = (max(mat.rows, mat.cols) + 31) & ~31;
@@ -423,80 +489,31 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
       out[(int64_t)r * mat.ld_out + c] = from_float<T>((to_float(at[0]) + (P == 2 ? to_float(at[plane_x / 2]) : 0.0f)) * kInvScale);
     }
   }
-  const int mb = m / 32, gblocks = mb * mb, xblocks = mb * (n / 32);
-  constexpr float kDown = kInvScale * kInvScale;
+  constexpr int NG = 4 / BI, NX = 2 * NB / BI;
+  const int mb = m / (16 * BI), gblocks = mb * (m / 32), xblocks = mb * (n / 32);
   for (int step = 0; step < steps; ++step) {
-    f32x4 g[NG][2][2], x[NB][2][2];
+    f32x4 g[NG][BI][2], x[NX][BI][2];
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const int b = block_of(w, q);
-      if (b < gblocks) {
-        small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b / mb * 32, b % mb * 32, n);
-        small_put<P>(G, ldg, plane_g, g[q], b / mb * 32, b % mb * 32, kInvScale);
-      }
+      if (b < gblocks) small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, n);
+    }
+    small_poly<P>(g, G, ldg, plane_g, m, ca, cb, cc);
+#pragma unroll
+    for (int q = 0; q < NX; ++q) {
+      const int b = block_of(w, q);
+      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < NG; ++q) {
+    for (int q = 0; q < NX; ++q) {
       const int b = block_of(w, q);
-      if (b < gblocks) {
-        f32x4 h[2][2];
-        const int a0 = b / mb * 32, b0 = b % mb * 32;
-        small_block<P, false>(h, G, ldg, plane_g, G, ldg, plane_g, a0, b0, m);
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const bool diag = a0 + 16 * i + (l & 15) == b0 + 16 * j + 4 * (l >> 4) + r;
-              g[q][i][j][r] = cb * (g[q][i][j][r] * kDown) + cc * (h[i][j][r] * kDown) + (diag ? ca : 0.0f);
-            }
-      }
+      if (b >= xblocks) continue;
+      const int r0 = b % mb * 16 * BI, c0 = b / mb * 32;
+      if (step + 1 < steps) small_put<P>(X, ldx, plane_x, x[q], r0, c0, kInvScale);
+      else small_out<T>(x[q], static_cast<T*>(mat.out), mat.ld_out, mat.rows, mat.cols, tall, r0, c0);
     }
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < NG; ++q) {
-      const int b = block_of(w, q);
-      if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b / mb * 32, b % mb * 32, kScale);
-    }
-    __syncthreads();
-#pragma unroll
-    for (int q = 0; q < NB; ++q) {
-      const int b = block_of(w, q);
-      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 32, b / mb * 32, m);
-    }
-    if (step + 1 < steps) {
-      __syncthreads();
-#pragma unroll
-      for (int q = 0; q < NB; ++q) {
-        const int b = block_of(w, q);
-        if (b < xblocks) small_put<P>(X, ldx, plane_x, x[q], b % mb * 32, b / mb * 32, kInvScale);
-      }
-      __syncthreads();
-    } else {
-      T* out = static_cast<T*>(mat.out);
-#pragma unroll
-      for (int q = 0; q < NB; ++q) {
-        const int b = block_of(w, q);
-        if (b >= xblocks) continue;
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = b % mb * 32 + 16 * i + (l & 15), c = b / mb * 32 + 16 * j + 4 * (l >> 4);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float v = x[q][i][j][e] * kDown;
-              if (tall) {
-                if (r < mat.cols && c + e < mat.rows) out[(int64_t)(c + e) * mat.ld_out + r] = from_float<T>(v);
-              } else if (r < mat.rows && c + e < mat.cols) {
-                out[(int64_t)r * mat.ld_out + c + e] = from_float<T>(v);
-              }
-            }
-          }
-      }
-    }
   }
 }
 
@@ -519,7 +536,146 @@ int launch_small(const sgnn_matrix* mats, int count, int32_t steps, float a, flo
     hipLaunchKernelGGL(kernel, dim3((unsigned)count), dim3(kSmallThreads), bytes, s, args, steps, a, b, c, eps);
     return check_launch("newton_schulz");
   };
-  return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2>) : go(k_ns_small<T, P, 6>);
+  if (full_side(mats[0].rows, mats[0].cols))
+    return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2, 4>) : go(k_ns_small<T, P, 6, 4>);
+  return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2, 2>) : go(k_ns_small<T, P, 6, 2>);
+}
+
+// ----------------------------------------------------------------------------- short and long matrices
+// A matrix whose short side fits as above but whose long one does not: a workgroup per kChunk of its long side.  G is the
+// sum of the chunks' X_c X_c^T, so one launch per step does: add the chunks' shares of G (in order, every workgroup for
+// itself), form Q, X_c <- Q X_c, and its share of the next G -- 2 + steps launches for 2 + 3 steps.
+//   shares [matrix][chunk][32 x 32 block of G][4][lane] as the accumulators hold them; x: planes [matrix][m][ld]
+constexpr int kChunk = 128, kMaxChunks = 16;
+inline bool chunk_ok(int rows, int cols) {
+  return std::min(rows, cols) <= 128 && std::max(rows, cols) <= kChunk * kMaxChunks;
+}
+inline int chunks_of(int rows, int cols) { return (std::max(rows, cols) + kChunk - 1) / kChunk; }
+inline size_t chunk_lds(int planes, int m) { return 2 * (size_t)planes * m * ((kChunk + 8) + (m + 8)); }
+
+struct ChunkArgs {
+  const double* norms;
+  f16_t* x;
+  const float* from;  // the shares of this step's G (null: the first launch, which has the norms instead)
+  float* to;          // of the next one (null: the last step)
+  int64_t plane;
+  int32_t nparts, m, ld;
+  float ca, cb, cc, eps;
+};
+
+template <typename T, int P, int BI>
+__global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs a) {
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ double red[kSmallWaves];
+  constexpr int V = 16 / sizeof(T);
+  const int l = lane_id(), w = wave_id(), mat = blockIdx.y, c0 = blockIdx.x * kChunk;
+  constexpr int NG = 4 / BI;
+  const int m = a.m, mb = m / (16 * BI), gblocks = mb * (m / 32), xblocks = mb * (kChunk / 32);
+  const int ldx = kChunk + 8, ldg = m + 8, plane_x = 2 * m * ldx, plane_g = 2 * m * ldg;
+  char *X = lds, *G = lds + P * plane_x;
+  const bool tall = grp.rows > grp.cols;
+  f16_t* home = a.x + (int64_t)mat * m * a.ld + c0;
+  f32x4 g[NG][BI][2];
+
+  if (a.from) {
+    // X's loads go out before those of the shares
+    constexpr int kPer = 128 * (kChunk / 8) / kSmallThreads;
+    u32x4 px[P][kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int t = i * kSmallThreads + threadIdx.x, r = min(t / (kChunk / 8), m - 1), c = t % (kChunk / 8) * 8;
+#pragma unroll
+      for (int p = 0; p < P; ++p) px[p][i] = *reinterpret_cast<const u32x4*>(home + p * a.plane + (int64_t)r * a.ld + c);
+    }
+    const f32x4* from = reinterpret_cast<const f32x4*>(a.from) + (int64_t)mat * gridDim.x * gblocks * 128 * BI + l;
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b >= gblocks) continue;
+#pragma unroll
+      for (int i = 0; i < 2 * BI; ++i) g[q][i >> 1][i & 1] = f32x4{0, 0, 0, 0};
+#pragma unroll 2
+      for (int c = 0; c < (int)gridDim.x; ++c)
+#pragma unroll
+        for (int i = 0; i < 2 * BI; ++i) g[q][i >> 1][i & 1] += from[((int64_t)c * gblocks + b) * 128 * BI + 64 * i];
+    }
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int t = i * kSmallThreads + threadIdx.x, r = t / (kChunk / 8), c = t % (kChunk / 8) * 8;
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+        if (r < m) *reinterpret_cast<u32x4*>(X + p * plane_x + 2 * (r * ldx + c)) = px[p][i];
+    }
+    __syncthreads();
+    small_poly<P>(g, G, ldg, plane_g, m, a.ca, a.cb, a.cc);
+    f32x4 x[NG][BI][2];
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < NG; ++q) {
+      const int b = block_of(w, q);
+      if (b >= xblocks) continue;
+      if (a.to)
+        small_put<P>(X, ldx, plane_x, x[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
+      else
+        small_out<T>(x[q], static_cast<T*>(grp.out[mat]), grp.ld_out[mat], grp.rows, grp.cols, tall, b % mb * 16 * BI,
+                     c0 + b / mb * 32);
+    }
+    if (!a.to) return;
+  } else {
+    double s = (int)threadIdx.x < a.nparts ? a.norms[mat * a.nparts + threadIdx.x] : 0.0;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o, 64);
+    if (l == 0) red[w] = s;
+    for (int t = threadIdx.x; t < P * plane_x / 16; t += kSmallThreads)
+      *reinterpret_cast<u32x4*>(X + 16 * t) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+    s = 0.0;
+#pragma unroll
+    for (int i = 0; i < kSmallWaves; ++i) s += red[i];
+    const float norm = (float)sqrt(s) + a.eps;
+    // this chunk of the caller's matrix: rows r0 .. of it where it is tall, columns where it is wide
+    const int r0 = tall ? c0 : 0, rows = tall ? min(kChunk, grp.rows - c0) : grp.rows;
+    const int k0 = tall ? 0 : c0, cols = tall ? grp.cols : min(kChunk, grp.cols - c0);
+    const T* in = static_cast<const T*>(grp.in[mat]) + (int64_t)r0 * grp.ld_in[mat] + k0;
+    const int per = (cols + V - 1) / V;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < rows * per; t += kSmallThreads) {
+      const int r = t / per, c = (t - r * per) * V;
+      float v[V];
+      load_some<V>(in + (int64_t)r * grp.ld_in[mat] + c, cols - c, v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        if (c + e >= cols) continue;
+        char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
+        const float y = (norm == 0.0f ? 0.0f : v[e] / norm) * kScale;
+        const f16_t h = (f16_t)y;
+        *reinterpret_cast<f16_t*>(at) = h;
+        if constexpr (P == 2) *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);
+      }
+    }
+  }
+  __syncthreads();
+  for (int t = threadIdx.x; t < m * (kChunk / 8); t += kSmallThreads) {
+    const int r = t / (kChunk / 8), c = t % (kChunk / 8) * 8;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      *reinterpret_cast<u32x4*>(home + p * a.plane + (int64_t)r * a.ld + c) =
+          *reinterpret_cast<const u32x4*>(X + p * plane_x + 2 * (r * ldx + c));
+  }
+  f32x4* to = reinterpret_cast<f32x4*>(a.to) + ((int64_t)mat * gridDim.x + blockIdx.x) * gblocks * 128 * BI + l;
+#pragma unroll
+  for (int q = 0; q < NG; ++q) {
+    const int b = block_of(w, q);
+    if (b >= gblocks) continue;
+    small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, kChunk);
+#pragma unroll
+    for (int i = 0; i < 2 * BI; ++i) to[(int64_t)b * 128 * BI + 64 * i] = g[q][i >> 1][i & 1];
+  }
 }
 
 // ----------------------------------------------------------------------------- large matrices
@@ -542,13 +698,59 @@ struct NsLayout {
   }
 };
 
+// The same for a group by chunks: the norms' partial sums, X, G's shares twice.
+struct ChunkLayout {
+  int chunks, m, ld;
+  size_t norms, x, share, total;
+  ChunkLayout(int32_t r, int32_t c, int count) {
+    chunks = chunks_of(r, c), m = pad32(std::min(r, c)), ld = chunks * kChunk;
+    norms = pad256(sizeof(double) * kNormParts * count);
+    x = pad256(2 * sizeof(f16_t) * (size_t)m * ld * count);
+    share = pad256(sizeof(float) * (size_t)m * m * chunks * count);
+    total = norms + x + 2 * share;
+  }
+};
+size_t group_bytes(int32_t r, int32_t c, int count) {  // steps 0 of a matrix by chunks takes the large path's layout
+  const size_t large = NsLayout(r, c, count).total;
+  return chunk_ok(r, c) ? std::max(large, ChunkLayout(r, c, count).total) : large;
+}
+
+unsigned blocks_for(int64_t items, int64_t most) {
+  return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, most));
+}
+
+template <typename T>
+int by_chunks(const Group& grp, int32_t steps, float a, float b, float c, float eps, char* ws, hipStream_t s) {
+  constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
+  const ChunkLayout at(grp.rows, grp.cols, grp.count);
+  double* norms = reinterpret_cast<double*>(ws);
+  float *from = reinterpret_cast<float*>(ws + at.norms + at.x), *to = reinterpret_cast<float*>(ws + at.norms + at.x + at.share);
+  const size_t lds = chunk_lds(P, at.m);
+  ChunkArgs g{norms, reinterpret_cast<f16_t*>(ws + at.norms), nullptr, to, (int64_t)at.m * at.ld * grp.count,
+              (int32_t)blocks_for((int64_t)grp.rows * grp.cols / 16, kNormParts), at.m, at.ld, a, b, c, eps};
+  hipLaunchKernelGGL(k_ns_norm<T>, dim3((unsigned)g.nparts, grp.count), dim3(256), 0, s, grp, norms);
+  const auto go = [&](auto kernel) {
+    if (hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, kMaxLds) !=
+        hipSuccess)
+      return check_launch("newton_schulz");
+    for (int32_t k = 0; k <= steps; ++k) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)at.chunks, (unsigned)grp.count), dim3(kSmallThreads), lds, s, grp, g);
+      std::swap(from, to);
+      g.from = from, g.to = k + 1 < steps ? to : nullptr;
+    }
+    return check_launch("newton_schulz");
+  };
+  return full_side(grp.rows, grp.cols) ? go(k_ns_chunk<T, P, 4>) : go(k_ns_chunk<T, P, 2>);
+}
+
 // The matrices from i on that share a launch: small ones of any shape, or large ones of one shape.  planes 1 (bf16) makes
 // more of them small than 2; the workspace is sized by 2.
 int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i, int planes) {
   int32_t n = 1;
   if (small_ok(planes, mats[i].rows, mats[i].cols)) {
     while (i + n < count && n < kMaxSmall && mats[i + n].rows > 0 && mats[i + n].cols > 0 &&
-           small_ok(planes, mats[i + n].rows, mats[i + n].cols))
+           small_ok(planes, mats[i + n].rows, mats[i + n].cols) &&
+           full_side(mats[i + n].rows, mats[i + n].cols) == full_side(mats[i].rows, mats[i].cols))
       ++n;
     return n;
   }
@@ -567,13 +769,10 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
   f16_t* poly = reinterpret_cast<f16_t*>(ws + at.norms + 2 * at.x + at.g);
   const int64_t batch_x = at.rows * at.cols, plane_x = batch_x * grp.count;
   const int64_t batch_g = at.side * at.side, plane_g = batch_g * grp.count;
-  const auto blocks = [](int64_t items, int64_t most) {
-    return (unsigned)std::max<int64_t>(1, std::min<int64_t>((items + 255) / 256, most));
-  };
-  const int parts = (int)blocks((int64_t)grp.rows * grp.cols / 16, kNormParts);
+  const int parts = (int)blocks_for((int64_t)grp.rows * grp.cols / 16, kNormParts);
   hipLaunchKernelGGL(k_ns_norm<T>, dim3(parts, grp.count), dim3(256), 0, s, grp, norms);
   constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
-  hipLaunchKernelGGL((k_ns_begin<T, P>), dim3(blocks(batch_x / 8, 4096), grp.count), dim3(256), 0, s, grp, norms, parts,
+  hipLaunchKernelGGL((k_ns_begin<T, P>), dim3(blocks_for(batch_x / 8, 4096), grp.count), dim3(256), 0, s, grp, norms, parts,
                      eps, steps > 0 ? x : nullptr, plane_x, batch_x, at.cols, at.rows);
   for (int32_t k = 0; k < steps; ++k) {
     NsGemm g{};
@@ -617,7 +816,7 @@ extern "C" size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, in
   for (int32_t i = 0, n; mats && i < count; i += n) {
     n = run_of(mats, count, i, 2);
     if (mats[i].rows > 0 && mats[i].cols > 0 && !small_ok(2, mats[i].rows, mats[i].cols))
-      most = std::max(most, NsLayout(mats[i].rows, mats[i].cols, n).total);
+      most = std::max(most, group_bytes(mats[i].rows, mats[i].cols, n));
   }
   return most;
 }
@@ -656,12 +855,14 @@ extern "C" int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_
       grp.in[k] = mats[i + k].in, grp.out[k] = mats[i + k].out;
       grp.ld_in[k] = mats[i + k].ld_in, grp.ld_out[k] = mats[i + k].ld_out;
     }
-    with_type(dtype, [&](auto* t) {
-      orthogonalise<std::remove_pointer_t<decltype(t)>>(grp, steps, a, b, c, eps, static_cast<char*>(workspace),
-                                                        static_cast<hipStream_t>(stream));
-      return 0;
+    const int st = with_type(dtype, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      char* ws = static_cast<char*>(workspace);
+      hipStream_t s = static_cast<hipStream_t>(stream);
+      if (steps > 0 && chunk_ok(grp.rows, grp.cols)) return by_chunks<T>(grp, steps, a, b, c, eps, ws, s);
+      orthogonalise<T>(grp, steps, a, b, c, eps, ws, s);
+      return check_launch("newton_schulz");
     });
-    const int st = check_launch("newton_schulz");
     if (st != SGNN_OK) return st;
   }
   return SGNN_OK;
