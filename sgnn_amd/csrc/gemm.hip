@@ -33,26 +33,29 @@ SGNN_DEV void act_row(const GemmArgs& g, int64_t at, int cnt, float (&v)[V]) {
   if (g.slope) {
     float s[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) act_both<ACT, true>(v[i], v[i], s[i]);
+    for (int i = 0; i < V; ++i) act_both<ACT, true, sizeof(T) == 2>(v[i], v[i], s[i]);
     store_slopes<T>(g.slope, at, cnt, s);
   } else {
     float unused;
 #pragma unroll
-    for (int i = 0; i < V; ++i) act_both<ACT, false>(v[i], v[i], unused);
+    for (int i = 0; i < V; ++i) act_both<ACT, false, sizeof(T) == 2>(v[i], v[i], unused);
   }
+}
+
+// The bias of columns n .., zeros where there is none; cnt of them exist.
+template <typename T, int V>
+SGNN_DEV void load_bias(const GemmArgs& g, int64_t n, int cnt, float (&t)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) t[i] = 0.0f;
+  if (g.bias && cnt > 0) load_some<V>(static_cast<const T*>(g.bias) + n, cnt, t);
 }
 
 // V = 16 bytes' consecutive outputs (m, n ..) of one lane; cnt of them exist.
 template <typename T, int V>
-SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float (&v)[V], int cnt) {
+SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float (&v)[V], const float (&bias)[V], int cnt) {
   float t[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] *= g.alpha;
-  if (g.bias) {
-    load_some<V>(static_cast<const T*>(g.bias) + n, cnt, t);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += t[i];
-  }
+  for (int i = 0; i < V; ++i) v[i] = g.alpha * v[i] + bias[i];
   switch (g.act) {  // the same for every lane
     case SGNN_ACT_RELU: act_row<SGNN_ACT_RELU, T>(g, m * g.N + n, cnt, v); break;
     case SGNN_ACT_GELU: act_row<SGNN_ACT_GELU, T>(g, m * g.N + n, cnt, v); break;
@@ -78,6 +81,13 @@ SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][T
   const int l = lane_id();
   constexpr int kPieces = 4 * TN;  // 16-byte pieces per row of 16 TN floats
   constexpr int kMask = kPieces - 1 < 15 ? kPieces - 1 : 15;
+  // a lane's columns are the same in every row it takes, so their bias is loaded once
+  constexpr int V = 16 / sizeof(T), kPer = V / 4, kAcross = kPieces / kPer;
+  static_assert(64 % kAcross == 0, "whole rows of pieces per wave");
+  const int64_t n_mine = n0 + 4 * kPer * (l % kAcross);
+  const int cnt = (int)min((int64_t)V, g.N - n_mine);
+  float bias[V];
+  if (!g.part) load_bias<T>(g, n_mine, cnt, bias);
 #pragma unroll
   for (int round = 0; round < TM / RP; ++round) {
 #pragma unroll
@@ -100,10 +110,9 @@ SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][T
           store_some<4>(g.part + ((int64_t)split * g.M + m) * g.N + n, (int)min((int64_t)4, g.N - n), v);
       }
     } else {
-      constexpr int V = 16 / sizeof(T), kPer = V / 4;
-#pragma unroll 1
-      for (int t = l; t < 16 * RP * kPieces / kPer; t += 64) {
-        const int r = t / (kPieces / kPer), p = (t % (kPieces / kPer)) * kPer;
+#pragma unroll 2
+      for (int r = l / kAcross; r < 16 * RP; r += 64 / kAcross) {
+        const int p = l % kAcross * kPer;
         float v[V];
 #pragma unroll
         for (int q = 0; q < kPer; ++q) {
@@ -111,8 +120,7 @@ SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][T
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
         }
-        const int64_t m = mr + r, n = n0 + 4 * p;
-        if (m < g.M && n < g.N) finish<T>(g, b, m, n, v, (int)min((int64_t)V, g.N - n));
+        if (mr + r < g.M && cnt > 0) finish<T>(g, b, mr + r, n_mine, v, bias, cnt);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -187,6 +195,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<T>(fb[j], fa[i], acc[i][j]);
     }
+    if constexpr (TM >= 4) order_products<TM, TN, ACOLS ? 2 : 1, BCOLS ? 2 : 1>();
   };
   constexpr int PA = BM * BK / 8 / kThreads, PB = BN * BK / 8 / kThreads;
   const auto fetch = [&](u32x4(&va)[PA], u32x4(&vb)[PB], int blk) {
@@ -638,7 +647,10 @@ __global__ __launch_bounds__(64 * W) void k_gemm_rows(GemmArgs g) {
     for (int q = 0; q < W; ++q)
 #pragma unroll
       for (int e = 0; e < V; ++e) v[e] += part[q][m][c + e];
-    finish<T>(g, 0, m, n0 + c, v, (int)min((int64_t)V, g.N - n0 - c));
+    const int cnt = (int)min((int64_t)V, g.N - n0 - c);
+    float bias[V];
+    load_bias<T>(g, n0 + c, cnt, bias);
+    finish<T>(g, 0, m, n0 + c, v, bias, cnt);
   }
 }
 
@@ -676,7 +688,9 @@ __global__ __launch_bounds__(32 * kJoinParts) void k_gemm_join(GemmArgs g) {
   for (int q = 1; q < kJoinParts; ++q)
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] += sums[q][i][e];
-  finish<T>(g, 0, m, n, v, cnt);
+  float bias[V];
+  load_bias<T>(g, n, cnt, bias);
+  finish<T>(g, 0, m, n, v, bias, cnt);
 }
 
 // ----------------------------------------------------------------------------- choice and launch

@@ -39,10 +39,10 @@ struct Tile16 {
   // this lane's chunks' bytes from the tile's first element, the same for every block of k.  Lines and chunks past
   // the last row read another one's data: their outputs are not stored.
   template <int THREADS, int KPER>
-  static SGNN_DEV void offsets(uint32_t (&o)[KPER], int64_t ld, int64_t rows, int64_t r0) {
+  static SGNN_DEV void offsets(uint32_t (&o)[KPER], int64_t ld, int64_t rows, int64_t r0, int tid = threadIdx.x) {
 #pragma unroll
     for (int i = 0; i < KPER; ++i) {
-      const int q = i * THREADS + threadIdx.x;
+      const int q = i * THREADS + tid;
       const int line = q / kChunks, c = (q % kChunks) ^ swizzle(line);
       const int left = (int)min(rows - r0, (int64_t)R);
       o[i] = 2 * (COLS ? (uint32_t)line * (uint32_t)ld + min(8 * c, left - 8)
@@ -53,14 +53,14 @@ struct Tile16 {
   // instructions, as the compiler makes every later LDS read wait for the builtin's.  The caller waits (vmcnt); no other code of
   // these kernels has a value in m0.
   template <int THREADS, int KPER>
-  static SGNN_DEV void direct(const char* lds, const char* first, const uint32_t (&o)[KPER]) {
+  static SGNN_DEV void direct(const char* lds, const char* first, const uint32_t (&o)[KPER], int tid = threadIdx.x) {
     const uint64_t at = (uint64_t)first;
     const uint64_t base = (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32 |
                           (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)at);
 #pragma unroll
     for (int i = 0; i < KPER; ++i) {
       const uint32_t to = __builtin_amdgcn_readfirstlane(
-          (uint32_t)(uintptr_t)(const SGNN_LDS char*)lds + (i * THREADS + threadIdx.x / 64 * 64) * 16);
+          (uint32_t)(uintptr_t)(const SGNN_LDS char*)lds + (i * THREADS + tid / 64 * 64) * 16);
       asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                    :
                    : "s"(to), "v"(o[i]), "s"(base)
@@ -150,6 +150,25 @@ struct Tile16 {
     }
   }
 };
+
+// The order asked of the scheduler for the products of two steps of 32 k (TM x TN sub-tiles, RA / RB LDS reads per
+// fragment): fragments are read two rows of products ahead of their use.  Left to itself the compiler reads each right
+// before its products, with LDS's latency in the open.
+template <int TM, int TN, int RA, int RB>
+SGNN_DEV void order_products() {
+  constexpr int kMfma = 0x008, kRead = 0x100, kNext = (TM * RA + TN * RB + TM - 1) / TM;
+  __builtin_amdgcn_sched_group_barrier(kRead, TN * RB + 2 * RA, 0);
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, TN, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, kNext, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < TM; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMfma, TN, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, RA, 0);
+  }
+}
 
 // Waits until at most `keep` stages' direct loads (PER of this wave each) are under way.
 template <int PER, int MOST>

@@ -106,14 +106,18 @@ struct NsGemm {
 
 // BT x BT outputs by four waves.  P planes per operand (1: hi alone).  SYM: the product is symmetric; only the tiles
 // on and above the diagonal are formed and each is written to both sides.
-template <int P, bool AC, bool BC, int BT, bool SYM, int NST>
-__global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
+// KG groups of four waves take every KG-th block of k each, with LDS of their own, and are added in order at the end:
+// these products have few tiles (36 of 128 x 128 in the triangle of 1024), and one wave per SIMD leaves memory's and
+// LDS's latencies in the open.
+template <int P, bool AC, bool BC, int BT, bool SYM, int KG>
+__global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
   constexpr int BK = 64 / P, kThreads = 256, TT = BT / 2 / 16;
   using TA = Tile16<BT, BK, AC>;
   using TB = Tile16<BT, BK, BC>;
   constexpr int kStage = 2 * P * TA::kBytes;
-  __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
-  const int w = wave_id(), wm = w >> 1, wn = w & 1, l = lane_id();
+  __shared__ __attribute__((aligned(16))) char all[2 * KG * kStage];
+  const int kg = wave_id() >> 2, w = wave_id() & 3, wm = w >> 1, wn = w & 1, l = lane_id(), tid = threadIdx.x & 255;
+  char* lds = all + kg * 2 * kStage;
   int tm, tn;
   if constexpr (SYM) {  // row tm of the triangle holds tiles_n - tm tiles
     int t = blockIdx.x;
@@ -136,29 +140,27 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
     for (int j = 0; j < TT; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
   constexpr int PER = BT * BK / 8 / kThreads;
   uint32_t oa[PER], ob[PER];
-  TA::template offsets<kThreads>(oa, g.lda, BT, 0);
-  TB::template offsets<kThreads>(ob, g.ldb, BT, 0);
+  TA::template offsets<kThreads>(oa, g.lda, BT, 0, tid);
+  TB::template offsets<kThreads>(ob, g.ldb, BT, 0, tid);
   const char* pa = reinterpret_cast<const char*>(g.A + b * g.batch_a + (AC ? m0 : m0 * g.lda));
   const char* pb = reinterpret_cast<const char*>(g.B + b * g.batch_b + (BC ? n0 : n0 * g.ldb));
   const int64_t sa = 2 * BK * (AC ? g.lda : 1), sb = 2 * BK * (BC ? g.ldb : 1);
   const auto stage = [&](char* to, int blk) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-      TA::template direct<kThreads>(to + p * TA::kBytes, pa + 2 * p * g.plane_a + blk * sa, oa);
-      TB::template direct<kThreads>(to + (P + p) * TA::kBytes, pb + 2 * p * g.plane_b + blk * sb, ob);
+      TA::template direct<kThreads>(to + p * TA::kBytes, pa + 2 * p * g.plane_a + blk * sa, oa, tid);
+      TB::template direct<kThreads>(to + (P + p) * TA::kBytes, pb + 2 * p * g.plane_b + blk * sb, ob, tid);
     }
   };
   const int blocks = g.K / BK;
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i)
-    if (i < blocks) stage(lds + i * kStage, i);
-  int turn = 0;
-  for (int blk = 0; blk < blocks; ++blk) {
-    wait_stages<2 * P * PER, NST - 2>(blocks - 1 - blk);
+  if (kg < blocks) stage(lds, kg);
+  for (int round = 0; round * KG < blocks; ++round) {
+    const int blk = round * KG + kg;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    if (blk + NST - 1 < blocks) stage(lds + (turn == 0 ? NST - 1 : turn - 1) * kStage, blk + NST - 1);
-    const char* here = lds + turn * kStage;
-    turn = turn == NST - 1 ? 0 : turn + 1;
+    if (blk + KG < blocks) stage(lds + ((round & 1) ^ 1) * kStage, blk + KG);
+    if (blk >= blocks) continue;
+    const char* here = lds + (round & 1) * kStage;
 #pragma unroll
     for (int kk = 0; kk < BK / 32; ++kk) {
       s16x8 fa[P][TT], fb[P][TT];
@@ -184,11 +186,26 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
 #pragma unroll
         for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
     }
+    // one workgroup per CU only: where two share it they hide each other's reads (42 us without, 44 with)
+    if constexpr (P == 1 && TT == 4 && KG > 1) order_products<TT, TT, AC ? 2 : 1, BC ? 2 : 1>();
   }
   __syncthreads();
+  if constexpr (KG > 1) {
+    f32x4* sums = reinterpret_cast<f32x4*>(all) + ((kg - 1) * 4 + w) * TT * TT * 64 + l;
+    static_assert((KG - 1) * 4 * TT * TT * 64 * 16 <= 2 * KG * kStage, "the groups' sums fit");
+    if (kg > 0)
+#pragma unroll
+      for (int i = 0; i < TT * TT; ++i) sums[64 * i] = acc[i / TT][i % TT];
+    __syncthreads();
+    if (kg > 0) return;
+    for (int q = 1; q < KG; ++q)
+#pragma unroll
+      for (int i = 0; i < TT * TT; ++i) acc[i / TT][i % TT] += sums[(q * 4 * TT * TT + i) * 64];
+    // the epilogue's buffers are this wave's own part of what it has read
+  }
   // through LDS by 16 rows of m (as in gemm.hip), so that every load and store is 16 bytes of a row
   constexpr int kPieces = 4 * TT, kMask = kPieces - 1;
-  float* buf = reinterpret_cast<float*>(lds) + w * 16 * 16 * TT;
+  float* buf = reinterpret_cast<float*>(all) + w * TT * TT * 256;
   const float alpha = g.alpha * kInvScale * kInvScale;
   const f16_t* R = g.R ? g.R + b * g.batch_c : nullptr;
   f16_t* C = g.C + b * g.batch_c;
@@ -255,12 +272,21 @@ __global__ __launch_bounds__(256) void k_ns_gemm(NsGemm g) {
   }
 }
 
+// Up to this many tiles in a launch, a workgroup of k_ns_gemm splits k over groups of waves (KG): each CU has one tile at
+// most and only its own waves hide its latency. Above it the groups of one tile cost LDS that a second tile would use: a
+// product of 512 tiles (2048 x 2048 by 2048 x 4096) took 47 us with two groups and 42 with one, the symmetric one of
+// 136 tiles 38 and 45.
+constexpr int64_t kFewTiles = 256;
+
 template <int P, bool AC, bool BC, bool SYM>
 void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
   const int tiles = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
   const dim3 grid((unsigned)tiles, 1, (unsigned)count);
-  if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 2>), grid, dim3(256), 0, s, g);
-  else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 4>), grid, dim3(256), 0, s, g);
+  const bool few = (int64_t)tiles * count <= kFewTiles;
+  if (bt == 128 && few) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 2>), grid, dim3(512), 0, s, g);
+  else if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 1>), grid, dim3(256), 0, s, g);
+  else if (few) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 4>), grid, dim3(1024), 0, s, g);
+  else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 1>), grid, dim3(256), 0, s, g);
 }
 
 // ----------------------------------------------------------------------------- small matrices
@@ -296,39 +322,50 @@ SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane
   for (int i = 0; i < BI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-  for (int k0 = 0; k0 < K; k0 += 32) {
-    s16x8 fa[P][BI], fb[P][2];
+  s16x8 fa[2][P][BI], fb[2][P][2];
+  const auto load = [&](int h, int k0) {
 #pragma unroll
     for (int p = 0; p < P; ++p) {
 #pragma unroll
       for (int i = 0; i < BI; ++i)
-        fa[p][i] = *reinterpret_cast<const s16x8*>(A + p * plane_a + 2 * ((a0 + 16 * i + (l & 15)) * lda + k0 + 8 * (l >> 4)));
+        fa[h][p][i] = *reinterpret_cast<const s16x8*>(A + p * plane_a + 2 * ((a0 + 16 * i + (l & 15)) * lda + k0 + 8 * (l >> 4)));
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         if constexpr (!BT) {
-          fb[p][i] = *reinterpret_cast<const s16x8*>(B + p * plane_b + 2 * ((b0 + 16 * i + (l & 15)) * ldb + k0 + 8 * (l >> 4)));
+          fb[h][p][i] = *reinterpret_cast<const s16x8*>(B + p * plane_b + 2 * ((b0 + 16 * i + (l & 15)) * ldb + k0 + 8 * (l >> 4)));
         } else {
           const char* at = B + p * plane_b + 2 * ((k0 + 8 * (l >> 4) + ((l & 15) >> 2)) * ldb + b0 + 16 * i + 4 * (l & 3));
           const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(at));
           const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((SGNN_LDS s16x4*)(at + 8 * ldb));
-          fb[p][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          fb[h][p][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
       }
     }
+  };
+  const auto multiply = [&](int h) {
     if constexpr (P == 2) {
 #pragma unroll
       for (int i = 0; i < BI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][1][j], fa[h][0][i], acc[i][j]);
 #pragma unroll
       for (int i = 0; i < BI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
+        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][1][i], acc[i][j]);
     }
 #pragma unroll
     for (int i = 0; i < BI; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][0][i], acc[i][j]);
+  };
+  // the next 32 k are read under this one's products (past the end: the last ones again)
+  load(0, 0);
+  for (int k0 = 0; k0 < K; k0 += 64) {
+    load(1, min(k0 + 32, K - 32));
+    multiply(0);
+    if (k0 + 32 >= K) break;
+    load(0, min(k0 + 64, K - 32));
+    multiply(1);
   }
 }
 
@@ -642,20 +679,30 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
     const int r0 = tall ? c0 : 0, rows = tall ? min(kChunk, grp.rows - c0) : grp.rows;
     const int k0 = tall ? 0 : c0, cols = tall ? grp.cols : min(kChunk, grp.cols - c0);
     const T* in = static_cast<const T*>(grp.in[mat]) + (int64_t)r0 * grp.ld_in[mat] + k0;
-    const int per = (cols + V - 1) / V;
-#pragma unroll 4
-    for (int t = threadIdx.x; t < rows * per; t += kSmallThreads) {
-      const int r = t / per, c = (t - r * per) * V;
-      float v[V];
-      load_some<V>(in + (int64_t)r * grp.ld_in[mat] + c, cols - c, v);
+    const int per = (cols + V - 1) / V, pieces = rows * per;
+    constexpr int U = 4;  // loads under way before the first is used
+    for (int t0 = threadIdx.x; t0 < pieces; t0 += U * kSmallThreads) {
+      u32x4 raw[U];
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        if (c + e >= cols) continue;
-        char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
-        const float y = (norm == 0.0f ? 0.0f : v[e] / norm) * kScale;
-        const f16_t h = (f16_t)y;
-        *reinterpret_cast<f16_t*>(at) = h;
-        if constexpr (P == 2) *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);
+      for (int u = 0; u < U; ++u) {
+        const int t = min(t0 + u * kSmallThreads, pieces - 1), r = t / per, c = (t - r * per) * V;
+        raw[u] = load_raw(in + (int64_t)r * grp.ld_in[mat] + c, cols - c);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int t = t0 + u * kSmallThreads, r = t / per, c = (t - r * per) * V;
+        if (t >= pieces) break;
+        float v[V];
+        unpack<T>(raw[u], v);
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          if (c + e >= cols) continue;
+          char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
+          const float y = (norm == 0.0f ? 0.0f : v[e] / norm) * kScale;
+          const f16_t h = (f16_t)y;
+          *reinterpret_cast<f16_t*>(at) = h;
+          if constexpr (P == 2) *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);
+        }
       }
     }
   }

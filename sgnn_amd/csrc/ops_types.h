@@ -169,10 +169,23 @@ constexpr float kGeluCubic = 0.044715f;
 
 SGNN_DEV float sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
 
-// act(z) and, where SLOPE, d act / d z, which share their functions.  ReLU keeps a NaN (a comparison, not a maximum);
+// The standard normal distribution function and e = exp(-z^2 / 2), which it shares with its density, by Abramowitz and
+// Stegun 7.1.26: 1 - Phi(|z|) = (a1 t + ... + a5 t^5) e / 2, t = 1 / (1 + p |z| / sqrt 2), good to 7.5e-8 (relative:
+// 6e-8 at z = -1, 5e-4 at -4, where 1 + erf(z) in fp32 is off by 1e-3) -- for the 16-bit types, whose rounding hides it.
+// A third of erff's instructions: 8192 x 2048 -> 8192 in bf16 with gelu and its slopes went from 325 to 296 us.
+SGNN_DEV float normal_cdf(float z, float& e) {
+  const float t = __builtin_amdgcn_rcpf(1.0f + 0.3275911f * kInvSqrt2 * fabsf(z));
+  e = __expf(-0.5f * z * z);
+  const float poly =
+      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float tail = 0.5f * poly * e;
+  return z < 0.0f ? tail : 1.0f - tail;
+}
+
+// act(z) and, where SLOPE, d act / d z, which share their functions; FAST: gelu by normal_cdf.  ReLU keeps a NaN (a comparison, not a maximum);
 // its slope at 0 is 0.  Far out, where the smooth ones' second terms are 0 in fp32 but for the products of 0 and
 // infinity in them, the slopes are the first terms alone.
-template <int ACT, bool SLOPE>
+template <int ACT, bool SLOPE, bool FAST>
 SGNN_DEV void act_both(float z, float& value, float& slope) {
   value = z, slope = 1.0f;
   if constexpr (ACT == SGNN_ACT_RELU) {
@@ -180,9 +193,15 @@ SGNN_DEV void act_both(float z, float& value, float& slope) {
     slope = z > 0.0f ? 1.0f : 0.0f;
   }
   if constexpr (ACT == SGNN_ACT_GELU) {
-    const float phi = 0.5f * (1.0f + erff(z * kInvSqrt2));
+    float phi, e;
+    if constexpr (FAST) {
+      phi = normal_cdf(z, e);
+    } else {
+      phi = 0.5f * (1.0f + erff(z * kInvSqrt2));
+      e = __expf(-0.5f * z * z);
+    }
     value = z * phi;
-    if constexpr (SLOPE) slope = fabsf(z) > 20.0f ? phi : phi + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    if constexpr (SLOPE) slope = fabsf(z) > 20.0f ? phi : phi + z * kInvSqrt2Pi * e;
   }
   if constexpr (ACT == SGNN_ACT_GELU_TANH) {  // 0.5 (1 + tanh u) = sigmoid(2 u)
     const float s = sigmoid(2.0f * kSqrt2OverPi * (z + kGeluCubic * z * z * z));
