@@ -1,30 +1,29 @@
-// The matrix product behind sgnn_linear, its backward pass and sgnn_newton_schulz (gemm.hip).
+// The matrix product behind sgnn_linear and its backward pass (gemm.hip).
 #pragma once
 #include <stddef.h>
 #include <stdint.h>
 
 namespace sgnn {
 
-// C[b][m][n] = act(alpha sum_k A[b](m, k) B[b](n, k) + bias[n]) + beta res[b][m][n] over the batch b.
+// C[m][n] = act(sum_k A(m, k) B(n, k) + bias[n]) + res[m][n].
 // An operand is stored with k contiguous ("rows": A[m * lda + k]) or, where a_cols / b_cols is set, with m / n
 // contiguous (A[k * lda + m]).  All operands are of type dtype.
 struct Gemm {
   int32_t dtype = 0;
-  int64_t M = 0, N = 0, K = 0, batch = 1;
+  int64_t M = 0, N = 0, K = 0;
   const void* A = nullptr;
-  int64_t lda = 0, batch_a = 0;
+  int64_t lda = 0;
   bool a_cols = false;
   const void* B = nullptr;
-  int64_t ldb = 0, batch_b = 0;
+  int64_t ldb = 0;
   bool b_cols = false;
   const void* bias = nullptr;
   int32_t act = 0;
-  float alpha = 1.0f, beta = 1.0f;
   const void* res = nullptr;
-  int64_t ldr = 0, batch_r = 0;
-  void* slope = nullptr;   // act'(alpha sum + bias), dense [M][N] as sgnn_linear describes it; batch 1 only
+  int64_t ldr = 0;
+  void* slope = nullptr;   // act'(sum + bias), dense [M][N] as sgnn_linear describes it
   void* C = nullptr;
-  int64_t ldc = 0, batch_c = 0;
+  int64_t ldc = 0;
 };
 
 size_t gemm_workspace_bytes(const Gemm& g);

@@ -22,9 +22,8 @@ struct GemmArgs {
   const void *A, *B, *bias, *res;
   void *slope, *C;
   float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
-  int64_t lda, ldb, ldr, ldc, M, N, K, batch_a, batch_b, batch_r, batch_c;
+  int64_t lda, ldb, ldr, ldc, M, N, K;
   int32_t act, nsplit, tiles_m, tiles_n;
-  float alpha, beta;
 };
 
 // ----------------------------------------------------------------------------- epilogue
@@ -52,10 +51,10 @@ SGNN_DEV void load_bias(const GemmArgs& g, int64_t n, int cnt, float (&t)[V]) {
 
 // V = 16 bytes' consecutive outputs (m, n ..) of one lane; cnt of them exist.
 template <typename T, int V>
-SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float (&v)[V], const float (&bias)[V], int cnt) {
+SGNN_DEV void finish(const GemmArgs& g, int64_t m, int64_t n, float (&v)[V], const float (&bias)[V], int cnt) {
   float t[V];
 #pragma unroll
-  for (int i = 0; i < V; ++i) v[i] = g.alpha * v[i] + bias[i];
+  for (int i = 0; i < V; ++i) v[i] += bias[i];
   switch (g.act) {  // the same for every lane
     case SGNN_ACT_RELU: act_row<SGNN_ACT_RELU, T>(g, m * g.N + n, cnt, v); break;
     case SGNN_ACT_GELU: act_row<SGNN_ACT_GELU, T>(g, m * g.N + n, cnt, v); break;
@@ -64,18 +63,18 @@ SGNN_DEV void finish(const GemmArgs& g, int64_t b, int64_t m, int64_t n, float (
     default: break;
   }
   if (g.res) {
-    load_some<V>(static_cast<const T*>(g.res) + b * g.batch_r + m * g.ldr + n, cnt, t);
+    load_some<V>(static_cast<const T*>(g.res) + m * g.ldr + n, cnt, t);
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += g.beta * t[i];
+    for (int i = 0; i < V; ++i) v[i] += t[i];
   }
-  store_some<V>(static_cast<T*>(g.C) + b * g.batch_c + m * g.ldc + n, cnt, v);
+  store_some<V>(static_cast<T*>(g.C) + m * g.ldc + n, cnt, v);
 }
 
 // A wave's accumulators (TM x TN sub-tiles of 16 x 16, lane l: m = l & 15, n = 4 (l >> 4) + r) to memory, RP sub-tile
 // rows at a time through `buf` (16 RP x 16 TN floats of its own).  16-byte pieces are XORed with m, so that the 16
 // rows of one write, which are a multiple of all banks apart, fall on different ones.
 template <typename T, int RP, int TM, int TN>
-SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][TN], int64_t b, int split, int64_t m0,
+SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][TN], int split, int64_t m0,
                          int64_t n0) {
   static_assert(TM % RP == 0, "whole rounds");
   const int l = lane_id();
@@ -120,7 +119,7 @@ SGNN_DEV void write_tile(const GemmArgs& g, float* buf, const f32x4 (&acc)[TM][T
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[4 * q + e] = f[e];
         }
-        if (mr + r < g.M && cnt > 0) finish<T>(g, b, mr + r, n_mine, v, bias, cnt);
+        if (mr + r < g.M && cnt > 0) finish<T>(g, mr + r, n_mine, v, bias, cnt);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -168,10 +167,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   int tm, tn;
   tile_of(g, tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int split = g.nsplit > 1 ? blockIdx.z : 0;
-  const int64_t batch = g.nsplit > 1 ? 0 : blockIdx.z;
-  const char* A = static_cast<const char*>(g.A) + 2 * batch * g.batch_a;
-  const char* B = static_cast<const char*>(g.B) + 2 * batch * g.batch_b;
+  const int split = blockIdx.z;
+  const char* A = static_cast<const char*>(g.A);
+  const char* B = static_cast<const char*>(g.B);
   int first, last;
   blocks_of(g, BK, split, first, last);
 
@@ -281,7 +279,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     }
   }
   __syncthreads();
-  write_tile<T, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, batch, split, m0 + wm * TM * 16,
+  write_tile<T, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, split, m0 + wm * TM * 16,
                     n0 + wn * TN * 16);
 }
 
@@ -442,10 +440,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
   int tm, tn;
   tile_of(g, tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
-  const int split = g.nsplit > 1 ? blockIdx.z : 0;
-  const int64_t batch = g.nsplit > 1 ? 0 : blockIdx.z;
-  const float* A = static_cast<const float*>(g.A) + batch * g.batch_a;
-  const float* B = static_cast<const float*>(g.B) + batch * g.batch_b;
+  const int split = blockIdx.z;
+  const float* A = static_cast<const float*>(g.A);
+  const float* B = static_cast<const float*>(g.B);
   int first, last;
   blocks_of(g, BK, split, first, last);
 
@@ -560,7 +557,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
         acc[i][j][r] = s;
       }
     }
-  write_tile<float, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, batch, split, m0 + wm * TM * 16,
+  write_tile<float, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, split, m0 + wm * TM * 16,
                         n0 + wn * TN * 16);
 }
 
@@ -650,7 +647,7 @@ __global__ __launch_bounds__(64 * W) void k_gemm_rows(GemmArgs g) {
     const int cnt = (int)min((int64_t)V, g.N - n0 - c);
     float bias[V];
     load_bias<T>(g, n0 + c, cnt, bias);
-    finish<T>(g, 0, m, n0 + c, v, bias, cnt);
+    finish<T>(g, m, n0 + c, v, bias, cnt);
   }
 }
 
@@ -690,7 +687,7 @@ __global__ __launch_bounds__(32 * kJoinParts) void k_gemm_join(GemmArgs g) {
     for (int e = 0; e < V; ++e) v[e] += sums[q][i][e];
   float bias[V];
   load_bias<T>(g, n, cnt, bias);
-  finish<T>(g, 0, m, n, v, bias, cnt);
+  finish<T>(g, m, n, v, bias, cnt);
 }
 
 // ----------------------------------------------------------------------------- choice and launch
@@ -701,13 +698,12 @@ struct Plan {
 // The larger tile moves fewer bytes per product through LDS and L2, the smaller ones fill the 256 CUs sooner; long
 // k is split over workgroups where the tiles alone leave CUs idle.
 Plan plan_of(const Gemm& g) {
-  const auto tiles = [&](int bm, int bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn) * g.batch; };
+  const auto tiles = [&](int bm, int bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
   const int bk = g.dtype == SGNN_F32 ? 32 : 64;
   Plan p{64, 64, 1};
   if (g.dtype != SGNN_F32 && tiles(256, 256) >= 192) p = {256, 256, 1};
   else if (g.dtype == SGNN_F32 && tiles(256, 128) >= 256 && g.K >= 1024) p = {256, 128, 1};
   else if (tiles(128, 128) >= 128 || g.K >= 2048) p = {128, 128, 1};
-  if (g.batch > 1) return p;
   // what is resident at once: one workgroup per CU of the large tiles, two of the others
   const int64_t blocks = (g.K + bk - 1) / bk, wgs = p.bm == 256 ? 256 : 512;
   const int64_t want = wgs / std::max<int64_t>(1, tiles(p.bm, p.bn));
@@ -739,7 +735,7 @@ void launch_tiles(const GemmArgs& g, const Plan& p, dim3 grid, bool direct, hipS
 }
 
 // The row kernel: 32 rows at most, and few enough columns per row of x that x's repeated reads stay below w's.
-bool rows_ok(const Gemm& g) { return !g.a_cols && !g.b_cols && g.batch == 1 && g.M <= 32; }
+bool rows_ok(const Gemm& g) { return !g.a_cols && !g.b_cols && g.M <= 32; }
 
 template <typename T>
 void launch_rows(const GemmArgs& g, hipStream_t s) {
@@ -758,8 +754,8 @@ void launch_rows(const GemmArgs& g, hipStream_t s) {
 }
 
 // Whether the direct-to-LDS loads serve an operand: 16-byte lines whose offsets within a tile fit 32 bits.
-bool direct_ok(const void* p, int64_t ld, int64_t batch, bool cols, int64_t rows) {
-  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && batch % 8 == 0 && ld < kNear &&
+bool direct_ok(const void* p, int64_t ld, bool cols, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % 8 == 0 && ld < kNear &&
          (!cols || rows % 8 == 0);
 }
 
@@ -774,10 +770,10 @@ size_t gemm_workspace_bytes(const Gemm& g) {
 }
 
 int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* stream) {
-  if (g.M == 0 || g.N == 0 || g.batch == 0) return SGNN_OK;
+  if (g.M == 0 || g.N == 0) return SGNN_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K, g.batch_a,
-             g.batch_b, g.batch_r, g.batch_c, g.act, 1, 0, 0, g.alpha, g.beta};
+  GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K,
+             g.act, 1, 0, 0};
   if (rows_ok(g)) {
     with_type(g.dtype, [&](auto* t) {
       launch_rows<std::remove_pointer_t<decltype(t)>>(a, s);
@@ -786,18 +782,18 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
     return check_launch("gemm");
   }
   Plan p = plan_of(g);
-  const bool direct = direct_ok(g.A, g.lda, g.batch_a, g.a_cols, g.M) && direct_ok(g.B, g.ldb, g.batch_b, g.b_cols, g.N);
+  const bool direct = direct_ok(g.A, g.lda, g.a_cols, g.M) && direct_ok(g.B, g.ldb, g.b_cols, g.N);
   if (!direct && p.bm == 256 && g.dtype != SGNN_F32) p.bm = p.bn = 128;
   const int64_t tm = (g.M + p.bm - 1) / p.bm, tn = (g.N + p.bn - 1) / p.bn;
-  if (tm > INT32_MAX / tn || g.batch > 65535 || g.K > (int64_t)INT32_MAX * 32)
-    return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k, or 65535 matrices");
+  if (tm > INT32_MAX / tn || g.K > (int64_t)INT32_MAX * 32)
+    return set_error(SGNN_ERR_UNSUPPORTED, "gemm: more than 2^31 tiles or blocks of k");
   a.nsplit = p.nsplit, a.tiles_m = (int32_t)tm, a.tiles_n = (int32_t)tn;
   if (p.nsplit > 1) {
     if (!workspace || workspace_bytes < gemm_workspace_bytes(g))
       return set_error(SGNN_ERR_INVALID, "gemm: workspace too small");
     a.part = static_cast<float*>(workspace);
   }
-  const dim3 grid((unsigned)(tm * tn), 1, (unsigned)(p.nsplit > 1 ? p.nsplit : g.batch));
+  const dim3 grid((unsigned)(tm * tn), 1, (unsigned)p.nsplit);
   with_type(g.dtype, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (!g.a_cols && !g.b_cols) launch_tiles<T, false, false>(a, p, grid, direct, s);

@@ -272,21 +272,21 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
   }
 }
 
-// Up to this many tiles in a launch, a workgroup of k_ns_gemm splits k over groups of waves (KG): each CU has one tile at
-// most and only its own waves hide its latency. Above it the groups of one tile cost LDS that a second tile would use: a
-// product of 512 tiles (2048 x 2048 by 2048 x 4096) took 47 us with two groups and 42 with one, the symmetric one of
-// 136 tiles 38 and 45.
-constexpr int64_t kFewTiles = 256;
+// Up to this many 128 x 128 tiles of one matrix, a workgroup of k_ns_gemm splits k over two groups of waves: a CU then has
+// one tile at most and only its own waves hide its latency. Above it the groups of one tile cost LDS that a second tile
+// would use: a product of 512 tiles (2048 x 2048 by 2048 x 4096) took 47 us with two groups and 42 with one, the symmetric
+// one of 136 tiles 38 and 45.  Neither the batch nor the tile's size decides, so a matrix gets the same bits in any batch.
+constexpr int kFewTiles = 256;
 
 template <int P, bool AC, bool BC, bool SYM>
 void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
-  const int tiles = SYM ? g.tiles_m * (g.tiles_m + 1) / 2 : g.tiles_m * g.tiles_n;
-  const dim3 grid((unsigned)tiles, 1, (unsigned)count);
-  const bool few = (int64_t)tiles * count <= kFewTiles;
-  if (bt == 128 && few) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 2>), grid, dim3(512), 0, s, g);
-  else if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 128, SYM, 1>), grid, dim3(256), 0, s, g);
-  else if (few) hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 4>), grid, dim3(1024), 0, s, g);
-  else hipLaunchKernelGGL((k_ns_gemm<P, AC, BC, 64, SYM, 1>), grid, dim3(256), 0, s, g);
+  const auto tiles = [&](int m, int n) { return SYM ? m * (m + 1) / 2 : m * n; };
+  const dim3 grid((unsigned)tiles(g.tiles_m, g.tiles_n), 1, (unsigned)count);
+  const int per = 128 / bt;
+  const bool few = tiles((g.tiles_m + per - 1) / per, (g.tiles_n + per - 1) / per) <= kFewTiles;
+  const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g); };
+  if (bt == 128) few ? go(k_ns_gemm<P, AC, BC, 128, SYM, 2>, 512) : go(k_ns_gemm<P, AC, BC, 128, SYM, 1>, 256);
+  else few ? go(k_ns_gemm<P, AC, BC, 64, SYM, 2>, 512) : go(k_ns_gemm<P, AC, BC, 64, SYM, 1>, 256);
 }
 
 // ----------------------------------------------------------------------------- small matrices

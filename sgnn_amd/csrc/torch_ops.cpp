@@ -73,6 +73,7 @@ int32_t dtype_of(const Tensor& t) { return dtype_of(t.scalar_type()); }
 
 void on_gpu(const Tensor& t, const char* name) {
   TORCH_CHECK_VALUE(t.is_cuda(), name, " must be a GPU tensor (sgnn_amd runs on MI355X only; no CPU path)");
+  TORCH_CHECK_VALUE(t.layout() == at::kStrided && !t.is_neg(), name, " must be a plain strided tensor");
 }
 void supported(const Tensor& t, const char* name) {
   on_gpu(t, name);
@@ -337,7 +338,11 @@ std::vector<Tensor> newton_schulz(const std::vector<Tensor>& gs, const std::vect
       TORCH_CHECK_VALUE(given[k].sizes() == g.sizes() &&
                             ((given[k].stride(-1) == 1 && given[k].stride(-2) >= n) || given[k].is_contiguous()),
                         "newton_schulz: out ", given[k].sizes(), " with strides ", given[k].strides(), " for ", g.sizes());
+      const int64_t count = g.dim() == 3 ? g.size(0) : 1, row = given[k].stride(-2), batch = count > 1 ? given[k].stride(0) : 0;
+      TORCH_CHECK_VALUE(count < 2 || batch >= (m - 1) * row + n || (batch >= n && row >= (count - 1) * batch + n),
+                        "newton_schulz: out's matrices overlap: strides ", given[k].strides(), " for ", g.sizes());
       outs.push_back(given[k]);
+      if (!given[k].is_inference()) given[k].unsafeGetTensorImpl()->bump_version();
     }
     const Tensor &in = ins.back(), &out = outs.back();
     if (g.numel() == 0) continue;

@@ -27,8 +27,8 @@ def newton_schulz(g: Union[torch.Tensor, Sequence[torch.Tensor]], steps: int = 5
     g: a matrix [m, n], a batch [b, m, n], or a sequence of these (of one type and
     device; any shapes: matrices of one shape next to each other share launches).
     Returns new tensors of g's shapes and type, or writes `out` (likewise; rows of
-    unit stride; it may be g itself, but no two of its matrices may overlap).  Not
-    differentiable."""
+    unit stride).  A matrix of `out` may be its own g; it may overlap nothing else
+    of g or `out`.  Not differentiable."""
     single = isinstance(g, torch.Tensor)
     outs = [] if out is None else [out] if single else list(out)
     got = torch_ops().newton_schulz([g] if single else list(g), outs, steps, *coefficients, eps)

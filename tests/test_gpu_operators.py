@@ -184,6 +184,55 @@ def test_linear_gradient_against_differences():
             assert abs(diff - float((grads[i].double() * dirs[i].double()).sum())) <= tol, (act, i)
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(3841, 3080, 40), (3841, 3081, 41), (8200, 1000, 1030), (8200, 1000, 1032),
+                                   (30, 700, 300), (32, 4096, 1100), (25, 33, 4100)])
+def test_linear_of_many_tiles_is_exact(dtype, M, N, K):
+    """The largest tiles with ragged edges, and some rows against wide weights (|sums| <= 4 * 8200 < 2^24)."""
+    from sgnn_amd import functional
+    x, w, dy = (whole(s, i, dtype=dtype).cuda() for i, s in enumerate([(M, K), (N, K), (M, N)]))
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    got = functional.linear(*leaves, activation="relu")
+    dx, dw = torch.autograd.grad(got, leaves, dy)
+    z = x.detach().double() @ w.detach().double().T
+    dz = dy.double() * (z > 0)
+    assert torch.equal(got.detach(), z.relu().to(dtype))
+    assert torch.equal(dx, (dz @ w.detach().double()).to(dtype))
+    assert torch.equal(dw, (dz.T.contiguous() @ x.detach().double()).to(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_linear_offsets_past_32_bits(dtype):
+    """Rows 20M elements apart, and 2^31 elements of x: whole numbers, so the far rows are exact."""
+    from sgnn_amd import functional
+    rows, K, N, ld = 130, 72, 40, 20_000_000
+    x, w, dy = whole((rows, K), 1, dtype=dtype), whole((N, K), 2, dtype=dtype), whole((rows, N), 3, dtype=dtype)
+    far = torch.empty(rows * ld, dtype=dtype, device="cuda").view(rows, ld)
+    xs, dys = far[:, :K], far[:, 100:100 + N]
+    xs.copy_(x), dys.copy_(dy)
+    leaves = [xs.detach().requires_grad_(True), w.cuda().requires_grad_(True)]
+    got = functional.linear(*leaves, residual=dys)
+    dx, dw = torch.autograd.grad(got, leaves, dys)
+    assert torch.equal(got.detach().cpu(), (x.double() @ w.double().T + dy.double()).to(dtype))
+    assert torch.equal(dx.cpu(), (dy.double() @ w.double()).to(dtype))
+    assert torch.equal(dw.cpu(), (dy.double().T @ x.double()).to(dtype))
+    y = functional.layer_norm(xs)
+    assert torch.equal(y, functional.layer_norm(xs.contiguous()))
+    del far, xs, dys, leaves, got, dx, dw
+    M = 2 ** 31 // K + 1000
+    tall = torch.zeros(M, K, dtype=dtype, device="cuda")
+    tall[-rows:] = x.cuda()
+    assert torch.equal(functional.linear(tall, w.cuda())[-rows:].cpu(), (x.double() @ w.double().T).to(dtype))
+    ones = torch.ones(K, dtype=dtype, device="cuda").requires_grad_(True)
+    leaf = tall.requires_grad_(True)
+    out = functional.layer_norm(leaf, ones)
+    assert torch.equal(out.detach()[-rows:], functional.layer_norm(x.cuda(), ones.detach()))
+    dx, = torch.autograd.grad(out, leaf, tall.detach())
+    few = x.cuda().requires_grad_(True)
+    want, = torch.autograd.grad(functional.layer_norm(few, ones), few, x.cuda())
+    assert torch.equal(dx[-rows:], want) and not dx[:-rows].any()
+
+
 def test_linear_edges_of_sizes():
     from sgnn_amd import functional
     for dtype in TYPES:
@@ -384,7 +433,7 @@ def ns_tol(ref, dtype, m, n):
 
 
 NS_SIZES = [(1, 1), (1, 7), (5, 1), (3, 4), (16, 16), (17, 31), (64, 64), (100, 60), (128, 128), (128, 384), (129, 200),
-            (60, 515), (300, 260), (200, 1031)]
+            (60, 515), (300, 260), (200, 1031), (128, 1024), (100, 2047), (33, 2050), (3, 4097), (520, 1100)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -432,6 +481,29 @@ def test_newton_schulz_batches_and_lists():
     assert muon.newton_schulz([]) == []
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("count,m,n", [(40, 20, 24), (70, 64, 64), (12, 128, 384), (33, 100, 300), (12, 300, 260), (9, 520, 640)])
+def test_newton_schulz_of_a_batch_keeps_each_matrix_bits(dtype, count, m, n):
+    from sgnn_amd import muon
+    batch = (0.02 * normal((count, m, n), 1)).to(dtype).cuda()
+    got = muon.newton_schulz(batch)
+    for i in (0, 1, count - 1):
+        assert torch.equal(got[i], muon.newton_schulz(batch[i])), i
+    flipped = muon.newton_schulz(list(batch.flip(0)))
+    assert all(torch.equal(a, b) for a, b in zip(flipped, got.flip(0)))
+    again = batch.clone()
+    assert muon.newton_schulz(again, out=again) is again and torch.equal(again, got)
+
+
+@pytest.mark.parametrize("m,n", [(5, 9), (128, 384), (300, 64), (100, 1500), (200, 260)])
+def test_newton_schulz_without_steps_normalises(m, n):
+    """x / |x| kept to 2^-21 of itself or, where it is small, 2^-34 (two fp16 planes of 2^10 x)."""
+    from sgnn_amd import muon
+    g = normal((m, n), 2)
+    ref = ns64(g, 0)
+    within(muon.newton_schulz(g.cuda(), steps=0), ref, 2.0 ** -21 * ref.abs() + 2.0 ** -34, "steps=0")
+
+
 def test_newton_schulz_special_values():
     from sgnn_amd import muon
     for dtype in TYPES:
@@ -458,7 +530,10 @@ def test_newton_schulz_refuses():
     x = torch.zeros(3, 4, device="cuda")
     bad = [lambda: muon.newton_schulz(x.double()), lambda: muon.newton_schulz(x[0]), lambda: muon.newton_schulz([x, x.half()]),
            lambda: muon.newton_schulz(x, steps=-1), lambda: muon.newton_schulz(x, eps=-1.0),
-           lambda: muon.newton_schulz(x[None, None]), lambda: muon.newton_schulz([x, x.cpu()])]
+           lambda: muon.newton_schulz(x[None, None]), lambda: muon.newton_schulz([x, x.cpu()]),
+           lambda: muon.newton_schulz(x, out=x.t()), lambda: muon.newton_schulz(x, out=x.half()),
+           lambda: muon.newton_schulz([x, x], out=[x]), lambda: muon.newton_schulz(x[None].repeat(2, 1, 1), out=x.expand(2, 3, 4)),
+           lambda: muon.newton_schulz(x.to_sparse())]
     for call in bad:
         with pytest.raises(ValueError):
             call()
