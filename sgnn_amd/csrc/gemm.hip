@@ -153,6 +153,9 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 // NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
 // longer than memory; the small tile has four.
+// 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 292
+// to 330 us, dz w 230 to 260, dz^T x 234 to 260.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
+// time, and the rest is the two barriers' waits per block and, forward, the epilogue's 268 MB.
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT, int NST>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   constexpr int BK = 64, kThreads = 64 * WM * WN;
@@ -564,7 +567,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
 // ----------------------------------------------------------------------------- few rows
 // M <= 16 MT rows of x, both operands with k contiguous: a workgroup takes 16 MT columns n, its W waves every W-th block
 // of k, straight from memory into the matrix instructions' registers (a lane reads 32 or 64 bytes of one row of w at a
-// time, a row's four lanes 128 or 256), and the waves' sums are added in order through LDS.  Bounded by w's bytes.
+// time, a row's four lanes 128 or 256), and the waves' sums are added in order through LDS.  Bounded by w's bytes: one row
+// by 4096 x 4096 bf16 takes 8 to 9 us, 3.9 TB/s, of which some 3 are launch and first latency (tiles of 64: 21 us).
 template <typename T, int MT, int W>
 __global__ __launch_bounds__(64 * W) void k_gemm_rows(GemmArgs g) {
   constexpr bool k32 = sizeof(T) == 4;

@@ -41,6 +41,6 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     """(x - mean) / sqrt(var + eps) * weight + bias (+ residual) over the last dimension
     (biased variance, as nn.LayerNorm).
 
-    x [..., W]; weight and bias [W] of x's type or float32 (both of one); residual
+    x [..., W] (W up to 2^23); weight and bias [W] of x's type or float32 (both of one); residual
     of x's shape and type.  Differentiable in x, weight, bias and residual."""
     return torch_ops().layer_norm(x, weight, bias, residual, eps)

@@ -38,13 +38,13 @@ def test_empty_calls_need_no_device(lib):
 
 
 def _linear_bwd(lib, dtype=0, M=4, N=4, K=4, dy=P, ldd=4, slope=P, x=P, ldx=4, w=P, ldw=4, dx=P, dw=P, db=P,
-                nws=1 << 30):
-    return lib.sgnn_linear_bwd(dtype, M, N, K, dy, ldd, slope, x, ldx, w, ldw, dx, dw, db, P, nws, None)
+                nws=1 << 30, ws=P):
+    return lib.sgnn_linear_bwd(dtype, M, N, K, dy, ldd, slope, x, ldx, w, ldw, dx, dw, db, ws, nws, None)
 
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=7), dict(M=-1), dict(dy=None), dict(ldd=3), dict(x=None), dict(ldx=3),
-    dict(w=None), dict(ldw=3), dict(nws=0)])
+    dict(w=None), dict(ldw=3), dict(nws=0), dict(ws=None)])
 def test_linear_bwd_refuses(lib, bad):
     assert _linear_bwd(lib, **bad) == INVALID
     assert "linear_bwd" in lib.sgnn_last_error().decode()
@@ -74,13 +74,15 @@ def test_norm_bwd_refuses(lib, bad):
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=4), dict(count=-1), dict(steps=-1), dict(eps=-1.0), dict(null=True),
-                                 dict(rows=-1), dict(ld=3), dict(in_=None), dict(nws=0)])
+                                 dict(rows=-1), dict(ld=3), dict(in_=None), dict(nws=0), dict(ws=None)])
 def test_newton_schulz_refuses(lib, bad):
-    a = dict(dtype=0, count=1, steps=5, eps=0.0, null=False, rows=4, ld=4, in_=P, nws=1 << 20)
+    a = dict(dtype=0, count=1, steps=5, eps=0.0, null=False, rows=4, ld=4, in_=P, nws=1 << 30, ws=P)
     a.update(bad)
-    mats = (_hip.SgnnMatrix * 1)(_hip.SgnnMatrix(a["in_"], P, a["ld"], 4, a["rows"], 4))
+    cols = 4 if a["nws"] == 1 << 30 and a["ws"] else 400   # 4 x 4 needs no workspace
+    a["rows"] = 400 if cols == 400 else a["rows"]
+    mats = (_hip.SgnnMatrix * 1)(_hip.SgnnMatrix(a["in_"], P, max(a["ld"], cols) if cols == 400 else a["ld"], cols, a["rows"], cols))
     assert lib.sgnn_newton_schulz(a["dtype"], None if a["null"] else mats, a["count"], a["steps"], 1.0, 0.0, 0.0,
-                                  a["eps"], P, a["nws"], None) == INVALID
+                                  a["eps"], a["ws"], a["nws"], None) == INVALID
     assert "newton_schulz" in lib.sgnn_last_error().decode()
 
 
