@@ -309,11 +309,12 @@ struct NormCut {
   }
 };
 
-// Workgroups of the backward pass, which are also the partial sums: enough for the memory's rate (8 of 256 threads
-// per CU for short rows; 2 for long ones, whose partial rows are as long), never more than there are rows for.
-int64_t bwd_blocks(const NormCut& cut, int64_t n) {
+// Workgroups of the backward pass, which are also the partial sums: as many as the registers of 4, 8 or 16 values per
+// lane let reside at once, never more than there are rows for.
+int64_t bwd_blocks(const NormCut& cut, size_t size, int64_t n) {
   const int64_t groups = cut.G == 0 || cut.G > 256 ? 1 : 256 / cut.G;
-  const int64_t most = cut.G == 16 ? 2048 : cut.G <= 256 ? 1024 : 512;
+  const int values = cut.NC * 16 / (int)size;
+  const int64_t most = 256 * (cut.G == 0 ? 2 : cut.G > 256 ? (values <= 4 ? 3 : values <= 8 ? 2 : 1) : values <= 4 ? 8 : values <= 8 ? 5 : 3);
   return std::max<int64_t>(1, std::min(most, (n + groups - 1) / groups));
 }
 
@@ -377,7 +378,7 @@ extern "C" int sgnn_norm(int32_t dtype, int32_t wdtype, const void* x, int64_t l
 
 extern "C" size_t sgnn_norm_bwd_workspace_bytes(int64_t n, int32_t width) {
   if (n <= 0 || width <= 0) return 0;
-  const auto blocks = [&](size_t size) { return bwd_blocks(NormCut(size, width), n); };
+  const auto blocks = [&](size_t size) { return bwd_blocks(NormCut(size, width), size, n); };
   return sizeof(float) * 2 * (size_t)width * (size_t)std::max(blocks(2), blocks(4));
 }
 
@@ -401,7 +402,7 @@ extern "C" int sgnn_norm_bwd(int32_t dtype, int32_t wdtype, const void* dy, int6
     using T = std::remove_pointer_t<decltype(t)>;
     using W = std::remove_pointer_t<decltype(w)>;
     const NormCut cut(sizeof(T), width);
-    const int64_t nblk = n > 0 ? bwd_blocks(cut, n) : 0;
+    const int64_t nblk = n > 0 ? bwd_blocks(cut, sizeof(T), n) : 0;
     const T *up = static_cast<const T*>(dy), *in = static_cast<const T*>(x);
     const W* ga = static_cast<const W*>(gamma);
     T* out = static_cast<T*>(dx);
