@@ -155,7 +155,9 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 // longer than memory; the small tile has four.
 // 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 292
 // to 330 us, dz w 230 to 260, dz^T x 234 to 260.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
-// time, and the rest is the two barriers' waits per block and, forward, the epilogue's 268 MB.
+// time, and the rest is LDS's latency after each block's barrier, which all waves meet together, and, forward, the
+// epilogue's 268 MB.  Memory is not waited for: four stages of 32 k took 334 / 248 / 244 us at their fastest, where these
+// two of 64 k took 290 / 230 / 230; the next block's loads issued behind the first fragments' reads took 292 / 226 / 237.
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT, int NST>
 __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   constexpr int BK = 64, kThreads = 64 * WM * WN;

@@ -7,9 +7,9 @@ using namespace sgnn;
 
 // Rows are held in registers: G lanes per row (16, 64, or a workgroup of 256 or 512), NC 16-byte pieces per lane,
 // piece j of lane i at column (j G + i) V.  Forward and backward read every input once and write every output once:
-// both are bounded by memory, where a copy reaches 6.2 TB/s: 200003 x 128 fp32 34 us forward (6.0 TB/s) and 53 + 6
-// backward (5.8); 16384 x 4096 bf16 51 us (5.3) and 89 + 11 (4.5: two barriers a row, and gamma and the sums hold the
-// registers that a second row in flight would need).
+// both are bounded by memory, where a copy reaches 6.2 TB/s: 200003 x 128 fp32 34 us forward (6.0 TB/s) and 52 + 5
+// backward (5.9); 16384 x 4096 bf16 52 us (5.2) and 84 + 9 (4.8: gamma and the sums hold the registers that another row
+// in flight would need, and every row has its barrier).
 constexpr int threads_of(int G) { return G > 256 ? G : 256; }
 
 // Sum over a row's G lanes; `red` is 2 x 16 floats of LDS, `turn` the half to use (the other may still be read).
@@ -310,7 +310,8 @@ struct NormCut {
 };
 
 // Workgroups of the backward pass, which are also the partial sums: as many as the registers of 4, 8 or 16 values per
-// lane let reside at once, never more than there are rows for.
+// lane let reside at once, never more than there are rows for (1024 and 2048 before, where a second round of fewer
+// workgroups followed: 16384 x 4096 bf16 88 + 12 us, 50000 x 1024 bf16 69 us in all against 60).
 int64_t bwd_blocks(const NormCut& cut, size_t size, int64_t n) {
   const int64_t groups = cut.G == 0 || cut.G > 256 ? 1 : 256 / cut.G;
   const int values = cut.NC * 16 / (int)size;
