@@ -600,9 +600,8 @@ typedef struct sgnn_matrix {
  * in / |in|_F goes through s <- a s + b s^3 + c s^5, which for (3.4445, -4.7750, 2.0315) brings it near 1 in
  * five steps (the update of the Muon optimiser).  `mats` is a HOST array of `count` matrices of any shapes
  * (read during the call only); matrices of one shape that stand next to each other share their launches.
- * Zero matrices give zeros.  Products: of fp32 and fp16 matrices to 22 bits of every operand, of bf16 ones to 11;
- * sums in fp32.  X and its polynomials must stay below 63 in magnitude (the quintic above keeps them below 4); past
- * that they become infinite.
+ * Zero matrices give zeros.  Products to 22 bits of every operand, whatever the type; sums in fp32.  X and its polynomials must
+ * stay below 63 in magnitude (the quintic above keeps them below 4); past that they become infinite.
  * workspace: sgnn_newton_schulz_workspace_bytes(mats, count) bytes (reads the shapes alone), 256-B aligned. */
 size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, int32_t count);
 int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_t count, int32_t steps, float a, float b,

@@ -1,19 +1,21 @@
 // sgnn_newton_schulz (include/sgnn.h): X = in / (|in|_F + eps), then X <- Q X, Q = a I + b G + c G^2, G = X X^T.
 //
 // A matrix taller than wide takes the same steps from its other side, X <- X Q with G = X^T X: no transposition.
-// X, G and Q are kept as fp16 planes of the value times 2^10; the singular values of X stay below 1.3, so that all of
-// them fit.  fp32 and fp16 matrices have two planes, hi + lo, 22 bits of every value that is not tiny against 1 and an
-// absolute 2^-35 below that, and products hi hi + hi lo + lo hi: good to 2^-22, below what an fp32 sum of some hundred
-// products loses.  bf16 matrices have the hi plane alone, a third of the instructions: its 11 bits are 3 more than
-// their elements have, and a I inside Q keeps the sum a X + (b G + c G^2) X, whose terms cancel to a fifth near 1,
-// out of the rounding.  The planes are padded with zeros to whole tiles (zeros stay zeros under the steps), so nothing
-// is checked inside the products; the last one writes the caller's type from its fp32 sums.
+// X, G and Q are kept as two fp16 planes, hi + lo, of the value times 2^10; the singular values of X stay below 1.3, so
+// that all of them fit: 22 bits of every value that is not tiny against 1 and an absolute 2^-35 below that.  Products
+// are hi hi + hi lo + lo hi, good to 2^-22, below what an fp32 sum of some hundred products loses, and a I inside Q
+// keeps the sum a X + (b G + c G^2) X, whose terms cancel to a fifth near 1, out of the rounding.  This holds for every
+// type of matrix: with the hi plane alone bf16 ones took 537 us instead of 1244 (4096 x 2048), but fifteen roundings to
+// 11 bits come out beside the one of the result (error 0.0028 instead of 0.0017 for a small matrix).  The planes are
+// padded with zeros to whole tiles (zeros stay zeros under the steps), so nothing is checked inside the products; the
+// last one writes the caller's type from its fp32 sums.
 #include "gemm_tile.h"
 
 namespace {
 using namespace sgnn;
 
 constexpr float kScale = 1024.0f, kInvScale = 1.0f / 1024.0f;
+constexpr int kPlanes = 2;     // hi, lo
 constexpr int kMaxGroup = 32;  // matrices of one shape per launch (their pointers are kernel arguments)
 constexpr int kNormParts = 256; // partial sums of squares per matrix, at most
 
@@ -64,7 +66,6 @@ __global__ __launch_bounds__(256) void k_ns_norm(Group g, double* part) {
 }
 
 // Eight values times scale into the planes, at a 16-byte address.
-template <int P>
 SGNN_DEV void put_planes(f16_t* p, int64_t plane, const float* v, float scale) {
   typedef f16_t h8 __attribute__((ext_vector_type(8)));
   h8 hi, lo;
@@ -75,12 +76,12 @@ SGNN_DEV void put_planes(f16_t* p, int64_t plane, const float* v, float scale) {
     hi[i] = h, lo[i] = (f16_t)(x - (float)h);
   }
   *reinterpret_cast<h8*>(p) = hi;
-  if constexpr (P == 2) *reinterpret_cast<h8*>(p + plane) = lo;
+  *reinterpret_cast<h8*>(p + plane) = lo;
 }
 
 // The planes of in / (|in|_F + eps), zero in the padding; one thread per 8 columns.  Without steps (x null) the
 // values go to out.
-template <typename T, int P>
+template <typename T>
 __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, int nparts, float eps, f16_t* x,
                                                   int64_t plane, int64_t batch, int64_t ld, int64_t rows_padded) {
   __shared__ double red[4];
@@ -102,7 +103,7 @@ __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, i
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = norm == 0.0f ? 0.0f : v[i] / norm;  // only zeros have the norm 0
     if (x)
-      put_planes<P>(x + b * batch + r * ld + c, plane, v, kScale);
+      put_planes(x + b * batch + r * ld + c, plane, v, kScale);
     else if (there)
       store_some<8>(static_cast<T*>(g.out[b]) + r * g.ld_out[b] + c, (int)(g.cols - c), v);
   }
@@ -118,15 +119,15 @@ struct NsGemm {
   Group last;
 };
 
-// BT x BT outputs by four waves.  P planes per operand (1: hi alone).  SYM: the product is symmetric; only the tiles
+// BT x BT outputs by four waves.  SYM: the product is symmetric; only the tiles
 // on and above the diagonal are formed and each is written to both sides.
 // KG groups of four waves take every KG-th block of k each, with LDS of their own, and are added in order at the end:
 // these products have few tiles (36 of 128 x 128 in the triangle of 1024), and one wave per SIMD leaves memory's and
 // LDS's latencies in the open.  bf16, 2048 x 4096: X X^T 38 us (136 tiles of 256 CUs; 18 GFLOP formed), G^2 26 us, Q X
 // 43 us (34 GFLOP, 800 TFLOP/s): bounded by the CUs without a tile and by LDS reads beside the matrix instructions.
-template <int P, bool AC, bool BC, int BT, bool SYM, int KG>
+template <bool AC, bool BC, int BT, bool SYM, int KG>
 __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
-  constexpr int BK = 64 / P, kThreads = 256, TT = BT / 2 / 16;
+  constexpr int P = kPlanes, BK = 32, kThreads = 256, TT = BT / 2 / 16;
   using TA = Tile16<BT, BK, AC>;
   using TB = Tile16<BT, BK, BC>;
   constexpr int kStage = 2 * P * TA::kBytes;
@@ -176,33 +177,26 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
     if (blk + KG < blocks) stage(lds + ((round & 1) ^ 1) * kStage, blk + KG);
     if (blk >= blocks) continue;
     const char* here = lds + (round & 1) * kStage;
+    s16x8 fa[P][TT], fb[P][TT];
 #pragma unroll
-    for (int kk = 0; kk < BK / 32; ++kk) {
-      s16x8 fa[P][TT], fb[P][TT];
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-      for (int p = 0; p < P; ++p)
-#pragma unroll
-        for (int i = 0; i < TT; ++i) {
-          fa[p][i] = TA::frag(here + p * TA::kBytes, (wm * TT + i) * 16, kk);
-          fb[p][i] = TB::frag(here + (P + p) * TA::kBytes, (wn * TT + i) * 16, kk);
-        }
-      if constexpr (P == 2) {
-#pragma unroll
-        for (int i = 0; i < TT; ++i)
-#pragma unroll
-          for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
-#pragma unroll
-        for (int i = 0; i < TT; ++i)
-#pragma unroll
-          for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
+      for (int i = 0; i < TT; ++i) {
+        fa[p][i] = TA::frag(here + p * TA::kBytes, (wm * TT + i) * 16, 0);
+        fb[p][i] = TB::frag(here + (P + p) * TA::kBytes, (wn * TT + i) * 16, 0);
       }
 #pragma unroll
-      for (int i = 0; i < TT; ++i)
+    for (int i = 0; i < TT; ++i)
 #pragma unroll
-        for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
-    }
-    // one workgroup per CU only: where two share it they hide each other's reads (42 us without, 44 with)
-    if constexpr (P == 1 && TT == 4 && KG > 1) order_products<TT, TT, AC ? 2 : 1, BC ? 2 : 1>();
+      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
+#pragma unroll
+    for (int i = 0; i < TT; ++i)
+#pragma unroll
+      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
   }
   __syncthreads();
   if constexpr (KG > 1) {
@@ -246,23 +240,23 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
         if (R) {
           float hi[8], lo[8];
           load_vec(R + at, hi);
-          if constexpr (P == 2) load_vec(R + g.plane_c + at, lo);
+          load_vec(R + g.plane_c + at, lo);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            v[e] += g.beta * kInvScale * (P == 2 ? hi[e] + lo[e] : hi[e]);
+            v[e] += g.beta * kInvScale * (hi[e] + lo[e]);
             if (n + e == m) v[e] += g.diag;
           }
         }
         // the values back into the buffer for the mirrored tile
         *reinterpret_cast<f32x4*>(at0) = f32x4{v[0], v[1], v[2], v[3]};
         *reinterpret_cast<f32x4*>(at1) = f32x4{v[4], v[5], v[6], v[7]};
-        put_planes<P>(C + at, g.plane_c, v, kScale);
+        put_planes(C + at, g.plane_c, v, kScale);
       } else if (g.last_dtype < 0) {
-        put_planes<P>(C + at, g.plane_c, v, kScale);
+        put_planes(C + at, g.plane_c, v, kScale);
       } else if (m < g.last.rows && n < g.last.cols) {
         const int64_t to = m * g.last.ld_out[b] + n;
         const int cnt = (int)(g.last.cols - n);
-        if constexpr (P == 1) store_some<8>(static_cast<bf16_t*>(g.last.out[b]) + to, cnt, v);
+        if (g.last_dtype == SGNN_BF16) store_some<8>(static_cast<bf16_t*>(g.last.out[b]) + to, cnt, v);
         else if (g.last_dtype == SGNN_F32) store_some<8>(static_cast<float*>(g.last.out[b]) + to, cnt, v);
         else store_some<8>(static_cast<f16_t*>(g.last.out[b]) + to, cnt, v);
       }
@@ -279,7 +273,7 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
             const int r = r0 + e;
             v[e] = buf[r * 16 * TT + ((n >> 2) ^ (r & kMask)) * 4 + (n & 3)];
           }
-          put_planes<P>(C + (ni + n) * g.ldc + mi + r0, g.plane_c, v, kScale);
+          put_planes(C + (ni + n) * g.ldc + mi + r0, g.plane_c, v, kScale);
         }
         __builtin_amdgcn_wave_barrier();
       }
@@ -293,15 +287,15 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
 // one of 136 tiles 38 and 45.  Neither the batch nor the tile's size decides, so a matrix gets the same bits in any batch.
 constexpr int kFewTiles = 256;
 
-template <int P, bool AC, bool BC, bool SYM>
+template <bool AC, bool BC, bool SYM>
 void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
   const auto tiles = [&](int m, int n) { return SYM ? m * (m + 1) / 2 : m * n; };
   const dim3 grid((unsigned)tiles(g.tiles_m, g.tiles_n), 1, (unsigned)count);
   const int per = 128 / bt;
   const bool few = tiles((g.tiles_m + per - 1) / per, (g.tiles_n + per - 1) / per) <= kFewTiles;
   const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g); };
-  if (bt == 128) few ? go(k_ns_gemm<P, AC, BC, 128, SYM, 2>, 512) : go(k_ns_gemm<P, AC, BC, 128, SYM, 1>, 256);
-  else few ? go(k_ns_gemm<P, AC, BC, 64, SYM, 2>, 512) : go(k_ns_gemm<P, AC, BC, 64, SYM, 1>, 256);
+  if (bt == 128) few ? go(k_ns_gemm<AC, BC, 128, SYM, 2>, 512) : go(k_ns_gemm<AC, BC, 128, SYM, 1>, 256);
+  else few ? go(k_ns_gemm<AC, BC, 64, SYM, 2>, 512) : go(k_ns_gemm<AC, BC, 64, SYM, 1>, 256);
 }
 
 // ----------------------------------------------------------------------------- small matrices
@@ -317,20 +311,20 @@ struct SmallArgs {
 };
 
 inline int pad32(int v) { return (v + 31) & ~31; }
-inline size_t small_lds(int planes, int rows, int cols) {
+inline size_t small_lds(int rows, int cols) {
   const size_t m = pad32(std::min(rows, cols)), n = pad32(std::max(rows, cols));
-  return 2 * (size_t)planes * m * ((n + 8) + (m + 8));
+  return 2 * (size_t)kPlanes * m * ((n + 8) + (m + 8));
 }
 inline int small_blocks(int rows, int cols) { return pad32(std::min(rows, cols)) / 32 * (pad32(std::max(rows, cols)) / 32); }
 // A short side of 128 fills the waves with blocks of 64 x 32, which read a quarter less of LDS than those of 32 x 32.
 inline bool full_side(int rows, int cols) { return pad32(std::min(rows, cols)) == 128; }
-inline bool small_ok(int planes, int rows, int cols) {
+inline bool small_ok(int rows, int cols) {
   return std::min(rows, cols) <= 128 && std::max(rows, cols) <= 4096 && small_blocks(rows, cols) <= 6 * kSmallWaves &&
-         small_lds(planes, rows, cols) <= kMaxLds;
+         small_lds(rows, cols) <= kMaxLds;
 }
 
 // acc = the 16 BI x 32 block (a0, b0) of A B^T, A's rows from LDS, B's from LDS (BT: its columns), over K.
-template <int P, bool BT, int BI>
+template <bool BT, int BI>
 SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane_a, const char* B, int ldb, int plane_b,
                           int a0, int b0, int K) {
   const int l = lane_id();
@@ -338,6 +332,7 @@ SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane
   for (int i = 0; i < BI; ++i)
 #pragma unroll
     for (int j = 0; j < 2; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  constexpr int P = kPlanes;
   s16x8 fa[2][P][BI], fb[2][P][2];
   const auto load = [&](int h, int k0) {
 #pragma unroll
@@ -359,16 +354,14 @@ SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane
     }
   };
   const auto multiply = [&](int h) {
-    if constexpr (P == 2) {
 #pragma unroll
-      for (int i = 0; i < BI; ++i)
+    for (int i = 0; i < BI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][1][j], fa[h][0][i], acc[i][j]);
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][1][j], fa[h][0][i], acc[i][j]);
 #pragma unroll
-      for (int i = 0; i < BI; ++i)
+    for (int i = 0; i < BI; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][1][i], acc[i][j]);
-    }
+      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][1][i], acc[i][j]);
 #pragma unroll
     for (int i = 0; i < BI; ++i)
 #pragma unroll
@@ -386,7 +379,7 @@ SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane
 }
 
 // The block's values times scale into planes of LDS.
-template <int P, int BI>
+template <int BI>
 SGNN_DEV void small_put(char* C, int ldc, int plane, const f32x4 (&acc)[BI][2], int a0, int b0, float scale) {
   typedef f16_t h4 __attribute__((ext_vector_type(4)));
   const int l = lane_id();
@@ -403,7 +396,7 @@ SGNN_DEV void small_put(char* C, int ldc, int plane, const f32x4 (&acc)[BI][2], 
       }
       char* at = C + 2 * ((a0 + 16 * i + (l & 15)) * ldc + b0 + 16 * j + 4 * (l >> 4));
       *reinterpret_cast<h4*>(at) = hi;
-      if constexpr (P == 2) *reinterpret_cast<h4*>(at + plane) = lo;
+      *reinterpret_cast<h4*>(at + plane) = lo;
     }
 }
 
@@ -418,13 +411,13 @@ SGNN_DEV int block_of(int w, int q) {
 constexpr float kDown = kInvScale * kInvScale;  // of a product of two scaled planes
 
 // The planes of Q = ca I + cb G + cc G^2 into LDS at G, from this wave's blocks g of kScale^2 G.
-template <int P, int NG, int BI>
+template <int NG, int BI>
 SGNN_DEV void small_poly(f32x4 (&g)[NG][BI][2], char* G, int ldg, int plane_g, int m, float ca, float cb, float cc) {
   const int l = lane_id(), w = wave_id(), mb = m / (16 * BI), gblocks = mb * (m / 32);
 #pragma unroll
   for (int q = 0; q < NG; ++q) {
     const int b = block_of(w, q);
-    if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
+    if (b < gblocks) small_put(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
   }
   __syncthreads();
 #pragma unroll
@@ -433,7 +426,7 @@ SGNN_DEV void small_poly(f32x4 (&g)[NG][BI][2], char* G, int ldg, int plane_g, i
     if (b < gblocks) {
       f32x4 h[BI][2];
       const int a0 = b % mb * 16 * BI, b0 = b / mb * 32;
-      small_block<P, false>(h, G, ldg, plane_g, G, ldg, plane_g, a0, b0, m);
+      small_block<false>(h, G, ldg, plane_g, G, ldg, plane_g, a0, b0, m);
 #pragma unroll
       for (int i = 0; i < BI; ++i)
 #pragma unroll
@@ -449,7 +442,7 @@ SGNN_DEV void small_poly(f32x4 (&g)[NG][BI][2], char* G, int ldg, int plane_g, i
 #pragma unroll
   for (int q = 0; q < NG; ++q) {
     const int b = block_of(w, q);
-    if (b < gblocks) small_put<P>(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kScale);
+    if (b < gblocks) small_put(G, ldg, plane_g, g[q], b % mb * 16 * BI, b / mb * 32, kScale);
   }
   __syncthreads();
 }
@@ -475,12 +468,12 @@ SGNN_DEV void small_out(const f32x4 (&x)[BI][2], T* out, int64_t ld, int rows, i
     }
 }
 
-template <typename T, int P, int NB, int BI>
+template <typename T, int NB, int BI>
 __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int steps, float ca, float cb, float cc,
                                                             float eps) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ double red[kSmallWaves];
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), P = kPlanes;
   const sgnn_matrix& mat = args.mats[blockIdx.x];
   const bool tall = mat.rows > mat.cols;
   const int m = (min(mat.rows, mat.cols) + 31) & ~31, n = (max(mat.rows, mat.cols) + 31) & ~31;
@@ -508,7 +501,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
       char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
       const uint32_t bits = __builtin_bit_cast(uint32_t, v[e]);
       *reinterpret_cast<uint16_t*>(at) = bits >> 16;
-      if constexpr (P == 2) *reinterpret_cast<uint16_t*>(at + plane_x) = bits;
+      *reinterpret_cast<uint16_t*>(at + plane_x) = bits;
     }
   }
 #pragma unroll
@@ -521,8 +514,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
   const float norm = (float)sqrt(s) + eps;
   // the bits into the planes of the value / norm
   for (int t = threadIdx.x; t < plane_x / 16; t += kSmallThreads) {
-    u32x4 hi = *reinterpret_cast<u32x4*>(X + 16 * t), lo = {0, 0, 0, 0};
-    if constexpr (P == 2) lo = *reinterpret_cast<u32x4*>(X + plane_x + 16 * t);
+    const u32x4 hi = *reinterpret_cast<u32x4*>(X + 16 * t), lo = *reinterpret_cast<u32x4*>(X + plane_x + 16 * t);
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -530,7 +522,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
       const float x = __builtin_bit_cast(float, up | low);
       v[e] = norm == 0.0f ? 0.0f : x / norm;
     }
-    put_planes<P>(reinterpret_cast<f16_t*>(X + 16 * t), plane_x / 2, v, kScale);
+    put_planes(reinterpret_cast<f16_t*>(X + 16 * t), plane_x / 2, v, kScale);
   }
   __syncthreads();
 
@@ -539,7 +531,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
     for (int t = threadIdx.x; t < mat.rows * mat.cols; t += kSmallThreads) {
       const int r = t / mat.cols, c = t - r * mat.cols;
       const f16_t* at = reinterpret_cast<const f16_t*>(X) + (tall ? c * ldx + r : r * ldx + c);
-      out[(int64_t)r * mat.ld_out + c] = from_float<T>((to_float(at[0]) + (P == 2 ? to_float(at[plane_x / 2]) : 0.0f)) * kInvScale);
+      out[(int64_t)r * mat.ld_out + c] = from_float<T>((to_float(at[0]) + to_float(at[plane_x / 2])) * kInvScale);
     }
   }
   constexpr int NG = 4 / BI, NX = 2 * NB / BI;
@@ -549,13 +541,13 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const int b = block_of(w, q);
-      if (b < gblocks) small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, n);
+      if (b < gblocks) small_block<false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, n);
     }
-    small_poly<P>(g, G, ldg, plane_g, m, ca, cb, cc);
+    small_poly(g, G, ldg, plane_g, m, ca, cb, cc);
 #pragma unroll
     for (int q = 0; q < NX; ++q) {
       const int b = block_of(w, q);
-      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
+      if (b < xblocks) small_block<true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
     }
     __syncthreads();
 #pragma unroll
@@ -563,7 +555,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
       const int b = block_of(w, q);
       if (b >= xblocks) continue;
       const int r0 = b % mb * 16 * BI, c0 = b / mb * 32;
-      if (step + 1 < steps) small_put<P>(X, ldx, plane_x, x[q], r0, c0, kInvScale);
+      if (step + 1 < steps) small_put(X, ldx, plane_x, x[q], r0, c0, kInvScale);
       else small_out<T>(x[q], static_cast<T*>(mat.out), mat.ld_out, mat.rows, mat.cols, tall, r0, c0);
     }
     __syncthreads();
@@ -572,13 +564,12 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
 
 template <typename T>
 int launch_small(const sgnn_matrix* mats, int count, int32_t steps, float a, float b, float c, float eps, hipStream_t s) {
-  constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
   SmallArgs args;
   size_t bytes = 0;
   int blocks = 0;
   for (int i = 0; i < count; ++i) {
     args.mats[i] = mats[i];
-    bytes = std::max(bytes, small_lds(P, mats[i].rows, mats[i].cols));
+    bytes = std::max(bytes, small_lds(mats[i].rows, mats[i].cols));
     blocks = std::max(blocks, small_blocks(mats[i].rows, mats[i].cols));
   }
   const auto go = [&](auto kernel) {
@@ -590,8 +581,8 @@ int launch_small(const sgnn_matrix* mats, int count, int32_t steps, float a, flo
     return check_launch("newton_schulz");
   };
   if (full_side(mats[0].rows, mats[0].cols))
-    return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2, 4>) : go(k_ns_small<T, P, 6, 4>);
-  return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, P, 2, 2>) : go(k_ns_small<T, P, 6, 2>);
+    return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, 2, 4>) : go(k_ns_small<T, 6, 4>);
+  return blocks <= 2 * kSmallWaves ? go(k_ns_small<T, 2, 2>) : go(k_ns_small<T, 6, 2>);
 }
 
 // ----------------------------------------------------------------------------- short and long matrices
@@ -606,7 +597,7 @@ inline bool chunk_ok(int rows, int cols) {
   return std::min(rows, cols) <= 128 && std::max(rows, cols) <= kChunk * kMaxChunks;
 }
 inline int chunks_of(int rows, int cols) { return (std::max(rows, cols) + kChunk - 1) / kChunk; }
-inline size_t chunk_lds(int planes, int m) { return 2 * (size_t)planes * m * ((kChunk + 8) + (m + 8)); }
+inline size_t chunk_lds(int m) { return 2 * (size_t)kPlanes * m * ((kChunk + 8) + (m + 8)); }
 
 struct ChunkArgs {
   const double* norms;
@@ -618,11 +609,11 @@ struct ChunkArgs {
   float ca, cb, cc, eps;
 };
 
-template <typename T, int P, int BI>
+template <typename T, int BI>
 __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ double red[kSmallWaves];
-  constexpr int V = 16 / sizeof(T);
+  constexpr int V = 16 / sizeof(T), P = kPlanes;
   const int l = lane_id(), w = wave_id(), mat = blockIdx.y, c0 = blockIdx.x * kChunk;
   constexpr int NG = 4 / BI;
   const int m = a.m, mb = m / (16 * BI), gblocks = mb * (m / 32), xblocks = mb * (kChunk / 32);
@@ -662,12 +653,12 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
         if (r < m) *reinterpret_cast<u32x4*>(X + p * plane_x + 2 * (r * ldx + c)) = px[p][i];
     }
     __syncthreads();
-    small_poly<P>(g, G, ldg, plane_g, m, a.ca, a.cb, a.cc);
+    small_poly(g, G, ldg, plane_g, m, a.ca, a.cb, a.cc);
     f32x4 x[NG][BI][2];
 #pragma unroll
     for (int q = 0; q < NG; ++q) {
       const int b = block_of(w, q);
-      if (b < xblocks) small_block<P, true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
+      if (b < xblocks) small_block<true>(x[q], G, ldg, plane_g, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, m);
     }
     __syncthreads();
 #pragma unroll
@@ -675,7 +666,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
       const int b = block_of(w, q);
       if (b >= xblocks) continue;
       if (a.to)
-        small_put<P>(X, ldx, plane_x, x[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
+        small_put(X, ldx, plane_x, x[q], b % mb * 16 * BI, b / mb * 32, kInvScale);
       else
         small_out<T>(x[q], static_cast<T*>(grp.out[mat]), grp.ld_out[mat], grp.rows, grp.cols, tall, b % mb * 16 * BI,
                      c0 + b / mb * 32);
@@ -719,7 +710,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
           const float y = (norm == 0.0f ? 0.0f : v[e] / norm) * kScale;
           const f16_t h = (f16_t)y;
           *reinterpret_cast<f16_t*>(at) = h;
-          if constexpr (P == 2) *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);
+          *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);
         }
       }
     }
@@ -737,7 +728,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
   for (int q = 0; q < NG; ++q) {
     const int b = block_of(w, q);
     if (b >= gblocks) continue;
-    small_block<P, false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, kChunk);
+    small_block<false>(g[q], X, ldx, plane_x, X, ldx, plane_x, b % mb * 16 * BI, b / mb * 32, kChunk);
 #pragma unroll
     for (int i = 0; i < 2 * BI; ++i) to[(int64_t)b * 128 * BI + 64 * i] = g[q][i >> 1][i & 1];
   }
@@ -786,11 +777,10 @@ unsigned blocks_for(int64_t items, int64_t most) {
 
 template <typename T>
 int by_chunks(const Group& grp, int32_t steps, float a, float b, float c, float eps, char* ws, hipStream_t s) {
-  constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
   const ChunkLayout at(grp.rows, grp.cols, grp.count);
   double* norms = reinterpret_cast<double*>(ws);
   float *from = reinterpret_cast<float*>(ws + at.norms + at.x), *to = reinterpret_cast<float*>(ws + at.norms + at.x + at.share);
-  const size_t lds = chunk_lds(P, at.m);
+  const size_t lds = chunk_lds(at.m);
   ChunkArgs g{norms, reinterpret_cast<f16_t*>(ws + at.norms), nullptr, to, (int64_t)at.m * at.ld * grp.count,
               (int32_t)blocks_for((int64_t)grp.rows * grp.cols / 16, kNormParts), at.m, at.ld, a, b, c, eps};
   hipLaunchKernelGGL(k_ns_norm<T>, dim3((unsigned)g.nparts, grp.count), dim3(256), 0, s, grp, norms);
@@ -805,16 +795,15 @@ int by_chunks(const Group& grp, int32_t steps, float a, float b, float c, float 
     }
     return check_launch("newton_schulz");
   };
-  return full_side(grp.rows, grp.cols) ? go(k_ns_chunk<T, P, 4>) : go(k_ns_chunk<T, P, 2>);
+  return full_side(grp.rows, grp.cols) ? go(k_ns_chunk<T, 4>) : go(k_ns_chunk<T, 2>);
 }
 
-// The matrices from i on that share a launch: small ones of any shape, or large ones of one shape.  planes 1 (bf16) makes
-// more of them small than 2; the workspace is sized by 2.
-int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i, int planes) {
+// The matrices from i on that share a launch: small ones of any shape, or large ones of one shape.
+int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i) {
   int32_t n = 1;
-  if (small_ok(planes, mats[i].rows, mats[i].cols)) {
+  if (small_ok(mats[i].rows, mats[i].cols)) {
     while (i + n < count && n < kMaxSmall && mats[i + n].rows > 0 && mats[i + n].cols > 0 &&
-           small_ok(planes, mats[i + n].rows, mats[i + n].cols) &&
+           small_ok(mats[i + n].rows, mats[i + n].cols) &&
            full_side(mats[i + n].rows, mats[i + n].cols) == full_side(mats[i].rows, mats[i].cols))
       ++n;
     return n;
@@ -836,8 +825,7 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
   const int64_t batch_g = at.side * at.side, plane_g = batch_g * grp.count;
   const int parts = (int)blocks_for((int64_t)grp.rows * grp.cols / 16, kNormParts);
   hipLaunchKernelGGL(k_ns_norm<T>, dim3(parts, grp.count), dim3(256), 0, s, grp, norms);
-  constexpr int P = std::is_same_v<T, bf16_t> ? 1 : 2;
-  hipLaunchKernelGGL((k_ns_begin<T, P>), dim3(blocks_for(batch_x / 8, 4096), grp.count), dim3(256), 0, s, grp, norms, parts,
+  hipLaunchKernelGGL(k_ns_begin<T>, dim3(blocks_for(batch_x / 8, 4096), grp.count), dim3(256), 0, s, grp, norms, parts,
                      eps, steps > 0 ? x : nullptr, plane_x, batch_x, at.cols, at.rows);
   for (int32_t k = 0; k < steps; ++k) {
     NsGemm g{};
@@ -847,13 +835,13 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
     g.C = gram, g.ldc = at.side, g.plane_c = plane_g, g.batch_c = batch_g;
     g.alpha = 1.0f;
     g.K = (int32_t)(tall ? at.rows : at.cols);
-    if (tall) launch_gemm<P, true, true, true>(g, at.bt, grp.count, s);
-    else launch_gemm<P, false, false, true>(g, at.bt, grp.count, s);
+    if (tall) launch_gemm<true, true, true>(g, at.bt, grp.count, s);
+    else launch_gemm<false, false, true>(g, at.bt, grp.count, s);
     g.A = g.B = g.R = gram, g.lda = g.ldb = at.side, g.plane_a = g.plane_b = plane_g, g.batch_a = g.batch_b = batch_g;
     g.C = poly;
     g.alpha = c, g.beta = b, g.diag = a;
     g.K = (int32_t)at.side;
-    launch_gemm<P, false, false, true>(g, at.bt, grp.count, s);
+    launch_gemm<false, false, true>(g, at.bt, grp.count, s);
     g.R = nullptr, g.C = next, g.ldc = at.cols, g.plane_c = plane_x, g.batch_c = batch_x;
     g.alpha = 1.0f;
     g.tiles_m = (int32_t)(at.rows / at.bt), g.tiles_n = (int32_t)(at.cols / at.bt);
@@ -864,11 +852,11 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
     if (tall) {  // X Q: Q is symmetric, its rows are its columns
       g.A = x, g.lda = at.cols, g.plane_a = plane_x, g.batch_a = batch_x;
       g.B = poly;
-      launch_gemm<P, false, false, false>(g, at.bt, grp.count, s);
+      launch_gemm<false, false, false>(g, at.bt, grp.count, s);
     } else {     // Q X
       g.A = poly;
       g.B = x, g.ldb = at.cols, g.plane_b = plane_x, g.batch_b = batch_x;
-      launch_gemm<P, false, true, false>(g, at.bt, grp.count, s);
+      launch_gemm<false, true, false>(g, at.bt, grp.count, s);
     }
     std::swap(x, next);
   }
@@ -879,8 +867,8 @@ void orthogonalise(const Group& grp, int32_t steps, float a, float b, float c, f
 extern "C" size_t sgnn_newton_schulz_workspace_bytes(const sgnn_matrix* mats, int32_t count) {
   size_t most = 0;
   for (int32_t i = 0, n; mats && i < count; i += n) {
-    n = run_of(mats, count, i, 2);
-    if (mats[i].rows > 0 && mats[i].cols > 0 && !small_ok(2, mats[i].rows, mats[i].cols))
+    n = run_of(mats, count, i);
+    if (mats[i].rows > 0 && mats[i].cols > 0 && !small_ok(mats[i].rows, mats[i].cols))
       most = std::max(most, group_bytes(mats[i].rows, mats[i].cols, n));
   }
   return most;
@@ -904,10 +892,9 @@ extern "C" int sgnn_newton_schulz(int32_t dtype, const sgnn_matrix* mats, int32_
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(SGNN_ERR_INVALID, "newton_schulz: workspace smaller than sgnn_newton_schulz_workspace_bytes");
   for (int32_t i = 0, n; i < count; i += n) {
-    const int planes = dtype == SGNN_BF16 ? 1 : 2;
-    n = run_of(mats, count, i, planes);
+    n = run_of(mats, count, i);
     if (mats[i].rows == 0 || mats[i].cols == 0) continue;
-    if (small_ok(planes, mats[i].rows, mats[i].cols)) {
+    if (small_ok(mats[i].rows, mats[i].cols)) {
       const int st = with_type(dtype, [&](auto* t) {
         return launch_small<std::remove_pointer_t<decltype(t)>>(mats + i, n, steps, a, b, c, eps,
                                                                 static_cast<hipStream_t>(stream));

@@ -495,6 +495,21 @@ def test_newton_schulz_of_a_batch_keeps_each_matrix_bits(dtype, count, m, n):
     assert muon.newton_schulz(again, out=again) is again and torch.equal(again, got)
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("m,n", [(16, 16), (30, 64), (64, 64), (128, 384), (100, 2047), (300, 260), (520, 1100)])
+def test_newton_schulz_rounds_16_bit_results_once(dtype, m, n):
+    """The steps lose no more than fp32 ones, so a 16-bit result is the rounding of a y off by at most d = fp32's ns_tol.
+    got is the nearest to y, so |got - y| <= |rounded(ref) - y|, and per element |got - ref| <= |got - y| + |y - ref|
+    <= |rounded(ref) - ref| + 2 |y - ref|."""
+    from sgnn_amd import muon
+    strong = normal((m, 4), 2) @ normal((4, n), 3)   # a few strong directions: the others start far below them
+    g = (0.02 * normal((m, n), 1) + 0.02 * strong).to(dtype)
+    ref = ns64(g)
+    once = float((ref.to(dtype).double() - ref).norm() / ref.norm())
+    err = float((muon.newton_schulz(g.cuda()).double().cpu() - ref).norm() / ref.norm())
+    assert err <= once + 2 * ns_tol(ref, torch.float32, m, n), (err, once)
+
+
 @pytest.mark.parametrize("m,n", [(5, 9), (128, 384), (300, 64), (100, 1500), (200, 260)])
 def test_newton_schulz_without_steps_normalises(m, n):
     """x / |x| kept to 2^-21 of itself or, where it is small, 2^-34 (two fp16 planes of 2^10 x)."""
