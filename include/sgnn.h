@@ -554,23 +554,21 @@ typedef enum sgnn_act {
 
 /* y[M][N] = act(z) (+ residual), z = x[M][K] w[N][K]^T (+ bias[N]): one nn.Linear of build_mlp
  * (graph_network.py:7-45) with its activation and the block's residual (:176) in the epilogue.
- * bias, residual and slope may be NULL.  slope (dense [M][N], elements of dtype's size) receives act'(z) for the
- * backward pass: fp32 for SGNN_F32; for the 16-bit types a fixed-point number of 16 bits, act'(z) to 2^-16, which is
- * 16 times finer than the type itself holds it.  K = 0 gives z = bias.  y and slope may overlap no input but that
- * residual may be y itself.
+ * bias, residual and slope may be NULL.  slope (dense [M][N] fp32, whatever dtype is) receives act'(z) for the
+ * backward pass.  K = 0 gives z = bias.  y and slope may overlap no input but that residual may be y itself.
  * workspace: sgnn_linear_workspace_bytes(dtype, M, N, K) bytes, 256-B aligned. */
 size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K);
 int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-                int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* slope, void* y,
+                int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, float* slope, void* y,
                 int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Its backward pass from dy [M][N]: dz = dy act'(z), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = sum_m dz
- * (all dense; NULL skips one; the residual's gradient is dy).  slope: as sgnn_linear wrote it for the same dtype;
- * NULL: act'(z) = 1 (SGNN_ACT_NONE).
+ * (all dense; NULL skips one; the residual's gradient is dy).  slope: as sgnn_linear wrote it; NULL:
+ * act'(z) = 1 (SGNN_ACT_NONE).
  * 16-bit types: dz is rounded once to the type before the two products, as their matrix instructions read it;
  * db sums the unrounded values.  M = 0 gives dw = db = 0.
  * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != NULL) bytes, 256-B aligned. */
 size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope);
-int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const void* slope,
+int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const float* slope,
                     const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw, void* db,
                     void* workspace, size_t workspace_bytes, void* stream);
 

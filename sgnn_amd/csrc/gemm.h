@@ -21,7 +21,7 @@ struct Gemm {
   int32_t act = 0;
   const void* res = nullptr;
   int64_t ldr = 0;
-  void* slope = nullptr;   // act'(sum + bias), dense [M][N] as sgnn_linear describes it
+  float* slope = nullptr;  // act'(sum + bias), dense [M][N] as sgnn_linear describes it
   void* C = nullptr;
   int64_t ldc = 0;
 };

@@ -20,7 +20,8 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 struct GemmArgs {
   const void *A, *B, *bias, *res;
-  void *slope, *C;
+  float* slope;
+  void* C;
   float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
   int64_t lda, ldb, ldr, ldc, M, N, K;
   int32_t act, nsplit, tiles_m, tiles_n;
@@ -33,7 +34,7 @@ SGNN_DEV void act_row(const GemmArgs& g, int64_t at, int cnt, float (&v)[V]) {
     float s[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) act_both<ACT, true, sizeof(T) == 2>(v[i], v[i], s[i]);
-    store_slopes<T>(g.slope, at, cnt, s);
+    store_some<V>(g.slope + at, cnt, s);
   } else {
     float unused;
 #pragma unroll

@@ -30,10 +30,10 @@ struct ActCut {
 // threads of one column in order.  Reads dy and the slopes, writes dz: bounded by memory (200003 x 128 fp32 52 us,
 // 5.9 TB/s; 8192 x 8192 bf16 84 us, 4.8 TB/s -- formed inside the two products instead, dz would be computed and its
 // inputs read twice, at every tile's pace).  Slopes rather than z are kept by the forward: it has the activation's
-// functions at hand, and this pass none.  For the 16-bit types they are fixed point of step 2^-15: half of bf16's or
-// fp16's own rounding of a slope near 1.
+// functions at hand, and this pass none.  They are fp32 for every type: in the tails of gelu and silu a slope is far below
+// 1, where fixed point of 16 bits leaves nothing of it.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const void* slope, int64_t M, int64_t N,
+__global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const float* slope, int64_t M, int64_t N,
                                                       int lanes, T* dz, float* partial) {
   constexpr int V = 16 / sizeof(T);
   __shared__ float sums[kThreads * V];
@@ -56,7 +56,7 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
         up[u] = u32x4{0, 0, 0, 0};
         if (r >= M) continue;
         up[u] = load_raw(dy + r * ldd + c, cnt);
-        if (slope) load_slopes<T>(slope, r * N + c, cnt, t[u]);
+        if (slope) load_some<V>(slope + r * N + c, cnt, t[u]);
       }
 #pragma unroll
       for (int u = 0; u < U; ++u) {
@@ -137,7 +137,7 @@ extern "C" size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t 
 }
 
 extern "C" int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-                           int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, void* slope,
+                           int64_t ldw, const void* bias, int32_t act, const void* residual, int64_t ldr, float* slope,
                            void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sgnn;
   if (!dtype_ok(dtype) || !act_ok(act)) return set_error(SGNN_ERR_INVALID, "linear: unknown dtype or activation");
@@ -163,7 +163,7 @@ extern "C" size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int6
 }
 
 extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd,
-                               const void* slope, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx,
+                               const float* slope, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx,
                                void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sgnn;
   if (!dtype_ok(dtype)) return set_error(SGNN_ERR_INVALID, "linear_bwd: unknown dtype");

@@ -216,46 +216,4 @@ SGNN_DEV void act_both(float z, float& value, float& slope) {
   }
 }
 
-// A slope in 16 bits: all of them lie in [-0.13, 1.13]; (slope + 1/4) 2^15 is a whole number below 2^16 - 1, which
-// marks a NaN.  0 and 1 are exact.
-SGNN_DEV uint16_t slope_to_bits(float s) { return s == s ? (uint16_t)rintf((s + 0.25f) * 32768.0f) : 0xffffu; }
-SGNN_DEV float slope_from_bits(uint16_t b) {
-  return b == 0xffffu ? __builtin_nanf("") : (float)b * (1.0f / 32768.0f) - 0.25f;
-}
-// V slopes (16 bytes of T's size) at any alignment.
-template <typename T, int V>
-SGNN_DEV void store_slopes(void* base, int64_t at, int cnt, const float (&s)[V]) {
-  if constexpr (sizeof(T) == 4) {
-    store_some<V>(static_cast<float*>(base) + at, cnt, s);
-  } else {
-    uint16_t* p = static_cast<uint16_t*>(base) + at;
-    if (cnt >= V) {
-      u32x4 t;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) t[i] = slope_to_bits(s[2 * i]) | (uint32_t)slope_to_bits(s[2 * i + 1]) << 16;
-      *reinterpret_cast<u32x4_any*>(p) = t;
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (i < cnt) p[i] = slope_to_bits(s[i]);
-    }
-  }
-}
-template <typename T, int V>
-SGNN_DEV void load_slopes(const void* base, int64_t at, int cnt, float (&s)[V]) {
-  if constexpr (sizeof(T) == 4) {
-    load_some<V>(static_cast<const float*>(base) + at, cnt, s);
-  } else {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    if (cnt >= V) {
-      const u32x4 t = *reinterpret_cast<const u32x4_any*>(p);
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = slope_from_bits((uint16_t)(t[i >> 1] >> (16 * (i & 1))));
-    } else {
-#pragma unroll
-      for (int i = 0; i < V; ++i) s[i] = i < cnt ? slope_from_bits(p[i]) : 0.0f;
-    }
-  }
-}
-
 }  // namespace sgnn

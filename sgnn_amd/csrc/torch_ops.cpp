@@ -145,13 +145,13 @@ std::pair<Tensor, Tensor> run_linear(const Tensor& x, const Tensor& w, const Ten
   const int64_t M = x.size(0), K = x.size(1), N = w.size(0);
   c10::DeviceGuard guard(x.device());
   Tensor y = at::empty({M, N}, x.options()), slope;
-  if (need_slope) slope = at::empty({M, N}, x.options());
+  if (need_slope) slope = at::empty({M, N}, x.options().dtype(at::kFloat));
   if (M && N) {
     const int32_t dt = dtype_of(x);
     const size_t nws = api.linear_bytes(dt, M, N, K);
     const Tensor ws = workspace(nws, x);
     check(api.linear(dt, M, N, K, ptr(x), ld(x), ptr(w), ld(w), ptr(bias), (int32_t)act, ptr(res), res.defined() ? ld(res) : 0,
-                     ptr(slope), ptr(y), N, ptr(ws), nws, stream_of(x)),
+                     slope.defined() ? slope.data_ptr<float>() : nullptr, ptr(y), N, ptr(ws), nws, stream_of(x)),
           "sgnn_linear");
   }
   return {y, slope};
@@ -183,7 +183,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
       const int32_t dt = dtype_of(x);
       const size_t nws = api.linear_bwd_bytes(dt, M, N, K, slope.defined());
       const Tensor ws = workspace(nws, x);
-      check(api.linear_bwd(dt, M, N, K, ptr(dy), ld(dy), ptr(slope), ptr(x), ld(x), ptr(w), ld(w), ptr(dx), ptr(dw),
+      check(api.linear_bwd(dt, M, N, K, ptr(dy), ld(dy), static_cast<const float*>(ptr(slope)), ptr(x), ld(x), ptr(w), ld(w), ptr(dx), ptr(dw),
                            ptr(db), ptr(ws), nws, stream_of(x)),
             "sgnn_linear_bwd");
     }

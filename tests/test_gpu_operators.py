@@ -151,6 +151,33 @@ def test_linear_against_64_bits(dtype, act, M, N, K):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("act,low,high", [("silu", -16.0, -8.0), ("gelu", -6.0, -4.0), ("gelu_tanh", -6.0, -4.0),
+                                          ("silu", 8.0, 16.0), ("gelu", 4.0, 6.0)])
+def test_linear_gradients_in_the_tails(dtype, act, low, high):
+    """z = x exactly (one feature of weight 1), far out where a slope is a small fraction of 1: dx = dy act'(z) to half a
+    step of its own size.  The functions: exp is good to (its argument + 8) 2 u, the normal distribution function to
+    7.5e-8 (16-bit types) or 4 u, and the sums of a slope's terms add 4 u of each."""
+    from sgnn_amd import functional
+    x = torch.linspace(low, high, 301).to(dtype)[:, None]
+    dy = (64.0 * normal((301, 1), 1)).to(dtype)
+    z = x.double().requires_grad_(True)
+    slope, = torch.autograd.grad(act64(z, act).sum(), z)
+    z = z.detach()
+    if act == "silu":
+        fn = torch.sigmoid(z) * (1 + z.abs()) * (z.abs() + 8) * 6 * U
+    elif act == "gelu":
+        pdf = torch.exp(-0.5 * z * z) / (2 * np.pi) ** 0.5
+        fn = (7.5e-8 if dtype != torch.float32 else 4 * U) + z.abs() * pdf * (0.5 * z * z + 8) * 6 * U + 4 * U * (z > 0)
+    else:
+        u = 2 * (2 / np.pi) ** 0.5 * (z + 0.044715 * z ** 3)
+        fn = torch.sigmoid(u) * (1 + z.abs() * 1.6 * (1 + 0.134145 * z * z)) * (u.abs() + 8) * 6 * U
+    xg, w = x.cuda().requires_grad_(True), torch.ones(1, 1, dtype=dtype, device="cuda")
+    dx, = torch.autograd.grad(functional.linear(xg, w, None, act), xg, dy.cuda())
+    ref = dy.double() * slope
+    within(dx, ref, dy.double().abs() * fn * (1 + half_step(dtype)) + rounded(dtype, ref) * (1 + 2.0 ** -10), act)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 def test_linear_long_reduction(dtype):
     """The weight's gradient of many rows, and its bias', are whole-number exact (each partial sum < 2^24)."""
     from sgnn_amd import functional
