@@ -564,8 +564,7 @@ int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, i
 /* Its backward pass from dy [M][N]: dz = dy act'(z), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = sum_m dz
  * (all dense; NULL skips one; the residual's gradient is dy).  slope: as sgnn_linear wrote it; NULL:
  * act'(z) = 1 (SGNN_ACT_NONE).
- * 16-bit types: dz is rounded once to the type before the two products, as their matrix instructions read it;
- * db sums the unrounded values.  M = 0 gives dw = db = 0.
+ * 16-bit types: the two products read dz to 16 bits (bf16) or 22 (fp16); db sums the unrounded values.  M = 0 gives dw = db = 0.
  * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != NULL) bytes, 256-B aligned. */
 size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope);
 int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const float* slope,

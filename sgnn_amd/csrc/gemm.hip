@@ -25,6 +25,9 @@ struct GemmArgs {
   float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
   int64_t lda, ldb, ldr, ldc, M, N, K;
   int32_t act, nsplit, tiles_m, tiles_n;
+  int64_t lo;           // of A's two planes (gemm.h)
+  const uint32_t* any;
+  int32_t nany;
 };
 
 // ----------------------------------------------------------------------------- epilogue
@@ -150,6 +153,22 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 }
 
 // ----------------------------------------------------------------------------- 16-bit operands
+// How many planes of A hold anything; `word` is LDS that nothing else uses yet.
+template <int THREADS>
+SGNN_DEV int planes_of(const GemmArgs& g, int* word) {
+  if (g.lo == 0) return 1;
+  if (g.nany == 0) return 2;
+  int any = 0;
+  for (int i = threadIdx.x; i < g.nany; i += THREADS) any |= g.any[i];
+  if (threadIdx.x == 0) *word = 0;
+  __syncthreads();
+  if (__any(any)) *word = 1;  // every lane that gets here writes the same
+  __syncthreads();
+  any = *word;
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(any) ? 2 : 1;
+}
+
 // BM x BN outputs per workgroup, WM x WN waves.  DIRECT: both operands' lines are 16-byte aligned (and in the cols
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 // NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
@@ -160,7 +179,7 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 // epilogue's 268 MB.  Memory is not waited for: four stages of 32 k took 334 / 248 / 244 us at their fastest, where these
 // two of 64 k took 290 / 230 / 230; the next block's loads issued behind the first fragments' reads took 292 / 226 / 237.
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT, int NST>
-__global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
   constexpr int BK = 64, kThreads = 64 * WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile16<BM, BK, ACOLS>;
@@ -178,12 +197,28 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
   const char* B = static_cast<const char*>(g.B);
   int first, last;
   blocks_of(g, BK, split, first, last);
+  const int planes = BCOLS ? planes_of<kThreads>(g, reinterpret_cast<int*>(lds)) : 1;
 
   f32x4 acc[TM][TN];
 #pragma unroll
   for (int i = 0; i < TM; ++i)
 #pragma unroll
     for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  // Two planes of A: the products of lo over all of k, brought to hi's scale, then those of hi.  A lo of 0 times an
+  // infinite operand is NaN where hi's product is infinite, so of lo's sums only finite ones count.
+  const auto settle = [&] {
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) {
+        f32x4& v = acc[i][j];
+        const float odd = (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);  // 0 where all four are finite
+        v *= 1.0f / (1 << kLoBits<T>);
+        if (odd == 0.0f) continue;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = v[r] - v[r] == 0.0f ? v[r] : 0.0f;
+      }
+  };
 
   const auto compute = [&](const char* a) {
     const char* b = a + TA::kBytes;
@@ -202,8 +237,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     if constexpr (TM >= 4) order_products<TM, TN, ACOLS ? 2 : 1, BCOLS ? 2 : 1>();
   };
   constexpr int PA = BM * BK / 8 / kThreads, PB = BN * BK / 8 / kThreads;
-  const auto fetch = [&](u32x4(&va)[PA], u32x4(&vb)[PB], int blk) {
-    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+  const auto fetch = [&](u32x4(&va)[PA], u32x4(&vb)[PB], int blk, int64_t plane) {
+    TA::template fetch<kThreads>(va, A + plane, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
     TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
   };
   const auto put = [&](char* a, const u32x4(&va)[PA], const u32x4(&vb)[PB]) {
@@ -218,24 +253,29 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     const char* pa = A + 2 * (ACOLS ? m0 : m0 * g.lda);
     const char* pb = B + 2 * (BCOLS ? n0 : n0 * g.ldb);
     const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
-    const auto stage = [&](char* a, int blk) {
+    // step t of the planes' blocks of k one after the other
+    const int blocks = last - first, total = planes * blocks;
+    const auto stage = [&](char* a, int t) {
+      const int64_t plane = planes == 2 && t < blocks ? g.lo : 0;
+      const int blk = first + (t < blocks ? t : t - blocks);
       if ((int64_t)(blk + 1) * BK <= g.K) {
-        TA::template direct<kThreads>(a, pa + blk * sa, oa);
+        TA::template direct<kThreads>(a, pa + plane + blk * sa, oa);
         TB::template direct<kThreads>(a + TA::kBytes, pb + blk * sb, ob);
       } else {  // its loads are waited for here, and with them all before them
         u32x4 va[PA], vb[PB];
-        fetch(va, vb, blk);
+        fetch(va, vb, blk, plane);
         put(a, va, vb);
       }
     };
 #pragma unroll
     for (int i = 0; i < NST - 1; ++i)
-      if (first + i < last) stage(lds + i * kStage, first + i);
+      if (i < total) stage(lds + i * kStage, i);
     int at = 0;
-    for (int blk = first; blk < last; ++blk) {
-      wait_stages<PA + PB, NST - 2>(last - 1 - blk);
+    for (int t = 0; t < total; ++t) {
+      wait_stages<PA + PB, NST - 2>(total - 1 - t);
       __syncthreads();
-      if (blk + NST - 1 < last) stage(lds + (at == 0 ? NST - 1 : at - 1) * kStage, blk + NST - 1);
+      if (t + NST - 1 < total) stage(lds + (at == 0 ? NST - 1 : at - 1) * kStage, t + NST - 1);
+      if (planes == 2 && t == blocks) settle();
       compute(lds + at * kStage);
       at = at == NST - 1 ? 0 : at + 1;
     }
@@ -248,8 +288,12 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
     const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
     const int whole = plain ? min(last, (int)(g.K / BK)) : first;
     u32x4 va[DEPTH][PA], vb[DEPTH][PB];
+#pragma unroll 1
+    for (int p = planes - 1; p >= 0; --p) {
+    const int64_t plane = p == 1 ? g.lo : 0;
+    if (planes == 2 && p == 0) settle();
     for (int blk = max(whole, first); blk < last; ++blk) {
-      fetch(va[0], vb[0], blk);
+      fetch(va[0], vb[0], blk, plane);
       put(lds, va[0], vb[0]);
       __syncthreads();
       compute(lds);
@@ -259,7 +303,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
       uint32_t oa[PA], ob[PB], move_a, move_b;
       TA::template places<kThreads>(oa, move_a, g.lda, g.M, m0);
       TB::template places<kThreads>(ob, move_b, g.ldb, g.N, n0);
-      const char* pa = A + 2 * (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda);
+      const char* pa = A + plane + 2 * (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda);
       const char* pb = B + 2 * (BCOLS ? n0 - TB::lead(n0) : n0 * g.ldb);
       const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
       const bool edge_a = m0 + BM > g.M, edge_b = n0 + BN > g.N;
@@ -282,7 +326,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm16(GemmArgs g) {
           if (blk + u < whole) compute(a);
         }
       }
+      __syncthreads();
     }
+    }
+  }
+  if (BCOLS && g.lo) {  // the planes are of half of A
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] *= 2.0f;
   }
   __syncthreads();
   write_tile<T, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, split, m0 + wm * TM * 16,
@@ -780,7 +832,7 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
   if (g.M == 0 || g.N == 0) return SGNN_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K,
-             g.act, 1, 0, 0};
+             g.act, 1, 0, 0, g.lo, g.any, g.nany};
   if (rows_ok(g)) {
     with_type(g.dtype, [&](auto* t) {
       launch_rows<std::remove_pointer_t<decltype(t)>>(a, s);

@@ -26,7 +26,8 @@ struct ActCut {
   }
 };
 
-// dz = dy act'(z), and the column sums of this workgroup's rows: every thread over its rows in order, then the
+// dz = dy act'(z), for 16 bits as two planes of its half (split2; dy times a slope of up to 1.13 may leave the type's
+// range), and the column sums of this workgroup's rows: every thread over its rows in order, then the
 // threads of one column in order.  Reads dy and the slopes, writes dz: bounded by memory (200003 x 128 fp32 52 us,
 // 5.9 TB/s; 8192 x 8192 bf16 84 us, 4.8 TB/s -- formed inside the two products instead, dz would be computed and its
 // inputs read twice, at every tile's pace).  Slopes rather than z are kept by the forward: it has the activation's
@@ -34,8 +35,9 @@ struct ActCut {
 // 1, where fixed point of 16 bits leaves nothing of it.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const float* slope, int64_t M, int64_t N,
-                                                      int lanes, T* dz, float* partial) {
+                                                      int lanes, T* dz, int64_t lo, uint32_t* any, float* partial) {
   constexpr int V = 16 / sizeof(T);
+  bool some = false;  // a lo that is not 0
   __shared__ float sums[kThreads * V];
   const int rows = kThreads / lanes, lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
   const int64_t c = ((int64_t)blockIdx.x * lanes + lane) * V;
@@ -66,13 +68,35 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
         unpack<T>(up[u], v);
         if (slope) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] *= t[u][i];
-          store_some<V>(dz + r * N + c, cnt, v);
+          for (int i = 0; i < V; ++i) v[i] *= sizeof(T) == 4 ? t[u][i] : 0.5f * t[u][i];
+          if constexpr (sizeof(T) == 4) {
+            store_some<V>(dz + r * N + c, cnt, v);
+          } else {
+            float h[V], l[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+              T hi, low;
+              split2(v[i], hi, low);
+              h[i] = to_float(hi), l[i] = to_float(low);
+              some |= i < cnt && l[i] != 0.0f;
+              v[i] *= 2.0f;
+            }
+            store_some<V>(dz + r * N + c, cnt, h);
+            store_some<V>(dz + lo + r * N + c, cnt, l);
+          }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) s[i] += v[i];
       }
     }
+  }
+  if (any) {
+    __shared__ uint32_t found;
+    if (threadIdx.x == 0) found = 0;
+    __syncthreads();
+    if (__any(some)) found = 1;
+    __syncthreads();
+    if (threadIdx.x == 0) any[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = found;
   }
   if (!partial) return;
 #pragma unroll
@@ -118,12 +142,21 @@ Gemm wgrad(int32_t dtype, int64_t M, int64_t N, int64_t K) {  // dw[N][K] = dz^T
   return g;
 }
 
-// Workspace of the backward pass: dz, the partial sums of db, and the products' own.
+// Workspace of the backward pass: dz (two planes of 16-bit types, and each workgroup's flag whether the second holds
+// anything), the partial sums of db, and the products' own.  relu's slopes leave the second plane empty, and a product
+// looks at the flags first; beyond kMostFlags of them it takes both planes unseen.
+constexpr int64_t kMostFlags = 4096;
 struct BwdLayout {
-  size_t dz, partial, gemm, total;
+  size_t plane, flags, dz, partial, gemm, total;
+  int32_t nany;
   BwdLayout(int32_t dtype, int64_t M, int64_t N, int64_t K, bool has_slope) {
-    dz = !has_slope ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
-    partial = pad256(sizeof(float) * (size_t)ActCut(dtype_size(dtype), M, N).blocks * (size_t)N);
+    const bool two = has_slope && dtype != SGNN_F32;
+    const ActCut cut(dtype_size(dtype), M, N);
+    plane = !has_slope ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
+    nany = two && cut.strips * cut.blocks <= kMostFlags ? (int32_t)(cut.strips * cut.blocks) : 0;
+    flags = two ? 2 * plane : plane;
+    dz = flags + pad256(sizeof(uint32_t) * (size_t)nany);
+    partial = pad256(sizeof(float) * (size_t)cut.blocks * (size_t)N);
     gemm = std::max(gemm_workspace_bytes(dgrad(dtype, M, N, K)), gemm_workspace_bytes(wgrad(dtype, M, N, K)));
     total = dz + partial + gemm;
   }
@@ -178,7 +211,9 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   const BwdLayout at(dtype, M, N, K, slope != nullptr);
   char* ws = static_cast<char*>(workspace);
   const void* up = dy;      // dz and its leading dimension
-  int64_t ldu = ldd;
+  int64_t ldu = ldd, lo = 0;
+  const bool two = slope && dtype != SGNN_F32;
+  uint32_t* any = two && at.nany > 0 ? reinterpret_cast<uint32_t*>(ws + at.flags) : nullptr;
   if (N > 0 && (slope || db))
     with_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -186,8 +221,9 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
       float* partial = db ? reinterpret_cast<float*>(ws + at.dz) : nullptr;
       if (M > 0) {
         hipLaunchKernelGGL(k_act_bwd<T>, dim3((unsigned)cut.strips, (unsigned)cut.blocks), dim3(kThreads), 0, s,
-                           static_cast<const T*>(dy), ldd, slope, M, N, cut.lanes, reinterpret_cast<T*>(ws), partial);
-        if (slope) up = ws, ldu = N;
+                           static_cast<const T*>(dy), ldd, slope, M, N, cut.lanes, reinterpret_cast<T*>(ws),
+                           (int64_t)(at.plane / sizeof(T)), any, partial);
+        if (slope) up = ws, ldu = N, lo = two ? (int64_t)at.plane : 0;
       }
       if (db)
         hipLaunchKernelGGL(k_bias_grad<T>, dim3(sum_grid(N)), dim3(kSumThreads), 0, s, partial,
@@ -199,7 +235,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   char* gws = ws + at.dz + at.partial;
   if (dx) {
     Gemm g = dgrad(dtype, M, N, K);
-    g.A = up, g.lda = ldu;
+    g.A = up, g.lda = ldu, g.lo = lo, g.any = any, g.nany = at.nany;
     g.B = w, g.ldb = ldw;
     g.C = dx, g.ldc = K;
     const int e = gemm_run(g, gws, at.gemm, stream);
@@ -207,7 +243,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   }
   if (dw) {
     Gemm g = wgrad(dtype, M, N, K);
-    g.A = up, g.lda = ldu;
+    g.A = up, g.lda = ldu, g.lo = lo, g.any = any, g.nany = at.nany;
     g.B = x, g.ldb = ldx;
     g.C = dw, g.ldc = K;
     return gemm_run(g, gws, at.gemm, stream);

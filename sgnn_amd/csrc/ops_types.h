@@ -101,6 +101,17 @@ SGNN_DEV void store_some(T* p, int cnt, const float (&v)[N]) {
   }
 }
 
+// v in two values of a 16-bit type, hi + lo 2^-kLoBits, good to 2^-16 (bf16) or 2^-22 (fp16) of it down to 2^-36: lo is
+// scaled to hi's size, which keeps it out of fp16's subnormal numbers.  An infinity or a NaN is hi's alone.
+template <typename T>
+constexpr int kLoBits = std::is_same_v<T, bf16_t> ? 8 : 11;
+template <typename T>
+SGNN_DEV void split2(float v, T& hi, T& lo) {
+  hi = from_float<T>(v);
+  const float rest = v - to_float(hi);
+  lo = from_float<T>(rest - rest == 0.0f ? rest * (float)(1 << kLoBits<T>) : 0.0f);
+}
+
 // Sum over groups of G consecutive lanes (16, 32 or 64), the same in each of them: within 16 lanes by DPP (xor 1, xor
 // 2, then the two mirrors), rows of 16 and halves of 32 by the swap instructions -- no LDS.
 template <int CTRL>

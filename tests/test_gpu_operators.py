@@ -150,6 +150,82 @@ def test_linear_against_64_bits(dtype, act, M, N, K):
         within(g, rg, tol * (1 + h) + rounded(dtype, rg) * (name != "dres"), f"{name} {act}")
 
 
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("M,N,K", [(37, 50, 70), (24, 72, 64), (130, 136, 264), (200, 328, 2056), (260, 515, 771), (3600, 72, 3600),
+                                   (72, 3600, 3600)])
+def test_linear_gradients_are_rounded_once(dtype, act, M, N, K):
+    """dz keeps h^2 of itself (two halves of h each) and 2^-36 where it is small, so a 16-bit gradient is off by its own
+    rounding and what fp32 sums lose.  Slopes: (|z| + 8) 8 u as in the test above, 7.5e-8 for gelu's distribution function,
+    and 0.8 times the error of z."""
+    from sgnn_amd import functional
+    h = half_step(dtype)
+    x, w, b, dy = (t.to(dtype).cuda() for t in (normal((M, K), 1), normal((N, K), 2, K ** -0.5), normal((N,), 3),
+                                                normal((M, N), 4)))
+    wide = lambda t: t.detach().double()
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(functional.linear(*leaves, act), leaves, dy)
+    z = (wide(x) @ wide(w).T + wide(b)).requires_grad_(True)
+    slope, = torch.autograd.grad(act64(z, act).sum(), z)
+    z, dz = z.detach(), dy.double() * slope
+    ez = (K + 4) * U * (wide(x).abs() @ wide(w).abs().T + wide(b).abs())
+    edz = dy.double().abs() * (0.8 * ez + (z.abs() + 8) * 8 * U + 7.5e-8) + h * h * dz.abs() + 2.0 ** -36
+    ad, aw, ax = dz.abs(), wide(w).abs(), wide(x).abs()
+    for name, got, ref, tol in (("dx", dx, dz @ wide(w), (N + 4) * 2 * U * (ad @ aw) + edz @ aw),
+                                ("dw", dw, dz.T.contiguous() @ wide(x), (M + 4) * 2 * U * (ad.T.contiguous() @ ax) + edz.T.contiguous() @ ax),
+                                ("db", db, dz.sum(0), (M + 4) * U * ad.sum(0) + edz.sum(0))):
+        within(got, ref.cpu(), (tol * (1 + h) + rounded(dtype, ref)).cpu(), f"{name} {act}")
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
+def test_linear_gradients_past_the_largest_value(dtype):
+    """dz = dy act'(z), with dy the type's largest value and a slope of 1.1, does not fit the type; dx = dz w does."""
+    from sgnn_amd import functional
+    x = torch.full((20, 3), 51.0, dtype=dtype, device="cuda", requires_grad=True)
+    w = torch.full((1, 3), 2.0 ** -6, dtype=dtype, device="cuda")
+    dy = torch.full((20, 1), torch.finfo(dtype).max, dtype=dtype, device="cuda")
+    z = (x.detach().double() @ w.double().T).requires_grad_(True)
+    slope, = torch.autograd.grad(torch.nn.functional.silu(z).sum(), z)
+    assert float(slope.min()) > 1.08
+    dx, = torch.autograd.grad(functional.linear(x, w, None, "silu"), x, dy)
+    ref = dy.double() * slope @ w.double()
+    # the slope to 100 u (of the same size), on top of the rounding
+    within(dx, ref.cpu(), ((half_step(dtype) + 100 * U) * ref).cpu(), "dx")
+
+
+def _linear_bwd_by_c(dy, slope, x, w):
+    from sgnn_amd import _hip
+    L = _hip.lib()
+    (M, N), K, dt = dy.shape, x.shape[1], _hip.DTYPES[x.dtype]
+    nws = L.sgnn_linear_bwd_workspace_bytes(dt, M, N, K, int(slope is not None))
+    ws = torch.empty(nws, dtype=torch.uint8, device="cuda")
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(N, dtype=x.dtype, device="cuda")
+    _hip.check(L.sgnn_linear_bwd(dt, M, N, K, dy.data_ptr(), N, slope.data_ptr() if slope is not None else None,
+                                 x.data_ptr(), K, w.data_ptr(), K, dx.data_ptr(), dw.data_ptr(), db.data_ptr(),
+                                 ws.data_ptr(), nws, torch.cuda.current_stream().cuda_stream), "sgnn_linear_bwd")
+    return dx, dw, db
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("K", [48, 50])
+def test_linear_gradients_non_finite_values_propagate(dtype, K):
+    """An infinity or NaN of w, x or dy reaches the gradients that read it as 64-bit arithmetic has it (slopes of 0.3: dz
+    is no value of a 16-bit type)."""
+    M, N = 40, 72
+    dy, x, w = (whole(s, i, 1, 4, dtype=dtype) for i, s in enumerate([(M, N), (M, K), (N, K)]))
+    w[11, 2], w[30, 7], x[7, 9], x[3, 5], dy[20, 40] = float("inf"), float("nan"), float("-inf"), float("nan"), float("inf")
+    slope = torch.full((M, N), 0.3)
+    dz = dy.double() * slope.double()
+    got = _linear_bwd_by_c(*(t.cuda() for t in (dy, slope, x, w)))
+    for name, g, ref in zip(("dx", "dw", "db"), got, (dz @ w.double(), dz.T @ x.double(), dz.sum(0))):
+        g = g.double().cpu()
+        assert torch.equal(g.isnan(), ref.isnan()) and torch.equal(g.isinf(), ref.isinf()), name
+        assert torch.equal(g[g.isinf()] > 0, ref[ref.isinf()] > 0), name
+        fine = ref.isfinite()
+        # sums of at most 72 positive terms; dz to 2^-16
+        within(g[fine], ref[fine], (half_step(dtype) + 2.0 ** -16 + 80 * U) * ref[fine], name)
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act,low,high", [("silu", -16.0, -8.0), ("gelu", -6.0, -4.0), ("gelu_tanh", -6.0, -4.0),
                                           ("silu", 8.0, 16.0), ("gelu", 4.0, 6.0)])
