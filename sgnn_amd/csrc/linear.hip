@@ -17,7 +17,7 @@ struct ActCut {
   int lanes;
   int64_t strips, blocks;
   ActCut(size_t size, int64_t M, int64_t N) {
-    const int64_t pieces = (N * (int64_t)size + 15) / 16;
+    const int64_t pieces = std::max<int64_t>(1, (N * (int64_t)size + 15) / 16);  // one of no columns where N = 0
     lanes = 16;
     while (lanes < kThreads && lanes < pieces) lanes *= 2;
     strips = (pieces + lanes - 1) / lanes;
@@ -214,7 +214,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   int64_t ldu = ldd, lo = 0;
   const bool two = slope && dtype != SGNN_F32;
   uint32_t* any = two && at.nany > 0 ? reinterpret_cast<uint32_t*>(ws + at.flags) : nullptr;
-  if (N > 0 && (slope || db))
+  if (N > 0 && (slope || db)) {
     with_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
       const ActCut cut(sizeof(T), M, N);
@@ -230,8 +230,9 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
                            M > 0 ? cut.blocks : 0, N, static_cast<T*>(db));
       return 0;
     });
-  const int st = check_launch("linear_bwd");
-  if (st != SGNN_OK) return st;
+    const int st = check_launch("linear_bwd");
+    if (st != SGNN_OK) return st;
+  }
   char* gws = ws + at.dz + at.partial;
   if (dx) {
     Gemm g = dgrad(dtype, M, N, K);

@@ -360,6 +360,21 @@ def test_linear_edges_of_sizes():
         assert torch.equal(functional.linear(xt, w.detach()), ref[0])
 
 
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M", [0, 5])
+def test_linear_without_outputs_has_gradients(dtype, M):
+    """No output features: y is [M, 0], the input's gradient a sum of nothing, the weight's and the bias' empty."""
+    from sgnn_amd import functional
+    x = torch.ones(M, 4, dtype=dtype, device="cuda", requires_grad=True)
+    w = torch.ones(0, 4, dtype=dtype, device="cuda", requires_grad=True)
+    b = torch.ones(0, dtype=dtype, device="cuda", requires_grad=True)
+    for act in ("none", "silu"):
+        y = functional.linear(x, w, b, act)
+        assert y.shape == (M, 0)
+        dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.empty(M, 0, dtype=dtype, device="cuda"))
+        assert torch.equal(dx, torch.zeros_like(x)) and dw.shape == (0, 4) and db.shape == (0,)
+
+
 def test_linear_non_finite_values_propagate():
     """A NaN or infinity reaches exactly the outputs that read it, as fp32 arithmetic has it; ReLU keeps a NaN."""
     from sgnn_amd import functional

@@ -50,6 +50,15 @@ def test_linear_bwd_refuses(lib, bad):
     assert "linear_bwd" in lib.sgnn_last_error().decode()
 
 
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("M", [0, 4])
+@pytest.mark.parametrize("slope", [None, P])
+def test_linear_bwd_without_outputs(lib, dtype, M, slope):
+    """N = 0: dw and db have no elements, and without dx there is nothing to launch."""
+    assert lib.sgnn_linear_bwd_workspace_bytes(dtype, M, 0, 4, int(slope is not None)) == 0
+    assert _linear_bwd(lib, dtype=dtype, M=M, N=0, dy=None, slope=slope, dx=None, ws=None, nws=0) == _hip.SGNN_OK
+
+
 @pytest.mark.parametrize("bad", [
     dict(dtype=5), dict(dtype=1, wdtype=2), dict(n=-1), dict(width=0), dict(x=None), dict(y=None), dict(ldx=3),
     dict(res=P, ldr=3), dict(eps=-1.0), dict(eps=float("nan"))])
