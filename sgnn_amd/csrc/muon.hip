@@ -798,9 +798,11 @@ int by_chunks(const Group& grp, int32_t steps, float a, float b, float c, float 
   return full_side(grp.rows, grp.cols) ? go(k_ns_chunk<T, 4>) : go(k_ns_chunk<T, 2>);
 }
 
-// The matrices from i on that share a launch: small ones of any shape, or large ones of one shape.
+// The matrices from i on that share a launch: small ones of any shape, or large ones of one shape; an empty one is a run
+// of its own.
 int32_t run_of(const sgnn_matrix* mats, int32_t count, int32_t i) {
   int32_t n = 1;
+  if (mats[i].rows == 0 || mats[i].cols == 0) return n;
   if (small_ok(mats[i].rows, mats[i].cols)) {
     while (i + n < count && n < kMaxSmall && mats[i + n].rows > 0 && mats[i + n].cols > 0 &&
            small_ok(mats[i + n].rows, mats[i + n].cols) &&

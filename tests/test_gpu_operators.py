@@ -599,6 +599,23 @@ def test_newton_schulz_batches_and_lists():
     assert muon.newton_schulz([]) == []
 
 
+def test_newton_schulz_by_c_with_empty_matrices():
+    """Empty matrices anywhere in the array: the others, of all three kinds of launch, get the bits they get alone."""
+    from sgnn_amd import _hip, muon
+    shapes = [(0, 7), (4, 4), (7, 0), (64, 30), (0, 0), (128, 500), (0, 128), (300, 260), (300, 260), (0, 300), (20, 9)]
+    ins = [normal(s, i).cuda() for i, s in enumerate(shapes)]
+    outs = [torch.full_like(t, 9.0) for t in ins]
+    mats = (_hip.SgnnMatrix * len(shapes))(*[_hip.SgnnMatrix(a.data_ptr(), b.data_ptr(), s[1], s[1], *s)
+                                             for a, b, s in zip(ins, outs, shapes)])
+    L = _hip.lib()
+    nws = L.sgnn_newton_schulz_workspace_bytes(mats, len(shapes))
+    ws = torch.empty(nws, dtype=torch.uint8, device="cuda")
+    _hip.check(L.sgnn_newton_schulz(0, mats, len(shapes), 5, *muon.QUINTIC, 1e-7, ws.data_ptr(), nws,
+                                    torch.cuda.current_stream().cuda_stream), "sgnn_newton_schulz")
+    for a, b in zip(ins, outs):
+        assert torch.equal(b, muon.newton_schulz(a))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("count,m,n", [(40, 20, 24), (70, 64, 64), (12, 128, 384), (33, 100, 300), (12, 300, 260), (9, 520, 640)])
 def test_newton_schulz_of_a_batch_keeps_each_matrix_bits(dtype, count, m, n):

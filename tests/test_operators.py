@@ -95,6 +95,19 @@ def test_newton_schulz_refuses(lib, bad):
     assert "newton_schulz" in lib.sgnn_last_error().decode()
 
 
+@pytest.mark.skipif(torch.cuda.is_available(), reason="the matrices' addresses are none of a device")
+@pytest.mark.parametrize("empty", [(0, 7), (7, 0), (0, 0)])
+def test_newton_schulz_goes_on_behind_an_empty_matrix(lib, empty):
+    """Without a device every call that has work ends in a launch error; one that skips its matrices reports success."""
+    def status(shapes):
+        mats = (_hip.SgnnMatrix * len(shapes))(*[_hip.SgnnMatrix(P, P, max(c, 1), max(c, 1), r, c) for r, c in shapes])
+        return lib.sgnn_newton_schulz(0, mats, len(shapes), 5, 1.0, 0.0, 0.0, 0.0, P, 1 << 30, None)
+    assert status([empty]) == _hip.SGNN_OK
+    assert status([(4, 4)]) != _hip.SGNN_OK
+    assert status([empty, (4, 4)]) != _hip.SGNN_OK
+    assert status([empty, empty, (300, 200)]) != _hip.SGNN_OK
+
+
 def test_matrix_struct_matches_header():
     assert ctypes.sizeof(_hip.SgnnMatrix) == 40
 
