@@ -64,7 +64,7 @@ SGNN_DEV void finish(const GemmArgs& g, int64_t m, int64_t n, float (&v)[V], con
     case SGNN_ACT_GELU: act_row<SGNN_ACT_GELU, T>(g, m * g.N + n, cnt, v); break;
     case SGNN_ACT_GELU_TANH: act_row<SGNN_ACT_GELU_TANH, T>(g, m * g.N + n, cnt, v); break;
     case SGNN_ACT_SILU: act_row<SGNN_ACT_SILU, T>(g, m * g.N + n, cnt, v); break;
-    default: break;
+    default: act_row<SGNN_ACT_NONE, T>(g, m * g.N + n, cnt, v); break;
   }
   if (g.res) {
     load_some<V>(static_cast<const T*>(g.res) + m * g.ldr + n, cnt, t);

@@ -207,6 +207,27 @@ def _linear_bwd_by_c(dy, slope, x, w):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(4, 20, 24), (70, 75, 88), (300, 264, 40), (70, 33, 4100), (5, 6, 0)])
+def test_linear_by_c_writes_every_slope(dtype, M, N, K):
+    """A slope buffer is written whatever the activation: ones without one, and relu's 0 and 1; the gradients that read
+    it are those without a buffer."""
+    from sgnn_amd import _hip
+    L, dt = _hip.lib(), _hip.DTYPES[dtype]
+    x, w, dy = (whole(s, i, dtype=dtype).cuda() for i, s in enumerate([(M, K), (N, K), (M, N)]))
+    nws = L.sgnn_linear_workspace_bytes(dt, M, N, K)
+    ws = torch.empty(max(nws, 1), dtype=torch.uint8, device="cuda")
+    for act, want in (("none", torch.ones(M, N)), ("relu", (x.double() @ w.double().T > 0).float().cpu())):
+        y, slope = torch.empty(M, N, dtype=dtype, device="cuda"), torch.full((M, N), 7.0, device="cuda")
+        _hip.check(L.sgnn_linear(dt, M, N, K, x.data_ptr(), K, w.data_ptr(), K, None, _hip.ACTIVATIONS[act], None, 0,
+                                 slope.data_ptr(), y.data_ptr(), N, ws.data_ptr(), nws,
+                                 torch.cuda.current_stream().cuda_stream), "sgnn_linear")
+        assert torch.equal(slope.cpu(), want), act
+        if act == "none" and K:
+            for a, b in zip(_linear_bwd_by_c(dy, slope, x, w), _linear_bwd_by_c(dy, None, x, w)):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("K", [48, 50])
 def test_linear_gradients_non_finite_values_propagate(dtype, K):
     """An infinity or NaN of w, x or dy reaches the gradients that read it as 64-bit arithmetic has it (slopes of 0.3: dz
