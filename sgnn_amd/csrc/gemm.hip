@@ -280,9 +280,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
       at = at == NST - 1 ? 0 : at + 1;
     }
   } else {
-    // The partial block of k (or all, of an operand too narrow for 16 bytes) one after the other; then whole blocks,
-    // DEPTH of them waiting in registers.  Their loads stand outside any branch (past the end the last block is
-    // loaded again), or the compiler waits for all of them at each use.
+    // Whole blocks, DEPTH of them waiting in registers (their loads stand outside any branch: past the end the last block
+    // is loaded again; or the compiler waits for all of them at each use); then the partial block of k (or all, of an
+    // operand too narrow for 16 bytes) one after the other.  The order of k is that of the direct loads, so an output
+    // has the same bits at any alignment.
     static_assert(NST == 2, "two stages");
     constexpr int DEPTH = BM > 64 ? 2 : 4;
     const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
@@ -290,44 +291,44 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
     u32x4 va[DEPTH][PA], vb[DEPTH][PB];
 #pragma unroll 1
     for (int p = planes - 1; p >= 0; --p) {
-    const int64_t plane = p == 1 ? g.lo : 0;
-    if (planes == 2 && p == 0) settle();
-    for (int blk = max(whole, first); blk < last; ++blk) {
-      fetch(va[0], vb[0], blk, plane);
-      put(lds, va[0], vb[0]);
-      __syncthreads();
-      compute(lds);
-      __syncthreads();
-    }
-    if (first < whole) {
-      uint32_t oa[PA], ob[PB], move_a, move_b;
-      TA::template places<kThreads>(oa, move_a, g.lda, g.M, m0);
-      TB::template places<kThreads>(ob, move_b, g.ldb, g.N, n0);
-      const char* pa = A + plane + 2 * (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda);
-      const char* pb = B + 2 * (BCOLS ? n0 - TB::lead(n0) : n0 * g.ldb);
-      const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
-      const bool edge_a = m0 + BM > g.M, edge_b = n0 + BN > g.N;
-      const auto get = [&](u32x4(&a)[PA], u32x4(&b)[PB], int blk) {
-        blk = min(blk, whole - 1);
-        TA::fetch_whole(a, pa + blk * sa, oa);
-        TB::fetch_whole(b, pb + blk * sb, ob);
-      };
+      const int64_t plane = p == 1 ? g.lo : 0;
+      if (planes == 2 && p == 0) settle();
+      if (first < whole) {
+        uint32_t oa[PA], ob[PB], move_a, move_b;
+        TA::template places<kThreads>(oa, move_a, g.lda, g.M, m0);
+        TB::template places<kThreads>(ob, move_b, g.ldb, g.N, n0);
+        const char* pa = A + plane + 2 * (ACOLS ? m0 - TA::lead(m0) : m0 * g.lda);
+        const char* pb = B + 2 * (BCOLS ? n0 - TB::lead(n0) : n0 * g.ldb);
+        const int64_t sa = 2 * BK * (ACOLS ? g.lda : 1), sb = 2 * BK * (BCOLS ? g.ldb : 1);
+        const bool edge_a = m0 + BM > g.M, edge_b = n0 + BN > g.N;
+        const auto get = [&](u32x4(&a)[PA], u32x4(&b)[PB], int blk) {
+          blk = min(blk, whole - 1);
+          TA::fetch_whole(a, pa + blk * sa, oa);
+          TB::fetch_whole(b, pb + blk * sb, ob);
+        };
 #pragma unroll
-      for (int u = 0; u < DEPTH; ++u) get(va[u], vb[u], first + u);
-      for (int blk = first; blk < whole; blk += DEPTH) {
+        for (int u = 0; u < DEPTH; ++u) get(va[u], vb[u], first + u);
+        for (int blk = first; blk < whole; blk += DEPTH) {
 #pragma unroll
-        for (int u = 0; u < DEPTH; ++u) {
-          // past the end: the same block once more, whose products are not formed
-          char* a = lds + (u & 1) * kStage;
-          TA::template put_moved<kThreads>(a, va[u], move_a, edge_a);
-          TB::template put_moved<kThreads>(a + TA::kBytes, vb[u], move_b, edge_b);
-          get(va[u], vb[u], blk + u + DEPTH);
-          __syncthreads();
-          if (blk + u < whole) compute(a);
+          for (int u = 0; u < DEPTH; ++u) {
+            // past the end: the same block once more, whose products are not formed
+            char* a = lds + (u & 1) * kStage;
+            TA::template put_moved<kThreads>(a, va[u], move_a, edge_a);
+            TB::template put_moved<kThreads>(a + TA::kBytes, vb[u], move_b, edge_b);
+            get(va[u], vb[u], blk + u + DEPTH);
+            __syncthreads();
+            if (blk + u < whole) compute(a);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
-    }
+      for (int blk = max(whole, first); blk < last; ++blk) {
+        fetch(va[0], vb[0], blk, plane);
+        put(lds, va[0], vb[0]);
+        __syncthreads();
+        compute(lds);
+        __syncthreads();
+      }
     }
   }
   if (BCOLS && g.lo) {  // the planes are of half of A
@@ -538,18 +539,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
       for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[0], acc[i][j]);
     }
   };
-  // As in k_gemm16: the partial block (or all, of an operand too narrow) first, then whole blocks without branches.
+  // As in k_gemm16: whole blocks without branches, then the partial one (or all, of an operand too narrow).
   const bool plain = TA::plain(g.lda, g.M) && TB::plain(g.ldb, g.N);
   const int whole = plain ? min(last, (int)(g.K / BK)) : first;
-  for (int blk = max(whole, first); blk < last; ++blk) {
-    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
-    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
-    TA::template put<kThreads>(lds, va);
-    TB::template put<kThreads>(lds + TA::kBytes, vb);
-    __syncthreads();
-    compute(lds);
-    __syncthreads();
-  }
   if (first < whole) {
     uint32_t oa[PA], ob[PB];
     int move_a, move_b;
@@ -592,6 +584,15 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
         here = there, there = t;
       }
     }
+  }
+  for (int blk = max(whole, first); blk < last; ++blk) {
+    TA::template fetch<kThreads>(va, A, g.lda, g.M, g.K, m0, (int64_t)blk * BK);
+    TB::template fetch<kThreads>(vb, B, g.ldb, g.N, g.K, n0, (int64_t)blk * BK);
+    TA::template put<kThreads>(lds, va);
+    TB::template put<kThreads>(lds + TA::kBytes, vb);
+    __syncthreads();
+    compute(lds);
+    __syncthreads();
   }
   __syncthreads();
   const int64_t k0 = (int64_t)first * BK, k1 = min((int64_t)last * BK, g.K);
@@ -793,7 +794,7 @@ void launch_tiles(const GemmArgs& g, const Plan& p, dim3 grid, bool direct, hipS
   }
 }
 
-// The row kernel: 32 rows at most, and few enough columns per row of x that x's repeated reads stay below w's.
+// The row kernel: 32 rows at most, both operands with k contiguous.
 bool rows_ok(const Gemm& g) { return !g.a_cols && !g.b_cols && g.M <= 32; }
 
 template <typename T>

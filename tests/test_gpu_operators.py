@@ -113,6 +113,41 @@ def test_linear_strides_and_alignment(dtype, lead, offset):
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(70, 80, 72), (200, 136, 200), (24, 40, 4168), (1000, 136, 72), (4000, 3200, 72)])
+def test_linear_has_the_same_bits_at_any_alignment(dtype, M, N, K):
+    """Dense operands, and views that start one element further on or have unused columns: the summation order depends on
+    the sizes alone (sizes whose last block of k is a part of one, in every product)."""
+    from sgnn_amd import functional
+    x, w, dy = normal((M, K), 1).to(dtype), normal((N, K), 2, K ** -0.5).to(dtype), normal((M, N), 3).to(dtype)
+    runs = []
+    for lead, offset in ((0, 0), (0, 1), (1, 0), (8, 8)):
+        xs, wsd, dys = (strided(t, lead, offset) for t in (x, w, dy))
+        for act in ("none", "silu"):
+            leaves = [xs.requires_grad_(True), wsd.requires_grad_(True)]
+            y = functional.linear(*leaves, None, act)
+            runs.append((act, lead, offset, [y.detach(), *torch.autograd.grad(y, leaves, dys)]))
+    for act, lead, offset, got in runs[2:]:
+        want = next(r for r in runs if r[0] == act)[3]
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), (act, lead, offset)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_linear_has_the_same_bits_at_any_leading_dimension(dtype):
+    """Rows far apart (2^22 elements and more) are loaded by another path than near ones, in the same order of k."""
+    from sgnn_amd import functional
+    M, N, K, ld = 40, 48, 72, (1 << 22) + 64
+    x, w, dy = normal((M, K), 1).to(dtype).cuda(), normal((N, K), 2).to(dtype).cuda(), normal((M, N), 3).to(dtype).cuda()
+    far = torch.zeros(M, ld, dtype=dtype, device="cuda")
+    far[:, :K] = x
+    outs = []
+    for a in (x, far[:, :K]):
+        leaves = [a.requires_grad_(True), w.requires_grad_(True)]
+        y = functional.linear(*leaves)
+        outs.append([y.detach(), *torch.autograd.grad(y, leaves, dy)])
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
 @pytest.mark.parametrize("act", ACTS)
 @pytest.mark.parametrize("M,N,K", [(37, 50, 70), (130, 140, 260), (1, 96, 600)])
 def test_linear_against_64_bits(dtype, act, M, N, K):
