@@ -477,16 +477,68 @@ struct Tile32 {
   }
 };
 
+// Sub-tiles of a wave's accumulators (at m0, n0) with a value that is not finite are formed once more over k0 .. k1 with
+// fp32 matrix instructions, straight from memory, and those values replaced.  Nothing is shared between sub-tiles, as few
+// products need it.  2048^3 forward and backward take 0.36 ms, of NaN alone 3.6.
+constexpr int kRedo = 4;  // k per lane and step
+template <bool ACOLS, bool BCOLS, int TM, int TN>
+SGNN_DEV void redo_non_finite(const GemmArgs& g, f32x4 (&acc)[TM][TN], int64_t m0, int64_t n0, int64_t k0, int64_t k1) {
+  static_assert(TM * TN <= 32, "a bit per sub-tile");
+  uint32_t odd_tiles = 0;
+#pragma unroll
+  for (int i = 0; i < TM; ++i)
+#pragma unroll
+    for (int j = 0; j < TN; ++j) {
+      const f32x4 v = acc[i][j];
+      // x - x is 0 for finite x alone
+      const float odd = (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
+      if (__any(odd != 0.0f)) odd_tiles |= 1u << (i * TN + j);
+    }
+  const int l = lane_id();
+  const float *A = static_cast<const float*>(g.A), *B = static_cast<const float*>(g.B);
+  while (odd_tiles) {  // the same in every lane
+    const int t = __builtin_ctz(odd_tiles);
+    odd_tiles &= odd_tiles - 1;
+    const int64_t m = m0 + t / TN * 16 + (l & 15), n = n0 + t % TN * 16 + (l & 15), kl = k0 + kRedo * (l >> 4);
+    const int64_t step_a = ACOLS ? g.lda : 1, step_b = BCOLS ? g.ldb : 1;
+    const float* pa = A + (ACOLS ? m : m * g.lda) + kl * step_a;
+    const float* pb = B + (BCOLS ? n : n * g.ldb) + kl * step_b;
+    int64_t left = k1 - kl;  // of this lane's k
+    const bool there_a = m < g.M, there_b = n < g.N;
+    f32x4 s = {0, 0, 0, 0};
+#pragma unroll 1
+    for (int64_t k = k0; k < k1; k += 4 * kRedo) {
+      float a[kRedo], b[kRedo];
+#pragma unroll
+      for (int e = 0; e < kRedo; ++e) {
+        a[e] = there_a && e < left ? pa[e * step_a] : 0.0f;
+        b[e] = there_b && e < left ? pb[e * step_b] : 0.0f;
+      }
+#pragma unroll
+      for (int e = 0; e < kRedo; ++e) s = __builtin_amdgcn_mfma_f32_16x16x4f32(b[e], a[e], s, 0, 0, 0);
+      pa += 4 * kRedo * step_a, pb += 4 * kRedo * step_b, left -= 4 * kRedo;
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        if (t == i * TN + j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!(acc[i][j][r] - acc[i][j][r] == 0.0f)) acc[i][j][r] = s[r];
+  }
+}
+
 // a b = sum of the parts' products; left out are mid lo, lo mid and lo lo, below 2^-22 of |a b| together.
 // An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
-// are not finite are formed once more in plain fp32 (`again`).
+// are not finite are formed once more (redo_non_finite).
 // NST = 2 stages of LDS: the next block is split and written while this one's products run; a matrix instruction takes
 // 16 cycles, in which a wave issues three others (4096^3: 695 us, 198 TFLOP/s; 765 with one stage, where split and
 // products take turns and the two waves of a SIMD fall into step; other mixtures asked of the scheduler: 704 to 733).
 // NST = 1: half the LDS, so two workgroups per CU, one's epilogue beside the other's products: better where k is short
 // (200003 x 384 x 128, silu: 180 us against 211).
 template <bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, int NST>
-__global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm32(GemmArgs g) {
   constexpr int BK = 32, kThreads = 64 * WM * WN;
   constexpr int TM = BM / WM / 16, TN = BN / WN / 16;
   using TA = Tile32<BM, ACOLS>;
@@ -495,7 +547,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
   __shared__ __attribute__((aligned(16))) char lds[NST * kStage];
   constexpr int RP = 2, kBuf = RP * 16 * 16 * TN;
   static_assert(kBuf * 4 * WM * WN <= NST * kStage, "the epilogue's buffers fit");
-  const int w = wave_id(), wm = w / WN, wn = w % WN, l = lane_id();
+  const int w = wave_id(), wm = w / WN, wn = w % WN;
   int tm, tn;
   tile_of(g, tm, tn);
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
@@ -595,27 +647,8 @@ __global__ __launch_bounds__(64 * WM * WN) void k_gemm32(GemmArgs g) {
     __syncthreads();
   }
   __syncthreads();
-  const int64_t k0 = (int64_t)first * BK, k1 = min((int64_t)last * BK, g.K);
-#pragma unroll
-  for (int i = 0; i < TM; ++i)
-#pragma unroll
-    for (int j = 0; j < TN; ++j) {
-      const f32x4 v = acc[i][j];
-      // x - x is 0 for finite x alone
-      const float odd = (v[0] - v[0]) + (v[1] - v[1]) + (v[2] - v[2]) + (v[3] - v[3]);
-      if (odd == 0.0f) continue;
-      const int64_t m = m0 + (wm * TM + i) * 16 + (l & 15);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t n = n0 + (wn * TN + j) * 16 + 4 * (l >> 4) + r;
-        if (v[r] - v[r] == 0.0f || m >= g.M || n >= g.N) continue;
-        float s = 0.0f;
-#pragma unroll 1
-        for (int64_t k = k0; k < k1; ++k)
-          s = fmaf(A[ACOLS ? k * g.lda + m : m * g.lda + k], B[BCOLS ? k * g.ldb + n : n * g.ldb + k], s);
-        acc[i][j][r] = s;
-      }
-    }
+  redo_non_finite<ACOLS, BCOLS>(g, acc, m0 + wm * TM * 16, n0 + wn * TN * 16, (int64_t)first * BK,
+                                min((int64_t)last * BK, g.K));
   write_tile<float, RP>(g, reinterpret_cast<float*>(lds) + w * kBuf, acc, split, m0 + wm * TM * 16,
                         n0 + wn * TN * 16);
 }

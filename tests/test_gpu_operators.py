@@ -445,6 +445,38 @@ def test_linear_non_finite_values_propagate():
                                                                           want.to(dtype).double().nan_to_num(1.5, 1e9, -1e9))
 
 
+def test_linear_of_nan_costs_no_multiple_of_the_product():
+    """A diverged fp32 step (every output NaN) is formed once more by matrix instructions: far below the more than
+    hundred times that one lane per output took.  Forward, dx and dw."""
+    from sgnn_amd import functional
+    n = 2048
+
+    def step(x, w, dy):
+        leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+        y = functional.linear(*leaves)
+        return y, *torch.autograd.grad(y, leaves, dy)
+
+    def best(args):
+        times = []
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            step(*args)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    args = [normal((n, n), i).cuda() for i in range(3)]
+    finite = best(args)
+    args[1].detach()[5, 7] = float("nan")
+    one = best(args)
+    bad = [torch.full_like(t, float("nan")) for t in args]
+    assert all(t.isnan().all() for t in step(*bad))
+    every = best(bad)
+    print(f"finite {finite:.3f} ms, one NaN {one:.3f} ms, all NaN {every:.3f} ms")
+    assert one <= 4 * finite + 1.0 and every <= 40 * finite
+
+
 def test_linear_refuses():
     from sgnn_amd import functional
     x, w = torch.zeros(3, 4, device="cuda"), torch.zeros(5, 4, device="cuda")
