@@ -99,6 +99,13 @@ Tensor rows_of(const Tensor& t) {
 // The leading dimension of rows_of's result (a single row's stride says nothing).
 int64_t ld(const Tensor& t) { return std::max(t.stride(0), t.size(1)); }
 
+// The operators have backward derivatives alone; a tangent would be lost without a word where no node is made.
+template <typename... Ts>
+void reverse_mode_only(const char* what, const Ts&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!((ts.defined() && ts._fw_grad(/*level=*/0).defined()) || ...), what,
+                              ": no forward-mode derivatives");
+}
+
 void* ptr(const Tensor& t) { return t.defined() && t.numel() ? t.data_ptr() : nullptr; }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
@@ -214,6 +221,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const MaybeTensor& bias, co
     r = rows_of(*residual);
   }
   const Tensor xr = rows_of(x), wr = rows_of(weight);
+  reverse_mode_only("linear", xr, wr, b, r);
   Tensor y;
   if (at::GradMode::is_enabled() && (wants_grad(xr) || wants_grad(wr) || wants_grad(b) || wants_grad(r)))
     y = LinearNode::apply(xr, wr, maybe(b), maybe(r), act);
@@ -304,6 +312,7 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor&
     r = rows_of(*residual);
   }
   const Tensor xr = rows_of(x);
+  reverse_mode_only("layer_norm", xr, w, b, r);
   Tensor y;
   if (at::GradMode::is_enabled() && (wants_grad(xr) || wants_grad(w) || wants_grad(b) || wants_grad(r)))
     y = NormNode::apply(xr, maybe(w), maybe(b), maybe(r), eps);

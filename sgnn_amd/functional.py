@@ -9,9 +9,10 @@ chain there does not cover on them: 16-bit parameters and other activations.
 
 Forward and backward run in libsgnn_hip.so on the caller's stream; every sum
 and statistic is held in fp32 and a 16-bit result is rounded once.  Everything
-is deterministic.  Backward passes are differentiable once.  To capture one
-into a graph, take the gradients with torch.autograd.grad (it needs no
-accumulation node of a leaf, which belongs to the stream that first used it).
+is deterministic.  Backward passes are differentiable once; forward-mode
+derivatives are refused.  To capture a backward pass into a graph, take the
+gradients with torch.autograd.grad (it needs no accumulation node of a leaf,
+which belongs to the stream that first used it).
 Checks, allocation and the autograd nodes are csrc/torch_ops.cpp.
 """
 from __future__ import annotations

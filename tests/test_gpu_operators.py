@@ -618,6 +618,27 @@ def test_layer_norm_refuses():
             call()
 
 
+def test_forward_mode_derivatives_are_refused():
+    """A dual tensor in any place, with or without a graph of the backward pass."""
+    import torch.autograd.forward_ad as ad
+    from sgnn_amd import functional
+    t = {k: normal(s, i).cuda() for i, (k, s) in enumerate([("x", (6, 8)), ("w", (5, 8)), ("b", (5,)), ("r", (6, 5)),
+                                                           ("g", (8,)), ("rx", (6, 8))])}
+    with ad.dual_level():
+        for k in t:
+            for graph in (False, True):
+                d = {n: v.clone().requires_grad_(graph) for n, v in t.items()}
+                d[k] = ad.make_dual(d[k], torch.ones_like(t[k]))
+                for grad in (True, False):
+                    with torch.set_grad_enabled(grad):
+                        if k in "xwbr":
+                            with pytest.raises(NotImplementedError, match="forward-mode"):
+                                functional.linear(d["x"], d["w"], d["b"], "silu", d["r"])
+                        if k in ("x", "g", "rx"):
+                            with pytest.raises(NotImplementedError, match="forward-mode"):
+                                functional.layer_norm(d["x"], d["g"], residual=d["rx"])
+
+
 # ----------------------------------------------------------------------------- newton-schulz
 def ns64(g, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
     a, b, c = coefficients
