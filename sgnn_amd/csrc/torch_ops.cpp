@@ -117,6 +117,13 @@ void* stream_of(const Tensor& x) { return c10::hip::getCurrentHIPStream(x.device
 MaybeTensor maybe(const Tensor& t) { return t.defined() ? MaybeTensor(t) : MaybeTensor(); }
 Tensor given(const MaybeTensor& t) { return t ? *t : Tensor(); }
 
+// The gradient that came in as rows of plain values: it may be lazily negated (the imaginary part of a conjugate) or
+// sparse, whatever the output was.
+Tensor grad_rows(const Tensor& g) {
+  const Tensor dense = g.layout() == at::kStrided ? g : g.to_dense();
+  return rows_of(dense.is_neg() ? dense.resolve_neg() : dense);
+}
+
 // Whether input i of a node (x, weight, bias, residual) wants its gradient.  `present` has a bit for each that was
 // given: the node numbers those alone.
 bool needs(AutogradContext* ctx, int64_t present, int i) {
@@ -180,7 +187,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
-    const Tensor dy = rows_of(grads[0]);
+    const Tensor dy = grad_rows(grads[0]);
     const int64_t present = ctx->saved_data["present"].toInt();
     Tensor dx, dw, db;
     if (needs(ctx, present, 0)) dx = at::empty({M, K}, x.options());
@@ -267,7 +274,7 @@ struct NormNode : torch::autograd::Function<NormNode> {
     const bool graph = at::GradMode::is_enabled();
     at::NoGradGuard no_grad;
     c10::DeviceGuard guard(x.device());
-    const Tensor dy = rows_of(grads[0]);
+    const Tensor dy = grad_rows(grads[0]);
     const auto affine_type = (at::ScalarType)ctx->saved_data["affine"].toInt();
     const auto affine = x.options().dtype(affine_type);
     const int64_t present = ctx->saved_data["present"].toInt();

@@ -618,6 +618,23 @@ def test_layer_norm_refuses():
             call()
 
 
+@pytest.mark.parametrize("kind", ["negated", "sparse", "expanded"])
+def test_gradients_of_other_forms(kind):
+    """An incoming gradient that is a lazily negated view, sparse, or one value for all."""
+    from sgnn_amd import functional
+    x, w, dy = normal((9, 12), 1).cuda(), normal((7, 12), 2).cuda(), normal((9, 7), 3).cuda()
+    if kind == "expanded":
+        dy = dy[:1, :1].expand(9, 7)
+    form = {"negated": lambda t: torch._neg_view(-t), "sparse": lambda t: t.to_sparse(), "expanded": lambda t: t}[kind]
+    for call in (lambda a, b: functional.linear(a, b, None, "silu"), functional.linear,
+                 lambda a, b: functional.layer_norm(a[:, :7], b[:, 0])):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        y = call(*leaves)
+        got = torch.autograd.grad(y, leaves, form(dy), retain_graph=True)
+        want = torch.autograd.grad(y, leaves, dy.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_forward_mode_derivatives_are_refused():
     """A dual tensor in any place, with or without a graph of the backward pass."""
     import torch.autograd.forward_ad as ad
