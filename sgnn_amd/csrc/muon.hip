@@ -65,6 +65,18 @@ __global__ __launch_bounds__(256) void k_ns_norm(Group g, double* part) {
   if (threadIdx.x == 0) part[b * gridDim.x + blockIdx.x] = red[0] + red[1] + red[2] + red[3];
 }
 
+// |in|_F + eps from the sum of squares.  A norm can pass fp32's range where no element does: it and the elements are
+// then brought down by 2^64 first.
+struct Norm {
+  float down, norm;
+  SGNN_DEV Norm(double squares, float eps) {
+    const double n = sqrt(squares);
+    down = n > 1e38 ? 0x1p-64f : 1.0f;
+    norm = (float)(n * down) + eps * down;
+  }
+  SGNN_DEV float of(float v) const { return norm == 0.0f ? 0.0f : v * down / norm; }  // only zeros have the norm 0
+};
+
 // Eight values times scale into the planes, at a 16-byte address.
 SGNN_DEV void put_planes(f16_t* p, int64_t plane, const float* v, float scale) {
   typedef f16_t h8 __attribute__((ext_vector_type(8)));
@@ -92,7 +104,7 @@ __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, i
   if (lane_id() == 0) red[wave_id()] = s;
   __syncthreads();
   s = red[0] + red[1] + red[2] + red[3];
-  const float norm = (float)sqrt(s) + eps;
+  const Norm norm(s, eps);
   const T* in = static_cast<const T*>(g.in[b]);
   const int64_t per = ld / 8, total = rows_padded * per;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += (int64_t)gridDim.x * 256) {
@@ -101,7 +113,7 @@ __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, i
     float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (there) load_some<8>(in + r * g.ld_in[b] + c, (int)(g.cols - c), v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = norm == 0.0f ? 0.0f : v[i] / norm;  // only zeros have the norm 0
+    for (int i = 0; i < 8; ++i) v[i] = norm.of(v[i]);
     if (x)
       put_planes(x + b * batch + r * ld + c, plane, v, kScale);
     else if (there)
@@ -511,7 +523,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
   s = 0.0;
 #pragma unroll
   for (int i = 0; i < kSmallWaves; ++i) s += red[i];
-  const float norm = (float)sqrt(s) + eps;
+  const Norm norm(s, eps);
   // the bits into the planes of the value / norm
   for (int t = threadIdx.x; t < plane_x / 16; t += kSmallThreads) {
     const u32x4 hi = *reinterpret_cast<u32x4*>(X + 16 * t), lo = *reinterpret_cast<u32x4*>(X + plane_x + 16 * t);
@@ -519,8 +531,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_small(SmallArgs args, int 
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const uint32_t up = hi[e >> 1] >> (16 * (e & 1)) << 16, low = lo[e >> 1] >> (16 * (e & 1)) & 0xffffu;
-      const float x = __builtin_bit_cast(float, up | low);
-      v[e] = norm == 0.0f ? 0.0f : x / norm;
+      v[e] = norm.of(__builtin_bit_cast(float, up | low));
     }
     put_planes(reinterpret_cast<f16_t*>(X + 16 * t), plane_x / 2, v, kScale);
   }
@@ -683,7 +694,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
     s = 0.0;
 #pragma unroll
     for (int i = 0; i < kSmallWaves; ++i) s += red[i];
-    const float norm = (float)sqrt(s) + a.eps;
+    const Norm norm(s, a.eps);
     // this chunk of the caller's matrix: rows r0 .. of it where it is tall, columns where it is wide
     const int r0 = tall ? c0 : 0, rows = tall ? min(kChunk, grp.rows - c0) : grp.rows;
     const int k0 = tall ? 0 : c0, cols = tall ? grp.cols : min(kChunk, grp.cols - c0);
@@ -707,7 +718,7 @@ __global__ __launch_bounds__(kSmallThreads) void k_ns_chunk(Group grp, ChunkArgs
         for (int e = 0; e < V; ++e) {
           if (c + e >= cols) continue;
           char* at = X + 2 * (tall ? (c + e) * ldx + r : r * ldx + c + e);
-          const float y = (norm == 0.0f ? 0.0f : v[e] / norm) * kScale;
+          const float y = norm.of(v[e]) * kScale;
           const f16_t h = (f16_t)y;
           *reinterpret_cast<f16_t*>(at) = h;
           *reinterpret_cast<f16_t*>(at + plane_x) = (f16_t)(y - (float)h);

@@ -801,6 +801,19 @@ def test_newton_schulz_special_values():
     assert float((muon.newton_schulz(small).double().cpu() - ref).norm() / ref.norm()) <= ns_tol(ref, torch.float32, 20, 30)
 
 
+@pytest.mark.parametrize("dtype", TYPES[:2], ids=IDS[:2])
+@pytest.mark.parametrize("m,n", [(30, 40), (128, 500), (300, 260), (2500, 20)])
+def test_newton_schulz_norm_past_the_type_s_range(dtype, m, n):
+    """Elements below 2^127 whose norm is above 2^128: the formula's X is an ordinary matrix."""
+    from sgnn_amd import muon
+    g = (normal((m, n), 1).clamp(-3.5, 3.5) * 2.0 ** 125).to(dtype)
+    assert float(g.double().norm()) > 2.0 ** 128
+    for steps in (0, 5):
+        ref = ns64(g, steps)
+        got = muon.newton_schulz(g.cuda(), steps=steps).double().cpu()
+        assert float((got - ref).norm() / ref.norm()) <= ns_tol(ref, dtype, m, n), steps
+
+
 def test_newton_schulz_refuses():
     from sgnn_amd import muon
     x = torch.zeros(3, 4, device="cuda")
