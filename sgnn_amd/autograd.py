@@ -249,35 +249,70 @@ class _MLP(torch.autograd.Function):
         return (None, None, dx, dres, *grads)
 
 
-_ACTIVATION_NAMES = {nn.ReLU: "relu", nn.SiLU: "silu", nn.Identity: "none"}
+_HALF = (torch.bfloat16, torch.float16)
 
 
 def _activation_name(m: nn.Module) -> str:
     if isinstance(m, nn.GELU):
         return "gelu" if m.approximate == "none" else "gelu_tanh"
-    name = _ACTIVATION_NAMES.get(type(m))
-    if name is None:
-        raise NotImplementedError(f"no kernel for the activation {m}")
-    return name
+    for kind, name in ((nn.ReLU, "relu"), (nn.SiLU, "silu"), (nn.Identity, "none")):
+        if isinstance(m, kind):
+            return name
+    raise NotImplementedError(f"no kernel for the activation {m}")
+
+
+def _relu_chain(body: nn.Module) -> bool:
+    """Whether an MLP is what the fp32 ReLU kernels compute: Linear, ReLU, Linear ... Linear (, Identity), none of
+    them with 16-bit parameters."""
+    linear_next = True
+    for m in body._modules.values():
+        if isinstance(m, nn.Linear):
+            if not linear_next or any(p is not None and p.dtype in _HALF for p in m._parameters.values()):
+                return False
+            linear_next = False
+        elif linear_next:
+            return False
+        elif type(m) is nn.ReLU:
+            linear_next = True
+        elif type(m) is not nn.Identity:
+            return False
+    return not linear_next
 
 
 def needs_typed(module: nn.Module) -> bool:
-    """Whether an MLP (or a module of them) is one the fp32 ReLU kernels do not compute: 16-bit
-    parameters, or build_mlp's `activation` (graph_network.py:7-45) set to GELU or SiLU."""
-    return (any(isinstance(m, (nn.GELU, nn.SiLU)) for m in module.modules())
-            or any(p.dtype in (torch.bfloat16, torch.float16) for p in module.parameters()))
+    """Whether a module holds an MLP that the fp32 ReLU kernels do not compute: 16-bit parameters, or another
+    `activation` or `output_activation` of build_mlp (graph_network.py:7-45).  Asked at every call (a module's parts
+    may be replaced), so it walks the tree by hand: 85 us for the 220 modules of a ten-layer EncodeProcessDecode,
+    where module.modules() and parameters() take 490."""
+    children = module._modules
+    for first in children.values():
+        if isinstance(first, nn.Linear) and isinstance(module, nn.Sequential):
+            return not _relu_chain(module)
+        break
+    for p in module._parameters.values():
+        if p is not None and p.dtype in _HALF:
+            return True
+    for m in children.values():
+        if m is not None and needs_typed(m):
+            return True
+    return False
 
 
 def _typed_mlp(body: nn.Module, ln: Optional[nn.Module], x: torch.Tensor, residual: Optional[torch.Tensor]):
     """The same MLP on the typed operators, in the type of its parameters (x and residual are cast to it)."""
-    layers = [m for m in body.modules() if not list(m.children())]   # Linear, activation, Linear, activation ...
-    lins = [m for m in layers if isinstance(m, nn.Linear)]
-    t = lins[0].weight.dtype
-    h = x.to(t)
-    for i, m in enumerate(layers):
+    t = _linears(body)[0].weight.dtype
+    h, lin = x.to(t), None
+    for m in [m for m in body.modules() if not m._modules]:   # Linear, activation, Linear, activation ...
         if isinstance(m, nn.Linear):
-            after = layers[i + 1] if i + 1 < len(layers) and not isinstance(layers[i + 1], nn.Linear) else nn.Identity()
-            h = functional.linear(h, m.weight, m.bias, _activation_name(after))
+            if lin is not None:
+                h = functional.linear(h, lin.weight, lin.bias)
+            lin = m
+        elif lin is None:
+            raise NotImplementedError(f"no kernel for {m} without a Linear before it")
+        else:
+            h, lin = functional.linear(h, lin.weight, lin.bias, _activation_name(m)), None
+    if lin is not None:
+        h = functional.linear(h, lin.weight, lin.bias)
     if ln is not None:
         return functional.layer_norm(h, ln.weight, ln.bias, residual.to(t) if residual is not None else None, ln.eps)
     if residual is not None:
@@ -287,7 +322,7 @@ def _typed_mlp(body: nn.Module, ln: Optional[nn.Module], x: torch.Tensor, residu
 
 def mlp(seq: nn.Module, has_ln: bool, x: torch.Tensor, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A reference-layout Sequential(build_mlp[, LayerNorm]) on rows x (any widths / depth).  fp32 with ReLU:
-    the chain above; 16-bit parameters, GELU or SiLU: functional.linear / layer_norm in the parameters' type."""
+    the chain above; 16-bit parameters or other activations: functional.linear / layer_norm in the parameters' type."""
     if has_ln:
         lins, ln = _linears(seq[0]), seq[1]
         params = [t for l in lins for t in (l.weight, l.bias)] + [ln.weight, ln.bias]
@@ -299,7 +334,7 @@ def mlp(seq: nn.Module, has_ln: bool, x: torch.Tensor, residual: Optional[torch.
     if x.shape[1] != lins[0].in_features:
         raise ValueError(f"MLP input width {x.shape[1]} != {lins[0].in_features}")
     body = seq[0] if has_ln else seq
-    if params[0].dtype in (torch.bfloat16, torch.float16) or any(type(m) in (nn.GELU, nn.SiLU) for m in body.children()):
+    if not _relu_chain(body):
         return _typed_mlp(body, seq[1] if has_ln else None, x, residual)
     return _MLP.apply(len(lins), has_ln, _c(x), residual, *params)
 

@@ -70,12 +70,28 @@ def mlp_struct(seq: nn.Module, has_ln: bool) -> SgnnMlp:
                    b3=lin[2].bias.data_ptr() if len(lin) == 3 else 0)
 
 
+def param_key(module: nn.Module) -> tuple:
+    """The addresses of a module's parameters; by hand, as module.parameters() takes 250 us for the 160 of a ten-layer
+    EncodeProcessDecode, this 140."""
+    out = []
+
+    def walk(m):
+        for p in m._parameters.values():
+            if p is not None:
+                out.append(p.data_ptr())
+        for c in m._modules.values():
+            if c is not None:
+                walk(c)
+    walk(module)
+    return tuple(out)
+
+
 class ParamPack:
     """The ctypes parameter structs of one EncodeProcessDecode, rebuilt only
     when a parameter tensor is replaced (e.g. after .to())."""
 
     def __init__(self, epd: nn.Module):
-        self.key = tuple(p.data_ptr() for p in epd.parameters())
+        self.key = param_key(epd)
         self.enc_node = mlp_struct(epd._encoder.node_fn, True)
         self.enc_edge = mlp_struct(epd._encoder.edge_fn, True)
         self.edge = [mlp_struct(g.edge_fn, True) for g in epd._processor.gnn_stacks]
@@ -90,7 +106,7 @@ class ParamPack:
 
     @staticmethod
     def get(epd: nn.Module) -> "ParamPack":
-        key = tuple(p.data_ptr() for p in epd.parameters())
+        key = param_key(epd)
         pack = getattr(epd, "_sgnn_pack", None)
         if pack is None or pack.key != key:
             pack = ParamPack(epd)

@@ -60,23 +60,23 @@ def predict_step(sim, inp: "engine.StepInputs", use_emb: bool):
                                 inp.vel_std, R, 1.0, sim._nparticle_types)
     ef = edge_features(g, pos, (T - 1) * d, T * d, d, R)
     ei = torch.stack([g.send[:g.num_edges], g.recv[:g.num_edges]])
-    return autograd.epd_forward(sim._encode_process_decode, nf, ei, ef)
+    return autograd.epd_forward(sim._encode_process_decode, nf, ei, ef).float()   # of 16-bit parameters too
 
 
 def fast_shapes(epd: nn.Module) -> bool:
     """True when the fused MFMA kernels implement this EncodeProcessDecode:
     hidden = latent in {64, 128}, nmlp_layers 1 or 2, <= 4 edge features and
-    the node-feature widths the encoder kernels tile (<= 96 / 64)."""
+    the node-feature widths the encoder kernels tile (<= 96 / 64), fp32 with ReLU."""
     H = epd.latent_dim
     return (H in (64, 128) and epd.mlp_hidden_dim == H and epd.nmlp_layers in (1, 2) and epd.nedge_in <= 4
-            and epd.nnode_in <= (96 if H == 64 else 64))
+            and epd.nnode_in <= (96 if H == 64 else 64) and not autograd.needs_typed(epd))
 
 
 def ms_fast_shapes(gnn: nn.Module) -> bool:
     """The same for MultiScaleGNN (nedge_out must equal latent_dim there)."""
     H = gnn.latent_dim
     return (H in (64, 128) and gnn.nedge_out == H and gnn.nmlp_layers in (1, 2) and gnn.nedge_in <= 4
-            and gnn.nnode_in <= (96 if H == 64 else 64))
+            and gnn.nnode_in <= (96 if H == 64 else 64) and not autograd.needs_typed(gnn))
 
 
 def block_fast_shapes(block: nn.Module) -> bool:
@@ -114,14 +114,14 @@ def processor_forward(proc: nn.Module, x, edge_index, edge_features):
 def epd_forward(epd: nn.Module, x, edge_index, edge_features) -> torch.Tensor:
     """EncodeProcessDecode.forward (graph_network.py:388-406): the fused chain in
     inference at the fast widths, else module by module (differentiable)."""
-    if not needs_grad(epd, x, edge_features) and fast_shapes(epd) and not autograd.needs_typed(epd):
+    if not needs_grad(epd, x, edge_features) and fast_shapes(epd):
         return engine.epd_forward(epd, x, edge_index, edge_features)
     return autograd.epd_forward(epd, x, edge_index, edge_features)
 
 
 def ms_gnn_forward(gnn: nn.Module, *args) -> torch.Tensor:
     """MultiScaleGNN.forward (multi_scale_gnn.py:277-326)."""
-    if not needs_grad(gnn, *args) and ms_fast_shapes(gnn) and not autograd.needs_typed(gnn):
+    if not needs_grad(gnn, *args) and ms_fast_shapes(gnn):
         from .multi_scale import ms_engine
         return ms_engine.gnn_forward(gnn, *args)
     return autograd.ms_gnn_forward(gnn, *args)

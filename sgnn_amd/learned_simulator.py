@@ -196,15 +196,15 @@ class LearnedSimulator(nn.Module):
         return next_pos, pred[:, -1]
 
     def _fast_path(self) -> bool:
-        """The fused MFMA kernels implement this model's widths (else generic.py)."""
+        """The fused MFMA kernels implement this model: its widths, fp32, ReLU (else generic.py)."""
         return generic.fast_shapes(self._encode_process_decode)
 
     def rollout_runner(self, window: torch.Tensor, nparticles_per_example, particle_types, nsteps: int):
         """Device-resident autoregressive rollout of `nsteps` predict_positions
         steps from `window` (evaluate.py:117-145): one sgnn_rollout call."""
         if not self._fast_path():
-            raise NotImplementedError("the device rollout needs the fused kernels' widths (hidden = latent "
-                                      "in {64, 128}); evaluate.rollout steps predict_positions instead")
+            raise NotImplementedError("the device rollout needs the fused kernels' shapes (hidden = latent "
+                                      "in {64, 128}, fp32, ReLU); evaluate.rollout steps predict_positions instead")
         inp, use_emb = self._step_inputs(window, nparticles_per_example, particle_types)
         n, T, d = inp.pos_seq.shape
         ws = self._workspace(n, T, inp.pos_seq.device)

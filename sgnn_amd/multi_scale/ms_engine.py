@@ -51,7 +51,7 @@ class ParamPack:
 
     def __init__(self, gnn):
         ms = engine.mlp_struct
-        self.key = tuple(p.data_ptr() for p in gnn.parameters())
+        self.key = engine.param_key(gnn)
         chain = gnn.chain()
         self.edge = [ms(b.edge_fn, True) for b in chain]
         self.node = [ms(b.node_fn, True) for b in chain]
@@ -62,7 +62,7 @@ class ParamPack:
 
     @staticmethod
     def get(gnn) -> "ParamPack":
-        key = tuple(p.data_ptr() for p in gnn.parameters())
+        key = engine.param_key(gnn)
         pk = getattr(gnn, "_sgnn_pack", None)
         if pk is None or pk.key != key:
             pk = ParamPack(gnn)

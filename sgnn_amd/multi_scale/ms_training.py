@@ -287,10 +287,10 @@ class MultiScaleTrainer:
                  lr_decay_steps: int = 15000, noise_std: float = 0.02,
                  loss_weight_position: float = 1.0, loss_weight_strain: float = 1.0,
                  group=None, nslab: int = MS_NSLAB, optimizer: str = "adam"):
-        self.fused = fused_trainable(simulator)
         self.sim = simulator
         self.gnn = simulator._multi_scale_gnn
-        self.flat = FlatParams(simulator)
+        self.flat = FlatParams(simulator)   # fp32 from here on
+        self.fused = fused_trainable(simulator)
         self.opt = make_optimizer(optimizer, self.flat, simulator, lr_init)
         self.grads = {k: p.grad for k, p in simulator.named_parameters()}
         self.lr_init, self.lr_decay, self.lr_decay_steps = lr_init, lr_decay, lr_decay_steps

@@ -174,7 +174,7 @@ class MultiScaleSimulator(nn.Module):
         return ws
 
     def _fast_path(self) -> bool:
-        """The fused MFMA chain implements this model's widths (else generic.py)."""
+        """The fused MFMA chain implements this model: its widths, fp32, ReLU (else generic.py)."""
         return generic.ms_fast_shapes(self._multi_scale_gnn)
 
     def _run(self, position_sequence, particle_types, window_out=None):
@@ -219,7 +219,7 @@ class MultiScaleSimulator(nn.Module):
         ef = {k: generic.edge_features(graphs[k], pos, (T - 1) * d, T * d, d, r)
               for k, r in (("g2m", rg), ("m2m", rm), ("m2g", rg))}
         return autograd.ms_gnn_forward(self._multi_scale_gnn, nf, None, ef["g2m"], None, ef["m2m"], None, ef["m2g"],
-                                       graphs=egs)
+                                       graphs=egs).float()   # of 16-bit parameters too
 
     def rollout_runner(self, window: torch.Tensor, particle_types, nsteps: int):
         """Device-resident rollout of `nsteps` predict_positions steps from

@@ -225,9 +225,9 @@ class Trainer:
                  group=None, nslab: Optional[int] = None, optimizer: str = "adam"):
         self.sim = simulator
         self.epd = simulator._encode_process_decode
-        # the fused kernels where they are built for the widths, else the width-generic autograd path
+        self.flat = training.FlatParams(simulator)   # fp32 from here on
+        # the fused kernels where they are built for the model, else the width-generic autograd path
         self.fused = training.fused_trainable(self.epd, simulator._nparticle_types)
-        self.flat = training.FlatParams(simulator)
         self.opt = make_optimizer(optimizer, self.flat, simulator, lr_init)   # "adam" (train.py:199) or "muon"
         self.grads: Dict[str, torch.Tensor] = {k: p.grad for k, p in simulator.named_parameters()}
         self.lr_init, self.lr_decay, self.lr_decay_steps = lr_init, lr_decay, lr_decay_steps

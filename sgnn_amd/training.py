@@ -30,7 +30,8 @@ NODE_NSLAB = 256     # node-level backward kernels (128 measured slower: fewer C
 class FlatParams:
     """Point every parameter of `module` into one flat fp32 buffer, and its
     `.grad` into one flat gradient buffer (+ the step's loss sums in its tail):
-    one RCCL all-reduce, one Adam launch."""
+    one RCCL all-reduce, one Adam launch.  Training is in fp32: parameters of
+    another type become fp32 ones."""
 
     def __init__(self, module: nn.Module):
         params = list(module.parameters())

@@ -1056,3 +1056,165 @@ def test_trainer_takes_muon(tmp_path):
     adam = T.Trainer(sim2)
     with pytest.raises(ValueError, match="Muon"):
         T.Trainer(sim2, optimizer="muon").opt.load_state_dict(adam.opt.state_dict())
+
+
+def _with_activation(module, make):
+    """Every ReLU of the module's MLPs replaced."""
+    for m in module.modules():
+        if isinstance(m, torch.nn.Sequential):
+            for name, child in list(m.named_children()):
+                if type(child) is torch.nn.ReLU:
+                    setattr(m, name, make())
+    return module
+
+
+@pytest.mark.parametrize("H,nmlp,activation", [(64, 1, "gelu"), (128, 2, "silu")])
+def test_simulators_and_trainers_honour_the_activation(H, nmlp, activation, monkeypatch):
+    """A LearnedSimulator at the fused kernels' widths whose MLPs have another activation: one inference step and one
+    Trainer step (loss and every gradient) against the oracle with that activation."""
+    from oracle import sgnn_oracle as O
+    from sgnn_amd.train import Trainer
+    from tests.test_gpu_autograd import _check_grads, _close, _setup
+    sim, osim, state, seq, types, _ = _setup(H, H, nmlp, 2)
+    f = torch.nn.functional
+    monkeypatch.setattr(f, "relu", getattr(f, activation))
+    _with_activation(sim, {"gelu": torch.nn.GELU, "silu": torch.nn.SiLU}[activation])
+    pos, nxt = torch.from_numpy(seq[:, :11]), torch.from_numpy(seq[:, 11])
+    n = pos.shape[0]
+    strain = torch.from_numpy(np.random.default_rng(1).normal(0, 1, n).astype(np.float32))
+    noise = O.random_walk_noise(pos, 0.02, generator=torch.Generator().manual_seed(7))
+    with torch.no_grad():
+        want, want_strain = osim.predict_positions(pos, [n], types)
+        got, got_strain = sim.predict_positions(pos.cuda(), [n], types.cuda())
+        _close(got.cpu().numpy(), want.numpy(), what="positions")
+        _close(got_strain.cpu().numpy(), want_strain.numpy(), what="strain")
+        acc = sim.predict_accelerations(nxt.cuda(), noise.cuda(), pos.cuda(), [n], types.cuda())[0]
+    pa, ta, ps = osim.predict_accelerations(nxt, noise, pos, [n], types)
+    _close(acc.cpu().numpy(), pa.detach().numpy(), what="accelerations")
+    with pytest.raises(NotImplementedError):
+        sim.rollout_runner(pos.cuda(), [n], types.cuda(), 2)
+    ref_loss = O.training_loss(pa, ta, ps, strain)
+    ref_loss.backward()
+    tr = Trainer(sim, lr_init=1e-3)
+    out = tr.train_step(pos.cuda(), nxt.cuda(), strain.cuda(), [n], types.cuda(), noise=noise.cuda())
+    assert abs(float(out["loss"]) - ref_loss.item()) <= 2e-5 * abs(ref_loss.item())
+    _check_grads(sim.named_parameters(), state)
+
+
+def _multi_scale(nedge_out=64):
+    from oracle import multi_scale_oracle as MO
+    from sgnn_amd import synthetic
+    from sgnn_amd.multi_scale import MultiScaleSimulator, build_static_multi_scale_graph
+    dim, T, L = 2, 6, 2
+    seq = synthetic.trajectory(synthetic.lattice_2d(30, 12, x0=-1.75), T + 1, seed=13)
+    st = synthetic.normalization_stats(dim, noise_std=0.02)
+    stats = {k: {kk: torch.from_numpy(vv) for kk, vv in v.items()} for k, v in st.items()}
+    torch.manual_seed(21)
+    sim = MultiScaleSimulator(dim, (T - 1) * dim + 1, dim + 1, nedge_out, 64, L, 2, stats, 1, 9, 2, 2, 2.0)
+    state = {k: v.detach().clone().requires_grad_(True) for k, v in sim.state_dict().items()}
+    osim = MO.MultiScaleOracle(state, dim, L, stats, MO.create_all_edges(torch.from_numpy(seq[:, 0]), 2, 2, 2.0), 2, 2.0, 1, 2)
+    sim = sim.cuda()
+    sim.set_static_graph(build_static_multi_scale_graph(torch.from_numpy(seq[:, 0]).cuda(), 2, 2, 2.0))
+    return sim, osim, state, torch.from_numpy(seq[:, :T]), torch.from_numpy(seq[:, T])
+
+
+def test_multi_scale_simulators_and_trainers_honour_the_activation(monkeypatch):
+    """The same of a MultiScaleSimulator at the fused chain's widths."""
+    from oracle import sgnn_oracle as O
+    from sgnn_amd.multi_scale.ms_training import MultiScaleTrainer
+    from tests.test_gpu_autograd import _check_grads, _close
+    sim, osim, state, pos, nxt = _multi_scale()
+    monkeypatch.setattr(torch.nn.functional, "relu", torch.nn.functional.gelu)
+    _with_activation(sim, torch.nn.GELU)
+    n = pos.shape[0]
+    strain = torch.from_numpy(np.random.default_rng(4).normal(0, 1, n).astype(np.float32))
+    noise = O.random_walk_noise(pos, 0.02, generator=torch.Generator().manual_seed(5))
+    pa, ta, ps = osim.predict_accelerations(nxt, noise, pos)
+    with torch.no_grad():
+        got = sim.predict_accelerations(nxt.cuda(), noise.cuda(), pos.cuda(), [n], None)
+    _close(got[0].cpu().numpy(), pa.detach().numpy(), what="accelerations")
+    _close(got[2].cpu().numpy(), ps.detach().numpy(), what="strain")
+    ref_loss = O.training_loss(pa, ta, ps, strain)
+    ref_loss.backward()
+    tr = MultiScaleTrainer(sim, lr_init=1e-3)
+    out = tr.train_step(pos.cuda(), nxt.cuda(), strain.cuda(), noise=noise.cuda())
+    assert abs(float(out["loss"]) - ref_loss.item()) <= 2e-5 * abs(ref_loss.item())
+    _check_grads(sim.named_parameters(), state)
+
+
+def test_multi_scale_trainer_takes_muon():
+    """MultiScaleTrainer(optimizer="muon"): its step is Muon's on the gradient that it formed."""
+    from sgnn_amd import muon, training
+    from sgnn_amd.multi_scale.ms_training import MultiScaleTrainer
+    (sim, _, _, pos, nxt), (other, *_) = _multi_scale(), _multi_scale()
+    tr = MultiScaleTrainer(sim, lr_init=1e-3, optimizer="muon")
+    assert tr.fused and sum(tr.opt.is_matrix) > 10
+    flat = training.FlatParams(other)
+    opt = muon.Muon(flat, other, 1e-3)
+    for _ in range(2):
+        opt.lr = tr.opt.lr   # the schedule sets the next step's after each
+        tr.train_step(pos.cuda(), nxt.cuda(), torch.zeros(pos.shape[0], device="cuda"))
+        flat.grad.copy_(tr.flat.grad)
+        before = flat.param.clone()
+        opt.step()
+        assert torch.equal(flat.param, tr.flat.param) and not torch.equal(flat.param, before)
+
+
+def test_activations_of_derived_classes_and_unknown_ones():
+    """A class derived from nn.GELU is GELU (it got ReLU); an activation that no kernel computes is refused everywhere,
+    and so is one where the ReLU kernels have none."""
+    from sgnn_amd import graph_network as G
+
+    class Named(torch.nn.GELU):
+        pass
+
+    x, e = normal((20, 7), 1).cuda(), normal((30, 3), 2).cuda()
+    outs = []
+    for make in (torch.nn.GELU, Named):
+        torch.manual_seed(5)
+        outs.append(_with_activation(G.Encoder(7, 40, 3, 40, 1, 40).cuda(), make)(x, e))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    with pytest.raises(NotImplementedError, match="Tanh"):
+        _with_activation(G.Encoder(7, 40, 3, 40, 1, 40).cuda(), torch.nn.Tanh)(x, e)
+    ei = torch.zeros(2, 30, dtype=torch.int64, device="cuda")
+    epd = _with_activation(G.EncodeProcessDecode(7, 3, 3, 64, 2, 1, 64).cuda(), torch.nn.Tanh)
+    with torch.no_grad(), pytest.raises(NotImplementedError, match="Tanh"):
+        epd(x, ei, e)
+    # an output activation
+    dec = G.Decoder(40, 3, 1, 40).cuda()
+    dec.node_fn = G.build_mlp(40, [40], 3, output_activation=torch.nn.ReLU).cuda()
+    h = normal((50, 40), 3).cuda()
+    got = dec(h)
+    p = dict(dec.node_fn.named_parameters())
+    ref = torch.relu(torch.relu(h.double() @ p["NN-0.weight"].double().T + p["NN-0.bias"].double()) @ p["NN-1.weight"].double().T
+                     + p["NN-1.bias"].double())
+    within(got, ref.detach().cpu(), 84 * U * 40, "output activation")   # sums of 40 products of magnitude < 1
+
+
+def test_simulators_with_16_bit_parameters():
+    """A bf16 simulator at the fused kernels' widths computes in bf16 and returns fp32 (26 roundings of the type along the
+    chain: encoder 3, three blocks of 7, decoder 2); a Trainer makes its parameters fp32 and takes the fused kernels."""
+    from oracle import sgnn_oracle as O
+    from sgnn_amd.train import Trainer
+    from tests.test_gpu_autograd import _setup
+    sim, osim, state, seq, types, _ = _setup(64, 64, 1, 2)
+    sim = sim.bfloat16()
+    with torch.no_grad():
+        for v in state.values():
+            v.copy_(v.bfloat16().float())
+        pos, nxt = torch.from_numpy(seq[:, :11]), torch.from_numpy(seq[:, 11])
+        n = pos.shape[0]
+        zero = torch.zeros_like(pos)
+        want = osim.predict_accelerations(nxt, zero, pos, [n], types)
+        got = sim.predict_accelerations(nxt.cuda(), zero.cuda(), pos.cuda(), [n], types.cuda())
+        for a, b in ((got[0], want[0]), (got[2], want[2])):
+            assert a.dtype == torch.float32
+            assert float((a.cpu() - b).norm() / b.norm()) <= 26 * half_step(torch.bfloat16)
+        assert sim.predict_positions(pos.cuda(), [n], types.cuda())[0].dtype == torch.float32
+    tr = Trainer(sim, lr_init=1e-3)
+    assert tr.fused and all(p.dtype == torch.float32 for p in sim.parameters())
+    pa, ta, ps = osim.predict_accelerations(nxt, zero, pos, [n], types)
+    strain = torch.zeros(n)
+    out = tr.train_step(pos.cuda(), nxt.cuda(), strain.cuda(), [n], types.cuda(), noise=zero.cuda())
+    ref = O.training_loss(pa, ta, ps, strain)
+    assert abs(float(out["loss"]) - ref.item()) <= 2e-5 * abs(ref.item())
