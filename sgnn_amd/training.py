@@ -655,6 +655,8 @@ class Adam:
             raise ValueError(f"optimizer state has {sum(len(g['params']) for g in groups)} parameters "
                              f"in {len(groups)} groups; this model has {len(f.order)} in one")
         g = groups[0]
+        if any(k not in st for st in sd["state"].values() for k in ("step", "exp_avg", "exp_avg_sq")):
+            raise ValueError("not the state of an Adam optimiser: it lacks step, exp_avg or exp_avg_sq")
         self.lr, self.betas, self.eps = float(g["lr"]), tuple(g["betas"]), float(g["eps"])
         steps = set()
         with torch.no_grad():

@@ -132,6 +132,22 @@ def test_muon_kernels_refuse(lib, bad):
         assert lib.sgnn_muon_apply(a["segs"], a["nseg"], a["param"], a["update"], 0.1, 0.0, None) == INVALID
 
 
+def test_optimizers_refuse_each_other_s_state():
+    """A checkpoint resumed with the other optimiser: refused before anything is changed."""
+    from sgnn_amd import training
+    module = torch.nn.Sequential(torch.nn.Linear(20, 30), torch.nn.Linear(30, 3))
+    flat = training.FlatParams(module)
+    made = {"adam": training.Adam(flat, 0.5), "muon": muon.Muon(flat, module, 0.5)}
+    for opt in made.values():
+        opt.step_count = 3
+        opt.exp_avg.fill_(2.0)
+    for name, other in (("adam", "muon"), ("muon", "adam")):
+        with pytest.raises(ValueError, match="optimiser"):
+            made[name].load_state_dict(dict(made[other].state_dict(), lr=9.0))
+        assert made[name].lr == 0.5 and made[name].step_count == 3 and (made[name].exp_avg == 2.0).all()
+        made[name].load_state_dict(made[name].state_dict())
+
+
 def test_optimizer_names():
     with pytest.raises(ValueError, match="adam"):
         muon.make_optimizer("sgd", None, None, 0.1)
