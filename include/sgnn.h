@@ -555,7 +555,8 @@ typedef enum sgnn_act {
 /* y[M][N] = act(z) (+ residual), z = x[M][K] w[N][K]^T (+ bias[N]): one nn.Linear of build_mlp
  * (graph_network.py:7-45) with its activation and the block's residual (:176) in the epilogue.
  * bias, residual and slope may be NULL.  slope (dense [M][N] fp32, whatever dtype is) receives act'(z) for the
- * backward pass.  K = 0 gives z = bias.  y and slope may overlap no input but that residual may be y itself.
+ * backward pass.  K = 0 gives z = bias.  M up to 2^30, N and K up to 2^25.  y and slope may overlap no input but that
+ * residual may be y itself.
  * workspace: sgnn_linear_workspace_bytes(dtype, M, N, K) bytes, 256-B aligned. */
 size_t sgnn_linear_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K);
 int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,

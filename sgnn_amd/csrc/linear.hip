@@ -118,6 +118,10 @@ __global__ __launch_bounds__(kSumThreads) void k_bias_grad(const float* partial,
   sum_partials(partial, nblk, N, [&](int64_t c, float s) { out[c] = from_float<T>(s); });
 }
 
+// A launch has fewer than 2^32 threads: k_bias_grad takes 64 per column, the products' tiles 4 per row of one column.
+constexpr int64_t kMostRows = (int64_t)1 << 30, kMostCols = (int64_t)1 << 25;
+bool too_many(int64_t M, int64_t N, int64_t K) { return M > kMostRows || std::max(N, K) > kMostCols; }
+
 bool act_ok(int32_t act) { return act >= SGNN_ACT_NONE && act <= SGNN_ACT_SILU; }
 size_t pad256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -175,6 +179,7 @@ extern "C" int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const
   using namespace sgnn;
   if (!dtype_ok(dtype) || !act_ok(act)) return set_error(SGNN_ERR_INVALID, "linear: unknown dtype or activation");
   if (M < 0 || N < 0 || K < 0) return set_error(SGNN_ERR_INVALID, "linear: negative size");
+  if (too_many(M, N, K)) return set_error(SGNN_ERR_UNSUPPORTED, "linear: more than 2^30 rows or 2^25 columns");
   if (M == 0 || N == 0) return SGNN_OK;
   if (!y || ldy < N || (residual && ldr < N)) return set_error(SGNN_ERR_INVALID, "linear: bad output or residual");
   if (K > 0 && (!x || !w || ldx < K || ldw < K)) return set_error(SGNN_ERR_INVALID, "linear: bad operand");
@@ -201,6 +206,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   using namespace sgnn;
   if (!dtype_ok(dtype)) return set_error(SGNN_ERR_INVALID, "linear_bwd: unknown dtype");
   if (M < 0 || N < 0 || K < 0) return set_error(SGNN_ERR_INVALID, "linear_bwd: negative size");
+  if (too_many(M, N, K)) return set_error(SGNN_ERR_UNSUPPORTED, "linear_bwd: more than 2^30 rows or 2^25 columns");
   if (M > 0 && N > 0 && (!dy || ldd < N)) return set_error(SGNN_ERR_INVALID, "linear_bwd: bad dy");
   if (K > 0 && ((dx && N > 0 && (!w || ldw < K)) || (dw && M > 0 && (!x || ldx < K))))
     return set_error(SGNN_ERR_INVALID, "linear_bwd: bad operand");

@@ -28,6 +28,13 @@ def test_linear_refuses(lib, bad):
     assert "linear" in lib.sgnn_last_error().decode()
 
 
+@pytest.mark.parametrize("big", [dict(M=(1 << 30) + 1), dict(N=(1 << 25) + 1), dict(K=(1 << 25) + 1)])
+def test_linear_refuses_more_than_a_launch_holds(lib, big):
+    far = dict(ldx=1 << 40, ldw=1 << 40)
+    assert _linear(lib, **far, ldy=1 << 40, nws=1 << 62, **big) == _hip.SGNN_ERR_UNSUPPORTED
+    assert _linear_bwd(lib, **far, ldd=1 << 40, nws=1 << 62, **big) == _hip.SGNN_ERR_UNSUPPORTED
+
+
 def test_empty_calls_need_no_device(lib):
     assert _linear(lib, M=0) == _hip.SGNN_OK and _linear(lib, N=0) == _hip.SGNN_OK
     assert lib.sgnn_norm(0, 0, None, 4, 0, 4, None, None, None, 4, 1e-5, None, None, None, None) == _hip.SGNN_OK
