@@ -173,10 +173,10 @@ SGNN_DEV int planes_of(const GemmArgs& g, int* word) {
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 // NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
 // longer than memory; the small tile has four.
-// 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 292
-// to 330 us, dz w 230 to 260, dz^T x 234 to 260.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
+// 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 307
+// to 330 us, dy w 230 to 260, dy^T x 234 to 260; with two planes of dz 437 to 480 and 451 to 496.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
 // time, and the rest is LDS's latency after each block's barrier, which all waves meet together, and, forward, the
-// epilogue's 268 MB.  Memory is not waited for: four stages of 32 k took 334 / 248 / 244 us at their fastest, where these
+// epilogue's 402 MB.  Memory is not waited for: four stages of 32 k took 334 / 248 / 244 us at their fastest, where these
 // two of 64 k took 290 / 230 / 230; the next block's loads issued behind the first fragments' reads took 292 / 226 / 237.
 template <typename T, bool ACOLS, bool BCOLS, int BM, int BN, int WM, int WN, bool DIRECT, int NST>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
@@ -533,7 +533,7 @@ SGNN_DEV void redo_non_finite(const GemmArgs& g, f32x4 (&acc)[TM][TN], int64_t m
 // An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
 // are not finite are formed once more (redo_non_finite).
 // NST = 2 stages of LDS: the next block is split and written while this one's products run; a matrix instruction takes
-// 16 cycles, in which a wave issues three others (4096^3: 695 us, 198 TFLOP/s; 765 with one stage, where split and
+// 16 cycles, in which a wave issues three others (4096^3: 640 to 695 us, 198 to 215 TFLOP/s; 765 with one stage, where split and
 // products take turns and the two waves of a SIMD fall into step; other mixtures asked of the scheduler: 704 to 733).
 // NST = 1: half the LDS, so two workgroups per CU, one's epilogue beside the other's products: better where k is short
 // (200003 x 384 x 128, silu: 180 us against 211).
@@ -788,17 +788,27 @@ struct Plan {
   int bm, bn, nsplit;
 };
 
-// The larger tile moves fewer bytes per product through LDS and L2, the smaller ones fill the 256 CUs sooner; long
-// k is split over workgroups where the tiles alone leave CUs idle.
+// The larger tile moves fewer bytes per product through LDS and L2, the smaller ones fill the 256 CUs sooner.  Square
+// outputs, x w^T, in us:
+//   256 x 256 (16 bits) or 128 x 128, k 2048: 169 of the larger tiles 51 / 56, 100 of them 59 / 32; k 512: 196 tiles
+//   22.5 / 23.4, 169 21.9 / 21.3.
+//   256 x 128 (fp32) or 128 x 128, 512 of the larger tiles: k 1024 160 / 168, k 256 58 / 55; 128 of them, k 1024 66 / 68.
+//   128 x 128 or 64 x 64: 16 bits, k 1024: 144 of the larger tiles 15 / 16, 100 of them 23 / 10; k 16384: 36 tiles
+//   42 / 44, 1 tile 12 / 9.  fp32, k 512: 400 tiles 44 / 55, 144 34 / 26; k 4096: 36 tiles 41 / 49, 4 tiles 23 / 14.  With
+//   64 rows or columns half of the larger tile is empty (dw of 100000 rows, 64 x 192, fp32: 48 / 36).
+// k is split over workgroups where the tiles leave CUs idle: one workgroup per CU, and two where k is long enough to pay
+// for the partial sums (128 x 128, two / one, us: bf16 2048^2, k 1024 38 / 16; 1536^2, k 16384 91 / 164; fp32 2048^2,
+// k 512 49 / 36; 1536^2, k 1024 47 / 61).
 Plan plan_of(const Gemm& g) {
   const auto tiles = [&](int bm, int bn) { return ((g.M + bm - 1) / bm) * ((g.N + bn - 1) / bn); };
   const int bk = g.dtype == SGNN_F32 ? 32 : 64;
   Plan p{64, 64, 1};
-  if (g.dtype != SGNN_F32 && tiles(256, 256) >= 192) p = {256, 256, 1};
-  else if (g.dtype == SGNN_F32 && tiles(256, 128) >= 256 && g.K >= 1024) p = {256, 128, 1};
-  else if (tiles(128, 128) >= 128 || g.K >= 2048) p = {128, 128, 1};
-  // what is resident at once: one workgroup per CU of the large tiles, two of the others
-  const int64_t blocks = (g.K + bk - 1) / bk, wgs = p.bm == 256 ? 256 : 512;
+  const bool f32 = g.dtype == SGNN_F32;
+  const bool long_k = std::min(g.M, g.N) > 64 && g.K >= (f32 ? 2048 : 8192) && tiles(128, 128) * g.K >= (f32 ? 1 << 16 : 1 << 18);
+  if (!f32 && tiles(256, 256) >= 192) p = {256, 256, 1};
+  else if (f32 && tiles(256, 128) >= 256 && g.K >= 1024) p = {256, 128, 1};
+  else if (tiles(128, 128) >= (f32 ? 256 : 128) || long_k) p = {128, 128, 1};
+  const int64_t blocks = (g.K + bk - 1) / bk, wgs = p.bm != 256 && blocks >= (f32 ? 32 : 64) ? 512 : 256;
   const int64_t want = wgs / std::max<int64_t>(1, tiles(p.bm, p.bn));
   p.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({want, blocks / 8, 256}));
   return p;

@@ -131,13 +131,16 @@ struct NsGemm {
   Group last;
 };
 
-// BT x BT outputs by four waves.  SYM: the product is symmetric; only the tiles
-// on and above the diagonal are formed and each is written to both sides.
+// BT x BT outputs by four waves.  SYM: the product is symmetric; only the tiles on and above the diagonal are formed and
+// each is written to both sides.
 // KG groups of four waves take every KG-th block of k each, with LDS of their own, and are added in order at the end:
 // these products have few tiles (36 of 128 x 128 in the triangle of 1024), and one wave per SIMD leaves memory's and
-// LDS's latencies in the open.  bf16, 2048 x 4096: X X^T 38 us (136 tiles of 256 CUs; 18 GFLOP formed), G^2 26 us, Q X
-// 43 us (34 GFLOP, 800 TFLOP/s): bounded by the CUs without a tile and by LDS reads beside the matrix instructions.
-template <bool AC, bool BC, int BT, bool SYM, int KG>
+// LDS's latencies in the open.  One group instead of two, all five steps in us: 1024 x 1024 301 / 225, 2048 x 4096
+// 1507 / 1228, 4096 x 4096 5253 / 4646; two of 2048 x 4096 2379 / 2420.  2048 x 4096: X X^T 82 to 87 us
+// (136 tiles of 256 CUs; three times 18 GFLOP formed), G^2 54 to 57, Q X 107 to 113 (three times 34 GFLOP, 910 to 960
+// TFLOP/s): bounded by the CUs without a tile and by LDS reads beside the matrix instructions.
+constexpr int KG = 2;
+template <bool AC, bool BC, int BT, bool SYM>
 __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
   constexpr int P = kPlanes, BK = 32, kThreads = 256, TT = BT / 2 / 16;
   using TA = Tile16<BT, BK, AC>;
@@ -211,19 +214,17 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
       for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
   }
   __syncthreads();
-  if constexpr (KG > 1) {
-    f32x4* sums = reinterpret_cast<f32x4*>(all) + ((kg - 1) * 4 + w) * TT * TT * 64 + l;
-    static_assert((KG - 1) * 4 * TT * TT * 64 * 16 <= 2 * KG * kStage, "the groups' sums fit");
-    if (kg > 0)
+  f32x4* sums = reinterpret_cast<f32x4*>(all) + ((kg - 1) * 4 + w) * TT * TT * 64 + l;
+  static_assert((KG - 1) * 4 * TT * TT * 64 * 16 <= 2 * KG * kStage, "the groups' sums fit");
+  if (kg > 0)
 #pragma unroll
-      for (int i = 0; i < TT * TT; ++i) sums[64 * i] = acc[i / TT][i % TT];
-    __syncthreads();
-    if (kg > 0) return;
-    for (int q = 1; q < KG; ++q)
+    for (int i = 0; i < TT * TT; ++i) sums[64 * i] = acc[i / TT][i % TT];
+  __syncthreads();
+  if (kg > 0) return;
+  for (int q = 1; q < KG; ++q)
 #pragma unroll
-      for (int i = 0; i < TT * TT; ++i) acc[i / TT][i % TT] += sums[(q * 4 * TT * TT + i) * 64];
-    // the epilogue's buffers are this wave's own part of what it has read
-  }
+    for (int i = 0; i < TT * TT; ++i) acc[i / TT][i % TT] += sums[(q * 4 * TT * TT + i) * 64];
+  // the epilogue's buffers are this wave's own part of what it has read
   // through LDS by 16 rows of m (as in gemm.hip), so that every load and store is 16 bytes of a row
   constexpr int kPieces = 4 * TT, kMask = kPieces - 1;
   float* buf = reinterpret_cast<float*>(all) + w * TT * TT * 256;
@@ -293,21 +294,12 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
   }
 }
 
-// Up to this many 128 x 128 tiles of one matrix, a workgroup of k_ns_gemm splits k over two groups of waves: a CU then has
-// one tile at most and only its own waves hide its latency. Above it the groups of one tile cost LDS that a second tile
-// would use: a product of 512 tiles (2048 x 2048 by 2048 x 4096) took 47 us with two groups and 42 with one, the symmetric
-// one of 136 tiles 38 and 45.  Neither the batch nor the tile's size decides, so a matrix gets the same bits in any batch.
-constexpr int kFewTiles = 256;
-
 template <bool AC, bool BC, bool SYM>
 void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
   const auto tiles = [&](int m, int n) { return SYM ? m * (m + 1) / 2 : m * n; };
   const dim3 grid((unsigned)tiles(g.tiles_m, g.tiles_n), 1, (unsigned)count);
-  const int per = 128 / bt;
-  const bool few = tiles((g.tiles_m + per - 1) / per, (g.tiles_n + per - 1) / per) <= kFewTiles;
-  const auto go = [&](auto kernel, int threads) { hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, s, g); };
-  if (bt == 128) few ? go(k_ns_gemm<AC, BC, 128, SYM, 2>, 512) : go(k_ns_gemm<AC, BC, 128, SYM, 1>, 256);
-  else few ? go(k_ns_gemm<AC, BC, 64, SYM, 2>, 512) : go(k_ns_gemm<AC, BC, 64, SYM, 1>, 256);
+  if (bt == 128) hipLaunchKernelGGL((k_ns_gemm<AC, BC, 128, SYM>), grid, dim3(256 * KG), 0, s, g);
+  else hipLaunchKernelGGL((k_ns_gemm<AC, BC, 64, SYM>), grid, dim3(256 * KG), 0, s, g);
 }
 
 // ----------------------------------------------------------------------------- small matrices
@@ -599,9 +591,11 @@ int launch_small(const sgnn_matrix* mats, int count, int32_t steps, float a, flo
 // ----------------------------------------------------------------------------- short and long matrices
 // A matrix whose short side fits as above but whose long one does not: a workgroup per kChunk of its long side.  G is the
 // sum of the chunks' X_c X_c^T, so one launch per step does: add the chunks' shares of G (in order, every workgroup for
-// itself), form Q, X_c <- Q X_c, and its share of the next G -- 2 + steps launches for 2 + 3 steps.  Ten 128 x 384 fp32:
-// 98 us against 104 by tiles, 12 to 16 us a launch, bounded as the small kernel is; beyond 16 chunks the sums of G's
-// shares, which every workgroup reads, cost more than the launches saved.
+// itself), form Q, X_c <- Q X_c, and its share of the next G -- 2 + steps launches for 2 + 3 steps, 12 to 16 us each,
+// bounded as the small kernel is.  fp32 by chunks / by tiles, us: one 32 x 2048 53 / 143, 64 x 1024 57 / 100, 128 x 384
+// 92 / 87, 128 x 2048 132 / 163; ten 128 x 384 98 / 98, 128 x 2048 160 / 210; 32 of 128 x 384 110 / 115, 128 x 2048
+// 384 / 390.  Beyond 16 chunks the sums of G's shares, which every workgroup reads, can cost more than the launches saved:
+// 128 x 4096 177 / 256, but 32 of them 833 / 656, and the number of matrices must not decide, or it would their bits.
 //   shares [matrix][chunk][32 x 32 block of G][4][lane] as the accumulators hold them; x: planes [matrix][m][ld]
 constexpr int kChunk = 128, kMaxChunks = 16;
 inline bool chunk_ok(int rows, int cols) {
@@ -755,8 +749,9 @@ struct NsLayout {
   size_t norms, x, g, total;
   NsLayout(int32_t r, int32_t c, int count) {
     const int64_t small = std::min(r, c), large = std::max(r, c);
-    // 128-tiles read half as much per product; the smaller ones pad less and fill the CUs sooner
-    bt = (small * large + 128 * 128 - 1) / (128 * 128) * count >= 192 && small > 64 ? 128 : 64;
+    // 128-tiles read half as much per product; the smaller ones pad less and fill the CUs sooner (fp32, 128 / 64, us:
+    // 2048 x 2048 763 / 885, twelve 512 x 768 411 / 399, 1536 x 2048 643 / 538, 512 x 512 267 / 140)
+    bt = (small * large + 128 * 128 - 1) / (128 * 128) * count >= 256 && small > 64 ? 128 : 64;
     rows = (r + bt - 1) / bt * bt, cols = (c + bt - 1) / bt * bt, side = std::min(rows, cols);
     norms = pad256(sizeof(double) * kNormParts * count);
     x = pad256(2 * sizeof(f16_t) * rows * cols * count);
