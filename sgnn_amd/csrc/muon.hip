@@ -121,6 +121,22 @@ __global__ __launch_bounds__(256) void k_ns_begin(Group g, const double* part, i
   }
 }
 
+// acc[j] += the products of 32 k: A's rows a_hi + a_lo by B's b[0][j] + b[1][j].  A matrix instruction lines its products
+// up with what it adds them to and drops what falls below: with the running sum as its addend a sum of some thousand
+// products lost 1e-6 of itself, always towards 0.  So each starts from zero and its 32 k are added by the vector units.
+template <int N>
+SGNN_DEV void add_products(f32x4 (&acc)[N], const s16x8 (&b)[kPlanes][N], s16x8 a_hi, s16x8 a_lo) {
+  f32x4 t[N];
+#pragma unroll
+  for (int j = 0; j < N; ++j) t[j] = mfma16<f16_t>(b[1][j], a_hi, f32x4{0, 0, 0, 0});
+#pragma unroll
+  for (int j = 0; j < N; ++j) t[j] = mfma16<f16_t>(b[0][j], a_lo, t[j]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) t[j] = mfma16<f16_t>(b[0][j], a_hi, t[j]);
+#pragma unroll
+  for (int j = 0; j < N; ++j) acc[j] += t[j];
+}
+
 // C = alpha A B^T + beta R + diag I on planes, all of them padded to whole tiles; last: into last's outputs instead.
 struct NsGemm {
   const f16_t *A, *B, *R;
@@ -201,17 +217,7 @@ __global__ __launch_bounds__(256 * KG) void k_ns_gemm(NsGemm g) {
         fb[p][i] = TB::frag(here + (P + p) * TA::kBytes, (wn * TT + i) * 16, 0);
       }
 #pragma unroll
-    for (int i = 0; i < TT; ++i)
-#pragma unroll
-      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[1][j], fa[0][i], acc[i][j]);
-#pragma unroll
-    for (int i = 0; i < TT; ++i)
-#pragma unroll
-      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[1][i], acc[i][j]);
-#pragma unroll
-    for (int i = 0; i < TT; ++i)
-#pragma unroll
-      for (int j = 0; j < TT; ++j) acc[i][j] = mfma16<f16_t>(fb[0][j], fa[0][i], acc[i][j]);
+    for (int i = 0; i < TT; ++i) add_products<TT>(acc[i], fb, fa[0][i], fa[1][i]);
   }
   __syncthreads();
   f32x4* sums = reinterpret_cast<f32x4*>(all) + ((kg - 1) * 4 + w) * TT * TT * 64 + l;
@@ -359,17 +365,7 @@ SGNN_DEV void small_block(f32x4 (&acc)[BI][2], const char* A, int lda, int plane
   };
   const auto multiply = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < BI; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][1][j], fa[h][0][i], acc[i][j]);
-#pragma unroll
-    for (int i = 0; i < BI; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][1][i], acc[i][j]);
-#pragma unroll
-    for (int i = 0; i < BI; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) acc[i][j] = mfma16<f16_t>(fb[h][0][j], fa[h][0][i], acc[i][j]);
+    for (int i = 0; i < BI; ++i) add_products<2>(acc[i], fb[h], fa[h][0][i], fa[h][1][i]);
   };
   // the next 32 k are read under this one's products (past the end: the last ones again)
   load(0, 0);

@@ -771,6 +771,27 @@ def test_newton_schulz_rounds_16_bit_results_once(dtype, m, n):
     assert err <= once + 2 * ns_tol(ref, torch.float32, m, n), (err, once)
 
 
+@pytest.mark.parametrize("count,m,n", [(36, 16, 1200), (10, 224, 16), (6, 30, 900), (2, 128, 2000), (1, 520, 1100)])
+def test_newton_schulz_is_as_exact_as_fp32_sums(count, m, n):
+    """fp32 matrices, long sums among them: the error is at most half as large again as that of the same formula in
+    fp32 products (operands have 22 bits here and 24 there; the sums must not lose more)."""
+    from sgnn_amd import muon
+    strong = normal((count, m, 4), 2) @ normal((count, 4, n), 3)
+    g = 0.02 * normal((count, m, n), 1) + 0.02 * strong
+    ref = torch.stack([ns64(t) for t in g])
+    x = g.mT.contiguous() if m > n else g
+    x = x / (x.square().sum((1, 2), keepdim=True).sqrt() + 1e-7)
+    a, b, c = muon.QUINTIC
+    for _ in range(5):
+        gram = x @ x.mT
+        x = a * x + (b * gram + c * (gram @ gram)) @ x
+    plain = x.mT if m > n else x
+    err = lambda t: float((t.double().cpu() - ref).norm() / ref.norm())
+    got = err(muon.newton_schulz(g.cuda()))
+    print(f"fp32 {err(plain):.2e}, here {got:.2e}")
+    assert got <= 1.5 * err(plain)
+
+
 @pytest.mark.parametrize("m,n", [(5, 9), (128, 384), (300, 64), (100, 1500), (200, 260)])
 def test_newton_schulz_without_steps_normalises(m, n):
     """x / |x| kept to 2^-21 of itself or, where it is small, 2^-34 (two fp16 planes of 2^10 x)."""
