@@ -533,7 +533,7 @@ SGNN_DEV void redo_non_finite(const GemmArgs& g, f32x4 (&acc)[TM][TN], int64_t m
 // An infinite operand gives inf - inf = NaN in its parts, and a part of 0 times infinity is one too: outputs that
 // are not finite are formed once more (redo_non_finite).
 // NST = 2 stages of LDS: the next block is split and written while this one's products run; a matrix instruction takes
-// 16 cycles, in which a wave issues three others (4096^3: 640 to 695 us, 198 to 215 TFLOP/s; 765 with one stage, where split and
+// 16 cycles, in which a wave issues three others (4096^3: 630 to 670 us, 205 to 218 TFLOP/s; 765 with one stage, where split and
 // products take turns and the two waves of a SIMD fall into step; other mixtures asked of the scheduler: 704 to 733).
 // NST = 1: half the LDS, so two workgroups per CU, one's epilogue beside the other's products: better where k is short
 // (200003 x 384 x 128, silu: 180 us against 211).
@@ -576,19 +576,24 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm32(GemmArgs g) {
       s16x8 fa[3];
 #pragma unroll
       for (int p = 0; p < 3; ++p) fa[p] = TA::frag(sa, p, (wm * TM + i) * 16);
-      // smallest products first
+      // Smallest products first, from zero, and added by the vector units: a matrix instruction drops what lies far below
+      // the sum it adds to, which took the small parts out of long sums (4096^3 of positive values: off by 1e-5, now by
+      // 1.5e-7, at 2 to 7 % more time).
+      f32x4 t[TN];
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][2], fa[0], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][2], fa[0], f32x4{0, 0, 0, 0});
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[2], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][0], fa[2], t[j]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][1], fa[1], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][1], fa[1], t[j]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][1], fa[0], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][1], fa[0], t[j]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[1], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][0], fa[1], t[j]);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma16<bf16_t>(fb[j][0], fa[0], acc[i][j]);
+      for (int j = 0; j < TN; ++j) t[j] = mfma16<bf16_t>(fb[j][0], fa[0], t[j]);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] += t[j];
     }
   };
   // As in k_gemm16: whole blocks without branches, then the partial one (or all, of an operand too narrow).

@@ -323,6 +323,27 @@ def test_linear_long_reduction(dtype):
     assert torch.equal(dx.cpu(), (dy.double() @ w.double()).to(dtype))
 
 
+@pytest.mark.parametrize("M,N,K,what", [(4096, 2048, 4096, "y"), (1000003, 64, 64, "dw"), (2048, 2048, 2048, "dx"), (20, 300, 4096, "y")])
+def test_linear_fp32_sums_of_positive_values(M, N, K, what):
+    """Products that all add up, as behind a ReLU: a sum by 32 k at a time is off by at most u of each partial sum, half
+    of the whole on the average, and 36 u within its blocks (32 products, six parts); at most 256 splits are added by
+    eights of 32."""
+    from sgnn_amd import functional
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    x, w, dy = (torch.rand(*s, generator=gen, device="cuda").requires_grad_(True) for s in ((M, K), (N, K), (M, N)))
+    y = functional.linear(x, w)
+    wide = lambda t: t.detach().double()
+    if what == "y":
+        got, ref, k = y.detach(), wide(x) @ wide(w).T.contiguous(), K
+    else:
+        got, = torch.autograd.grad(y, x if what == "dx" else w, dy.detach())
+        ref, k = (wide(dy) @ wide(w), N) if what == "dx" else (wide(dy).T.contiguous() @ wide(x), M)
+    adds = min(k / 32 / 2, k / 256 / 32 / 2 + 20) if k > 1 << 18 else k / 32 / 2
+    worst = float(((got.double() - ref).abs() / ref).max())
+    print(f"worst {worst:.2e} at {(adds + 36) * U:.2e}")
+    assert worst <= (adds + 36) * U
+
+
 def test_linear_gradient_against_differences():
     """fp32 gradients against central differences of the operator's own sum, in a direction of each input."""
     from sgnn_amd import functional
