@@ -43,6 +43,13 @@ def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def emb_ptr(weight: Optional[torch.Tensor]) -> int:
+    """The type embedding's address for the encoder kernels, which read fp32 rows."""
+    if weight is not None and not (weight.dtype == torch.float32 and weight.is_contiguous()):
+        raise ValueError(f"the particle-type embedding must be contiguous fp32, got {weight.dtype}")
+    return _ptr(weight)
+
+
 def _linears(seq: nn.Module) -> List[nn.Linear]:
     return [m for m in seq.modules() if isinstance(m, nn.Linear)]
 
@@ -339,7 +346,7 @@ def step_in(inp: StepInputs, ws: StepWorkspace, radius: float, emb_weight: Optio
     emb_dim = emb_weight.shape[1] if (use_emb and emb_weight is not None) else 0
     return _hip.SgnnStepIn(n=ws.n, T=ws.T, dim=ws.dim, ex_ptr=inp.ex_ptr.data_ptr(), n_ex=inp.n_ex,
                            radius=float(radius), K=ws.K, types=_ptr(inp.types) if use_emb else 0,
-                           emb_w=_ptr(emb_weight) if use_emb else 0, emb_dim=emb_dim, use_emb=int(use_emb),
+                           emb_w=emb_ptr(emb_weight) if use_emb else 0, emb_dim=emb_dim, use_emb=int(use_emb),
                            vel_mean=inp.vel_mean.data_ptr(), vel_std=inp.vel_std.data_ptr(),
                            acc_mean=inp.acc_mean.data_ptr(), acc_std=inp.acc_std.data_ptr(),
                            wall_max=float(radius), wall_div=1.0)
@@ -370,7 +377,7 @@ def forward_step(epd: nn.Module, emb_weight: Optional[torch.Tensor], use_emb: bo
     radius_graph(ws, pos, (T - 1) * d, T * d, inp.ex_ptr, inp.n_ex, radius)
     emb_dim = emb_weight.shape[1] if (use_emb and emb_weight is not None) else 0
     check(L.sgnn_encode_nodes(pos.data_ptr(), n, T, d, _ptr(inp.types) if use_emb else 0,
-                              _ptr(emb_weight) if use_emb else 0, emb_dim, int(use_emb),
+                              emb_ptr(emb_weight) if use_emb else 0, emb_dim, int(use_emb),
                               inp.vel_mean.data_ptr(), inp.vel_std.data_ptr(), float(radius), 1.0,
                               ctypes.byref(pk.enc_node), ctypes.byref(pk.edge[0]),
                               ws.x_a.data_ptr(), ws.u.data_ptr(), ws.v.data_ptr(), None, s),

@@ -86,7 +86,7 @@ def forward_step(gnn, emb_weight: Optional[torch.Tensor], use_emb: bool, inp: en
     emb_dim = emb_weight.shape[1] if (use_emb and emb_weight is not None) else 0
     # wall feature clamp(x + 2, 0, R_g) / R_g (multi_scale_simulator.py:193-196)
     check(L.sgnn_encode_nodes(pos.data_ptr(), n, T, d, engine._ptr(inp.types) if use_emb else 0,
-                              engine._ptr(emb_weight) if use_emb else 0, emb_dim, int(use_emb),
+                              engine.emb_ptr(emb_weight) if use_emb else 0, emb_dim, int(use_emb),
                               inp.vel_mean.data_ptr(), inp.vel_std.data_ptr(), float(grid_radius),
                               float(grid_radius), ctypes.byref(enc), ctypes.byref(edge_s[0]),
                               ws.x_a.data_ptr(), ws.u.data_ptr(), ws.v.data_ptr(), None, s),

@@ -395,7 +395,7 @@ def emb_args(inp: engine.StepInputs, emb_weight: Optional[torch.Tensor]):
     """(types, emb_w, emb_dim, use_emb) for the encoder kernels."""
     if emb_weight is None or inp.types is None:
         return 0, 0, 0, 0
-    return inp.types.data_ptr(), emb_weight.data_ptr(), int(emb_weight.shape[1]), 1
+    return inp.types.data_ptr(), engine.emb_ptr(emb_weight), int(emb_weight.shape[1]), 1
 
 
 DW1E_IN_LAYER = False  # experiment switch (tools/exp_train_ablate.py): measured slower, see DESIGN §3

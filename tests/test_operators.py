@@ -139,6 +139,20 @@ def test_muon_kernels_refuse(lib, bad):
         assert lib.sgnn_muon_apply(a["segs"], a["nseg"], a["param"], a["update"], 0.1, 0.0, None) == INVALID
 
 
+@pytest.mark.parametrize("weight", [torch.zeros(3, 9, dtype=torch.bfloat16), torch.zeros(9, 3).t()], ids=["bf16", "strided"])
+def test_fused_encoders_refuse_an_embedding_of_another_layout(weight):
+    """The encoder kernels read fp32 rows: a 16-bit embedding beside an fp32 network would be read past its end."""
+    from types import SimpleNamespace
+    from sgnn_amd import engine, training
+    t = torch.zeros(4)
+    inp = SimpleNamespace(types=torch.zeros(4, dtype=torch.int64), ex_ptr=t, n_ex=1, vel_mean=t, vel_std=t, acc_mean=t, acc_std=t)
+    with pytest.raises(ValueError, match="embedding"):
+        training.emb_args(inp, weight)
+    with pytest.raises(ValueError, match="embedding"):
+        engine.step_in(inp, SimpleNamespace(n=4, T=6, dim=2, K=20), 1.0, weight, True)
+    assert training.emb_args(inp, weight.float().contiguous())[3] == 1
+
+
 def test_optimizers_refuse_each_other_s_state():
     """A checkpoint resumed with the other optimiser: refused before anything is changed."""
     from sgnn_amd import training
