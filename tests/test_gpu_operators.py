@@ -188,7 +188,7 @@ def test_linear_against_64_bits(dtype, act, M, N, K):
 @pytest.mark.parametrize("dtype", TYPES[1:], ids=IDS[1:])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("M,N,K", [(37, 50, 70), (24, 72, 64), (130, 136, 264), (200, 328, 2056), (260, 515, 771), (3600, 72, 3600),
-                                   (72, 3600, 3600)])
+                                   (72, 3600, 3600), (20011, 40, 24), (5000, 136, 200)])
 def test_linear_gradients_are_rounded_once(dtype, act, M, N, K):
     """dz keeps h^2 of itself (two halves of h each) and 2^-36 where it is small, so a 16-bit gradient is off by its own
     rounding and what fp32 sums lose.  Slopes: (|z| + 8) 8 u as in the test above, 7.5e-8 for gelu's distribution function,
@@ -226,6 +226,26 @@ def test_linear_gradients_past_the_largest_value(dtype):
     ref = dy.double() * slope @ w.double()
     # the slope to 100 u (of the same size), on top of the rounding
     within(dx, ref.cpu(), ((half_step(dtype) + 100 * U) * ref).cpu(), "dx")
+
+
+@pytest.mark.parametrize("act", ["relu", "silu"])
+def test_linear_backward_of_very_many_columns(act):
+    """Nine million output features: more column strips than the products look through for an empty second plane.  relu:
+    whole numbers, exact; silu: dz to 2^-16 of itself, sums of 9e6 products by 32 and by splits."""
+    from sgnn_amd import functional
+    M, N, t = 2, 9_000_000, torch.bfloat16
+    x, w, dy = (whole(s, i, -1, 2, dtype=t).cuda() for i, s in enumerate([(M, 1), (N, 1), (M, N)]))
+    leaves = [x.requires_grad_(True), w.requires_grad_(True)]
+    dx, dw = torch.autograd.grad(functional.linear(*leaves, None, act), leaves, dy)
+    z = (x.detach().double() @ w.detach().double().T).requires_grad_(True)
+    slope, = torch.autograd.grad(act64(z, act).sum(), z)
+    dz = dy.double() * slope
+    for g, ref, mags in ((dx, dz @ w.detach().double(), dz.abs() @ w.detach().double().abs()),
+                         (dw, dz.T.contiguous() @ x.detach().double(), dz.abs().T.contiguous() @ x.detach().double().abs())):
+        if act == "relu":
+            assert torch.equal(g, ref.to(t))
+        else:
+            within(g, ref.cpu(), (rounded(t, ref) * 1.01 + (2.0 ** -16 + (9e6 / 256 / 32 + 60) * U) * mags).cpu(), act)
 
 
 def _linear_bwd_by_c(dy, slope, x, w):
