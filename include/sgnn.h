@@ -564,9 +564,12 @@ int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* x, i
                 int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
 /* Its backward pass from dy [M][N]: dz = dy act'(z), dx[M][K] = dz w, dw[N][K] = dz^T x, db[N] = sum_m dz
  * (all dense; NULL skips one; the residual's gradient is dy).  slope: as sgnn_linear wrote it; NULL:
- * act'(z) = 1 (SGNN_ACT_NONE).
- * 16-bit types: the two products read dz to 16 bits (bf16) or 22 (fp16); db sums the unrounded values.  M = 0 gives dw = db = 0.
+ * act'(z) = 1 (SGNN_ACT_NONE).  M = 0 gives dw = db = 0.
+ * 16-bit types: the two products read dz to 16 bits (bf16) or 22 (fp16), as two values of the type; db sums the
+ * unrounded ones.  SGNN_SLOPES_01 or-ed to dtype, here and in the query, says that every slope is 0 or 1
+ * (SGNN_ACT_RELU): dz is a value of the type then and is read as one, in half the time.
  * workspace: sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != NULL) bytes, 256-B aligned. */
+enum { SGNN_SLOPES_01 = 0x100 };
 size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope);
 int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd, const float* slope,
                     const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx, void* dw, void* db,

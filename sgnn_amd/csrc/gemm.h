@@ -14,11 +14,9 @@ struct Gemm {
   const void* A = nullptr;
   int64_t lda = 0;
   bool a_cols = false;
-  // 16-bit types with b_cols: A in two planes (ops_types.h, split2), the second lo bytes behind the first (0: one plane,
-  // as it is).  any: nany flags; where all are 0 the second plane holds zeros alone and is not read (nany = 0: it is read).
+  // 16-bit types with b_cols: half of A in two planes (ops_types.h, split2), the second lo bytes behind the first (0: one
+  // plane, A as it is).
   int64_t lo = 0;
-  const uint32_t* any = nullptr;
-  int32_t nany = 0;
   const void* B = nullptr;
   int64_t ldb = 0;
   bool b_cols = false;

@@ -25,9 +25,7 @@ struct GemmArgs {
   float* part;  // split-K partials [split][M][N] (null: one split, the epilogue in place)
   int64_t lda, ldb, ldr, ldc, M, N, K;
   int32_t act, nsplit, tiles_m, tiles_n;
-  int64_t lo;           // of A's two planes (gemm.h)
-  const uint32_t* any;
-  int32_t nany;
+  int64_t lo;  // of A's two planes (gemm.h)
 };
 
 // ----------------------------------------------------------------------------- epilogue
@@ -153,22 +151,6 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 }
 
 // ----------------------------------------------------------------------------- 16-bit operands
-// How many planes of A hold anything; `word` is LDS that nothing else uses yet.
-template <int THREADS>
-SGNN_DEV int planes_of(const GemmArgs& g, int* word) {
-  if (g.lo == 0) return 1;
-  if (g.nany == 0) return 2;
-  int any = 0;
-  for (int i = threadIdx.x; i < g.nany; i += THREADS) any |= g.any[i];
-  if (threadIdx.x == 0) *word = 0;
-  __syncthreads();
-  if (__any(any)) *word = 1;  // every lane that gets here writes the same
-  __syncthreads();
-  any = *word;
-  __syncthreads();
-  return __builtin_amdgcn_readfirstlane(any) ? 2 : 1;
-}
-
 // BM x BN outputs per workgroup, WM x WN waves.  DIRECT: both operands' lines are 16-byte aligned (and in the cols
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 // NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
@@ -197,7 +179,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
   const char* B = static_cast<const char*>(g.B);
   int first, last;
   blocks_of(g, BK, split, first, last);
-  const int planes = BCOLS ? planes_of<kThreads>(g, reinterpret_cast<int*>(lds)) : 1;
+  const int planes = BCOLS && g.lo != 0 ? 2 : 1;
 
   f32x4 acc[TM][TN];
 #pragma unroll
@@ -331,7 +313,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_gemm16(GemmArgs g) {
       }
     }
   }
-  if (BCOLS && g.lo) {  // the planes are of half of A
+  if (planes == 2) {  // of half of A
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -881,7 +863,7 @@ int gemm_run(const Gemm& g, void* workspace, size_t workspace_bytes, void* strea
   if (g.M == 0 || g.N == 0) return SGNN_OK;
   hipStream_t s = static_cast<hipStream_t>(stream);
   GemmArgs a{g.A, g.B, g.bias, g.res, g.slope, g.C, nullptr, g.lda, g.ldb, g.ldr, g.ldc, g.M, g.N, g.K,
-             g.act, 1, 0, 0, g.lo, g.any, g.nany};
+             g.act, 1, 0, 0, g.lo};
   if (rows_ok(g)) {
     with_type(g.dtype, [&](auto* t) {
       launch_rows<std::remove_pointer_t<decltype(t)>>(a, s);

@@ -26,8 +26,8 @@ struct ActCut {
   }
 };
 
-// dz = dy act'(z), for 16 bits as two planes of its half (split2; dy times a slope of up to 1.13 may leave the type's
-// range), and the column sums of this workgroup's rows: every thread over its rows in order, then the
+// dz = dy act'(z), for lo != 0 as two planes of its half, lo values apart (split2; dy times a slope of up to 1.13 may leave
+// the type's range), and the column sums of this workgroup's rows: every thread over its rows in order, then the
 // threads of one column in order.  Reads dy and the slopes, writes dz: bounded by memory (200003 x 128 fp32 52 us,
 // 5.9 TB/s; 8192 x 8192 bf16, two planes, 162 us, 4.1 TB/s -- formed inside the two products instead, dz would be computed and its
 // inputs read twice, at every tile's pace).  Slopes rather than z are kept by the forward: it has the activation's
@@ -35,9 +35,8 @@ struct ActCut {
 // 1, where fixed point of 16 bits leaves nothing of it.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, const float* slope, int64_t M, int64_t N,
-                                                      int lanes, T* dz, int64_t lo, uint32_t* any, float* partial) {
+                                                      int lanes, T* dz, int64_t lo, float* partial) {
   constexpr int V = 16 / sizeof(T);
-  bool some = false;  // a lo that is not 0
   __shared__ float sums[kThreads * V];
   const int rows = kThreads / lanes, lane = threadIdx.x % lanes, row = threadIdx.x / lanes;
   const int64_t c = ((int64_t)blockIdx.x * lanes + lane) * V;
@@ -68,17 +67,16 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
         unpack<T>(up[u], v);
         if (slope) {
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] *= sizeof(T) == 4 ? t[u][i] : 0.5f * t[u][i];
-          if constexpr (sizeof(T) == 4) {
+          for (int i = 0; i < V; ++i) v[i] *= lo ? 0.5f * t[u][i] : t[u][i];
+          if (lo == 0) {
             store_some<V>(dz + r * N + c, cnt, v);
-          } else {
+          } else if constexpr (sizeof(T) == 2) {
             float h[V], l[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
               T hi, low;
               split2(v[i], hi, low);
               h[i] = to_float(hi), l[i] = to_float(low);
-              some |= i < cnt && l[i] != 0.0f;
               v[i] *= 2.0f;
             }
             store_some<V>(dz + r * N + c, cnt, h);
@@ -89,14 +87,6 @@ __global__ __launch_bounds__(kThreads) void k_act_bwd(const T* dy, int64_t ldd, 
         for (int i = 0; i < V; ++i) s[i] += v[i];
       }
     }
-  }
-  if (any) {
-    __shared__ uint32_t found;
-    if (threadIdx.x == 0) found = 0;
-    __syncthreads();
-    if (__any(some)) found = 1;
-    __syncthreads();
-    if (threadIdx.x == 0) any[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = found;
   }
   if (!partial) return;
 #pragma unroll
@@ -146,25 +136,26 @@ Gemm wgrad(int32_t dtype, int64_t M, int64_t N, int64_t K) {  // dw[N][K] = dz^T
   return g;
 }
 
-// Workspace of the backward pass: dz (two planes of 16-bit types, and each workgroup's flag whether the second holds
-// anything), the partial sums of db, and the products' own.  relu's slopes leave the second plane empty, and a product
-// looks at the flags first; beyond kMostFlags of them it takes both planes unseen.
-constexpr int64_t kMostFlags = 4096;
+// Workspace of the backward pass: dz (two planes of 16-bit types but for slopes of 0 and 1), the partial sums of db, and
+// the products' own.
 struct BwdLayout {
-  size_t plane, flags, dz, partial, gemm, total;
-  int32_t nany;
-  BwdLayout(int32_t dtype, int64_t M, int64_t N, int64_t K, bool has_slope) {
-    const bool two = has_slope && dtype != SGNN_F32;
-    const ActCut cut(dtype_size(dtype), M, N);
+  size_t plane, dz, partial, gemm, total;
+  bool two;
+  BwdLayout(int32_t dtype, bool slopes_01, int64_t M, int64_t N, int64_t K, bool has_slope) {
+    two = has_slope && dtype != SGNN_F32 && !slopes_01;
     plane = !has_slope ? 0 : pad256(dtype_size(dtype) * (size_t)M * (size_t)N);
-    nany = two && cut.strips * cut.blocks <= kMostFlags ? (int32_t)(cut.strips * cut.blocks) : 0;
-    flags = two ? 2 * plane : plane;
-    dz = flags + pad256(sizeof(uint32_t) * (size_t)nany);
-    partial = pad256(sizeof(float) * (size_t)cut.blocks * (size_t)N);
+    dz = two ? 2 * plane : plane;
+    partial = pad256(sizeof(float) * (size_t)ActCut(dtype_size(dtype), M, N).blocks * (size_t)N);
     gemm = std::max(gemm_workspace_bytes(dgrad(dtype, M, N, K)), gemm_workspace_bytes(wgrad(dtype, M, N, K)));
     total = dz + partial + gemm;
   }
 };
+
+bool take_slopes_01(int32_t& dtype) {
+  const bool set = (dtype & SGNN_SLOPES_01) != 0;
+  dtype &= ~SGNN_SLOPES_01;
+  return set;
+}
 
 }  // namespace
 
@@ -196,30 +187,31 @@ extern "C" int sgnn_linear(int32_t dtype, int64_t M, int64_t N, int64_t K, const
 }
 
 extern "C" size_t sgnn_linear_bwd_workspace_bytes(int32_t dtype, int64_t M, int64_t N, int64_t K, int32_t has_slope) {
+  const bool slopes_01 = take_slopes_01(dtype);
   if (!sgnn::dtype_ok(dtype) || M <= 0 || N <= 0 || K < 0) return 0;
-  return BwdLayout(dtype, M, N, K, has_slope != 0).total;
+  return BwdLayout(dtype, slopes_01, M, N, K, has_slope != 0).total;
 }
 
 extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, const void* dy, int64_t ldd,
                                const float* slope, const void* x, int64_t ldx, const void* w, int64_t ldw, void* dx,
                                void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sgnn;
+  const int32_t asked = dtype;
+  const bool slopes_01 = take_slopes_01(dtype);
   if (!dtype_ok(dtype)) return set_error(SGNN_ERR_INVALID, "linear_bwd: unknown dtype");
   if (M < 0 || N < 0 || K < 0) return set_error(SGNN_ERR_INVALID, "linear_bwd: negative size");
   if (too_many(M, N, K)) return set_error(SGNN_ERR_UNSUPPORTED, "linear_bwd: more than 2^30 rows or 2^25 columns");
   if (M > 0 && N > 0 && (!dy || ldd < N)) return set_error(SGNN_ERR_INVALID, "linear_bwd: bad dy");
   if (K > 0 && ((dx && N > 0 && (!w || ldw < K)) || (dw && M > 0 && (!x || ldx < K))))
     return set_error(SGNN_ERR_INVALID, "linear_bwd: bad operand");
-  const size_t need = sgnn_linear_bwd_workspace_bytes(dtype, M, N, K, slope != nullptr);
+  const size_t need = sgnn_linear_bwd_workspace_bytes(asked, M, N, K, slope != nullptr);
   if (need > 0 && (!workspace || workspace_bytes < need))
     return set_error(SGNN_ERR_INVALID, "linear_bwd: workspace smaller than sgnn_linear_bwd_workspace_bytes");
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const BwdLayout at(dtype, M, N, K, slope != nullptr);
+  const BwdLayout at(dtype, slopes_01, M, N, K, slope != nullptr);
   char* ws = static_cast<char*>(workspace);
   const void* up = dy;      // dz and its leading dimension
   int64_t ldu = ldd, lo = 0;
-  const bool two = slope && dtype != SGNN_F32;
-  uint32_t* any = two && at.nany > 0 ? reinterpret_cast<uint32_t*>(ws + at.flags) : nullptr;
   if (N > 0 && (slope || db)) {
     with_type(dtype, [&](auto* t) {
       using T = std::remove_pointer_t<decltype(t)>;
@@ -228,8 +220,8 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
       if (M > 0) {
         hipLaunchKernelGGL(k_act_bwd<T>, dim3((unsigned)cut.strips, (unsigned)cut.blocks), dim3(kThreads), 0, s,
                            static_cast<const T*>(dy), ldd, slope, M, N, cut.lanes, reinterpret_cast<T*>(ws),
-                           (int64_t)(at.plane / sizeof(T)), any, partial);
-        if (slope) up = ws, ldu = N, lo = two ? (int64_t)at.plane : 0;
+                           at.two ? (int64_t)(at.plane / sizeof(T)) : 0, partial);
+        if (slope) up = ws, ldu = N, lo = at.two ? (int64_t)at.plane : 0;
       }
       if (db)
         hipLaunchKernelGGL(k_bias_grad<T>, dim3(sum_grid(N)), dim3(kSumThreads), 0, s, partial,
@@ -242,7 +234,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   char* gws = ws + at.dz + at.partial;
   if (dx) {
     Gemm g = dgrad(dtype, M, N, K);
-    g.A = up, g.lda = ldu, g.lo = lo, g.any = any, g.nany = at.nany;
+    g.A = up, g.lda = ldu, g.lo = lo;
     g.B = w, g.ldb = ldw;
     g.C = dx, g.ldc = K;
     const int e = gemm_run(g, gws, at.gemm, stream);
@@ -250,7 +242,7 @@ extern "C" int sgnn_linear_bwd(int32_t dtype, int64_t M, int64_t N, int64_t K, c
   }
   if (dw) {
     Gemm g = wgrad(dtype, M, N, K);
-    g.A = up, g.lda = ldu, g.lo = lo, g.any = any, g.nany = at.nany;
+    g.A = up, g.lda = ldu, g.lo = lo;
     g.B = x, g.ldb = ldx;
     g.C = dw, g.ldc = K;
     return gemm_run(g, gws, at.gemm, stream);

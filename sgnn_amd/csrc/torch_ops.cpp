@@ -176,6 +176,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
                         const MaybeTensor& maybe_res, int64_t act) {
     const Tensor bias = given(maybe_bias), res = given(maybe_res);
     ctx->saved_data["present"] = presence(x, w, bias, res);
+    ctx->saved_data["act"] = act;
     auto [y, slope] = run_linear(x, w, bias, res, act, act != SGNN_ACT_NONE);
     ctx->save_for_backward({x, w, slope});
     return y;
@@ -194,7 +195,7 @@ struct LinearNode : torch::autograd::Function<LinearNode> {
     if (needs(ctx, present, 1)) dw = at::empty({N, K}, x.options());
     if (needs(ctx, present, 2)) db = at::empty({N}, x.options());
     if (dx.defined() || dw.defined() || db.defined()) {
-      const int32_t dt = dtype_of(x);
+      const int32_t dt = dtype_of(x) | (ctx->saved_data["act"].toInt() == SGNN_ACT_RELU ? SGNN_SLOPES_01 : 0);
       const size_t nws = api.linear_bwd_bytes(dt, M, N, K, slope.defined());
       const Tensor ws = workspace(nws, x);
       check(api.linear_bwd(dt, M, N, K, ptr(dy), ld(dy), static_cast<const float*>(ptr(slope)), ptr(x), ld(x), ptr(w), ld(w), ptr(dx), ptr(dw),

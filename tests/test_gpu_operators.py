@@ -230,8 +230,7 @@ def test_linear_gradients_past_the_largest_value(dtype):
 
 @pytest.mark.parametrize("act", ["relu", "silu"])
 def test_linear_backward_of_very_many_columns(act):
-    """Nine million output features: more column strips than the products look through for an empty second plane.  relu:
-    whole numbers, exact; silu: dz to 2^-16 of itself, sums of 9e6 products by 32 and by splits."""
+    """Nine million output features (and terms of dx).  relu: whole numbers, exact; silu: dz to 2^-16 of itself, sums of 9e6 products by 32 and by splits."""
     from sgnn_amd import functional
     M, N, t = 2, 9_000_000, torch.bfloat16
     x, w, dy = (whole(s, i, -1, 2, dtype=t).cuda() for i, s in enumerate([(M, 1), (N, 1), (M, N)]))
@@ -248,10 +247,24 @@ def test_linear_backward_of_very_many_columns(act):
             within(g, ref.cpu(), (rounded(t, ref) * 1.01 + (2.0 ** -16 + (9e6 / 256 / 32 + 60) * U) * mags).cpu(), act)
 
 
-def _linear_bwd_by_c(dy, slope, x, w):
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("M,N,K", [(70, 75, 88), (300, 264, 40), (1030, 96, 384)])
+def test_linear_by_c_with_slopes_of_0_and_1(dtype, M, N, K):
+    """relu's slopes with and without SGNN_SLOPES_01: exact on whole numbers, the tiniest values among them."""
+    dy, x, w = (whole(s, i, dtype=dtype).cuda() for i, s in enumerate([(M, N), (M, K), (N, K)]))
+    slope = whole((M, N), 9, 0, 2).cuda()
+    dy[3], dy[:, 5], dy[3, 5], slope[3, 5] = 0, 0, 3 * 2.0 ** -24, 1   # alone in its sums; its half is no fp16 value
+    dz = dy.double() * slope.double()
+    want = [t.to(dtype) for t in (dz @ w.double(), dz.T.contiguous() @ x.double(), dz.sum(0))]
+    for flags in (0, 0x100):
+        for got, ref in zip(_linear_bwd_by_c(dy, slope, x, w, flags), want):
+            assert torch.equal(got, ref), flags
+
+
+def _linear_bwd_by_c(dy, slope, x, w, flags=0):
     from sgnn_amd import _hip
     L = _hip.lib()
-    (M, N), K, dt = dy.shape, x.shape[1], _hip.DTYPES[x.dtype]
+    (M, N), K, dt = dy.shape, x.shape[1], _hip.DTYPES[x.dtype] | flags
     nws = L.sgnn_linear_bwd_workspace_bytes(dt, M, N, K, int(slope is not None))
     ws = torch.empty(nws, dtype=torch.uint8, device="cuda")
     dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty(N, dtype=x.dtype, device="cuda")

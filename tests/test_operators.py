@@ -57,6 +57,15 @@ def test_linear_bwd_refuses(lib, bad):
     assert "linear_bwd" in lib.sgnn_last_error().decode()
 
 
+def test_linear_bwd_workspace_of_slopes_of_0_and_1(lib):
+    """SGNN_SLOPES_01: one plane of dz instead of two for the 16-bit types, nothing else; no other bit passes."""
+    size = lambda dtype: lib.sgnn_linear_bwd_workspace_bytes(dtype, 1000, 512, 64, 1)
+    for dtype in (1, 2):
+        assert size(dtype) - size(dtype | 0x100) == 1000 * 512 * 2
+    assert size(0) == size(0x100) > 0 and size(1 | 0x200) == 0
+    assert _linear_bwd(lib, dtype=1 | 0x200) == INVALID and _linear_bwd(lib, dtype=3 | 0x100) == INVALID
+
+
 @pytest.mark.parametrize("dtype", [0, 1, 2])
 @pytest.mark.parametrize("M", [0, 4])
 @pytest.mark.parametrize("slope", [None, P])
