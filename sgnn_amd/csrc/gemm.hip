@@ -155,8 +155,8 @@ SGNN_DEV void blocks_of(const GemmArgs& g, int bk, int split, int& first, int& l
 // layout a multiple of 8 rows): LDS is filled without passing registers but for the last, partial block of k.
 // NST stages of LDS: NST - 1 blocks are under way while one is worked on.  Two suffice where a block's products take
 // longer than memory; the small tile has four.
-// 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 307
-// to 330 us, dy w 230 to 260, dy^T x 234 to 260; with two planes of dz 437 to 480 and 451 to 496.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
+// 8192 x 8192 x 2048 in bf16 (275 GFLOP; the library's products take 187 to 230 us): x w^T with gelu and its slopes 290
+// to 330 us, dy w 230 to 260, dy^T x 234 to 260; with two planes of dz 409 to 480 and 403 to 496.  No bank conflicts are left; the matrix units are busy 50 to 60 % of the
 // time, and the rest is LDS's latency after each block's barrier, which all waves meet together, and, forward, the
 // epilogue's 402 MB.  Memory is not waited for: four stages of 32 k took 334 / 248 / 244 us at their fastest, where these
 // two of 64 k took 290 / 230 / 230; the next block's loads issued behind the first fragments' reads took 292 / 226 / 237.

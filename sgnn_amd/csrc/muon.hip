@@ -5,7 +5,7 @@
 // that all of them fit: 22 bits of every value that is not tiny against 1 and an absolute 2^-35 below that.  Products
 // are hi hi + hi lo + lo hi, good to 2^-22, below what an fp32 sum of some hundred products loses, and a I inside Q
 // keeps the sum a X + (b G + c G^2) X, whose terms cancel to a fifth near 1, out of the rounding.  This holds for every
-// type of matrix: with the hi plane alone bf16 ones took 537 us instead of 1244 (4096 x 2048), but fifteen roundings to
+// type of matrix: with the hi plane alone bf16 ones took 537 us instead of 1250 to 1380 (4096 x 2048), but fifteen roundings to
 // 11 bits come out beside the one of the result (error 0.0028 instead of 0.0017 for a small matrix).  The planes are
 // padded with zeros to whole tiles (zeros stay zeros under the steps), so nothing is checked inside the products; the
 // last one writes the caller's type from its fp32 sums.
@@ -152,8 +152,8 @@ struct NsGemm {
 // KG groups of four waves take every KG-th block of k each, with LDS of their own, and are added in order at the end:
 // these products have few tiles (36 of 128 x 128 in the triangle of 1024), and one wave per SIMD leaves memory's and
 // LDS's latencies in the open.  One group instead of two, all five steps in us: 1024 x 1024 301 / 225, 2048 x 4096
-// 1507 / 1228, 4096 x 4096 5253 / 4646; two of 2048 x 4096 2379 / 2420.  2048 x 4096: X X^T 82 to 87 us
-// (136 tiles of 256 CUs; three times 18 GFLOP formed), G^2 54 to 57, Q X 107 to 113 (three times 34 GFLOP, 910 to 960
+// 1507 / 1228, 4096 x 4096 5253 / 4646; two of 2048 x 4096 2379 / 2420.  2048 x 4096: X X^T 87 to 98 us
+// (136 tiles of 256 CUs; three times 18 GFLOP formed), G^2 55 to 60, Q X 107 to 116 (three times 34 GFLOP, 890 to 960
 // TFLOP/s): bounded by the CUs without a tile and by LDS reads beside the matrix instructions.
 constexpr int KG = 2;
 template <bool AC, bool BC, int BT, bool SYM>
@@ -314,7 +314,7 @@ void launch_gemm(const NsGemm& g, int bt, int count, hipStream_t s) {
 // m <= n in whole 32s, zeros in the padding.  A tall matrix is laid down transposed.  Each wave has up to NB times
 // 32 x 32 of a product in registers, in blocks of 16 BI x 32; G and X are read along k from their rows, X as the second factor transposed
 // (ds_read_b64_tr_b16).  One launch instead of 2 + 3 per step, whose latency is all a small matrix costs: 64 x 64 fp32
-// 20 us against 60 by tiles; bounded by the chain of LDS reads, matrix instructions and barriers, about 3.5 us a step.
+// 22 us against 60 by tiles; bounded by the chain of LDS reads, matrix instructions and barriers, about 4 us a step.
 constexpr int kMaxSmall = 48, kSmallThreads = 512, kSmallWaves = kSmallThreads / 64, kMaxLds = 160 * 1024 - 256;
 struct SmallArgs {
   sgnn_matrix mats[kMaxSmall];
